@@ -1,0 +1,529 @@
+// Shared parts of the paged KV-cache kernels: the view of cache and batch that
+// kernels take, host checks, TMA maps over pages, bounded barrier waits, and
+// the division of ragged attention work over a persistent grid.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+
+#include <cstring>
+#include <mutex>
+
+#include "common.cuh"
+#include "jfb/jfb_paged.h"
+
+namespace jfb {
+namespace paged {
+
+constexpr int kTileKeys = 128;  // keys of one tile of work
+
+// ---- kernel view ----------------------------------------------------------------
+
+struct View {
+    const int32_t * q_start;
+    const int32_t * kv_len;
+    const int32_t * table;
+    uint64_t table_stride;
+    uint64_t page_stride, token_stride, head_stride;  // elements
+    uint32_t sequences, table_width;
+    uint32_t pages, page_size, page_shift;
+    uint32_t kv_heads, head_dim;
+    uint32_t rows;  // rows of the call's row arrays
+    int32_t * error;
+};
+
+__device__ __forceinline__ void flag_error(int32_t * error, int32_t bit) {
+    if (error != nullptr) atomicOr(error, bit);
+}
+
+// Rows [q0, q0 + count) and keys kv of one sequence, cut to the call's arrays.
+struct Sequence {
+    uint32_t q0, count, kv;
+};
+
+__device__ __forceinline__ uint32_t cut_length(const View & v, int32_t len, bool & bad) {
+    const uint64_t cap = uint64_t(v.table_width) * v.page_size;
+    if (len < 0) bad = true;
+    const uint32_t n = len < 0 ? 0u : uint32_t(len);
+    if (n > cap) bad = true;
+    return n > cap ? uint32_t(cap) : n;
+}
+
+__device__ __forceinline__ Sequence load_sequence(const View & v, uint32_t b) {
+    const int32_t a = v.q_start[b], e = v.q_start[b + 1];
+    bool bad = false;
+    Sequence s;
+    s.kv = cut_length(v, v.kv_len[b], bad);
+    if (a < 0 || e < a || uint32_t(e) > v.rows) {
+        bad = true;
+        s.q0 = s.count = 0;
+    } else {
+        s.q0 = uint32_t(a);
+        s.count = uint32_t(e - a);
+    }
+    if (bad) flag_error(v.error, JFB_PAGED_ERROR_RANGE);
+    return s;
+}
+
+// ---- mbarriers and TMA -----------------------------------------------------------
+
+constexpr uint64_t kWaitNs = 2000000000ull;  // bound of every wait
+constexpr uint32_t kSuspendNs = 1000000;
+
+__device__ __forceinline__ uint32_t smem_u32(const void * p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ uint64_t global_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+__device__ __forceinline__ void mbar_init(uint64_t * bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+
+__device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+
+__device__ __forceinline__ void mbar_arrive(uint64_t * bar) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t * bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+                 "r"(bytes)
+                 : "memory");
+}
+
+__device__ __forceinline__ bool mbar_try_wait(uint64_t * bar, uint32_t parity, uint32_t hint_ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns)
+        : "memory");
+    return ok != 0;
+}
+
+// False when the phase has not completed within kWaitNs (recorded in *error)
+// or another thread of the CTA has given up.
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        if (mbar_try_wait(bar, parity, kSuspendNs)) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitNs) break;
+    }
+    *abort_flag = 1;
+    flag_error(error, JFB_PAGED_ERROR_TIMEOUT);
+    return false;
+}
+
+__device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0 || mbar_wait_slow(bar, parity, abort_flag, error);
+}
+
+// After an abort: waits (bounded by itself) for a copy in flight.
+static __device__ __noinline__ void mbar_drain(uint64_t * bar, uint32_t parity) {
+    const uint64_t t0 = global_ns();
+    while (!mbar_try_wait(bar, parity, kSuspendNs) && global_ns() - t0 < kWaitNs) {}
+}
+
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Box (64 elements, up to 128 tokens) of one page and head (no multicast);
+// x is 0 or 64 elements: 16-byte aligned.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap * map, int32_t x, int32_t token, int32_t head,
+                                              int32_t page, uint64_t * bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(token), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Bytes of a tile of kTileKeys keys of D elements, stored as D / 64 halves of
+// [key][64] in the 128-byte swizzle (16-byte chunk c of key r at c ^ (r % 8)).
+template <int D>
+constexpr uint32_t kTileBytes = kTileKeys * D * 2;
+
+// The calling warp loads the pages of keys [key0, key1) (key1 - key0 <= 128,
+// key0 a multiple of min(page_size, 128)) of one sequence and kv head. Every
+// lane fetches one page's id and issues its boxes; lane 0 announces the bytes
+// first. Ids outside the pool are turned into one that reads as zeros: the
+// tensor map fills coordinates outside the pool.
+template <int D>
+__device__ __forceinline__ void load_tile(const View & v, const CUtensorMap * map, const int32_t * row, uint32_t head,
+                                          uint32_t key0, uint32_t key1, uint32_t dst, uint64_t * bar) {
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t step = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
+    const uint32_t boxes = (key1 - key0 + step - 1) / step;
+    int32_t page = 0;
+    const uint32_t key = key0 + lane * step;
+    if (lane < boxes) {
+        page = row[key >> v.page_shift];
+        if (page < 0 || uint32_t(page) >= v.pages) {
+            flag_error(v.error, JFB_PAGED_ERROR_RANGE);
+            page = int32_t(v.pages);
+        }
+    }
+    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * step * D * 2);
+    __syncwarp();
+    if (lane < boxes) {
+        const uint32_t to = dst + lane * step * 128;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+            tma_load_page(to + h * (kTileKeys * 128), map, h * 64, int32_t(key & (v.page_size - 1)), int32_t(head), page, bar);
+        }
+    }
+    __syncwarp();
+}
+
+// ---- division of the attention work ------------------------------------------------
+//
+// The (row, head of the group) pairs of one sequence and kv head are packed
+// into rows i * G + g and cut into row tiles of M; an item is one (kv head,
+// sequence, row tile), its units the key tiles that any of its rows sees (one
+// for an item that sees none, which then writes zeros). The units of all
+// items, kv head outermost, form one line that the persistent CTAs divide
+// evenly, so long contexts are split, short ones gathered and causal tiles
+// balanced by the same rule from lengths that only the device knows. The
+// parts of an item that spans CTAs are joined in CTA order by the last one
+// to arrive.
+
+struct KeyRange {
+    uint32_t lo, hi;   // keys [lo, hi) are seen by some row of the tile
+    uint32_t begin;    // first tile's first key: lo rounded down to a box
+    uint32_t units;    // max(1, tiles of [begin, hi))
+};
+
+template <int M>
+__device__ __forceinline__ uint32_t row_tiles(const Sequence & s, uint32_t group) {
+    return uint32_t((uint64_t(s.count) * group + M - 1) / M);
+}
+
+template <int M>
+__device__ __forceinline__ KeyRange key_range(const View & v, const Sequence & s, uint32_t group, uint32_t window,
+                                              uint32_t tile) {
+    const uint64_t packed = uint64_t(s.count) * group;
+    const uint64_t r0 = uint64_t(tile) * M;
+    const uint64_t r1 = (r0 + M < packed ? r0 + M : packed) - 1;
+    const int64_t first = int64_t(s.kv) - s.count;
+    const int64_t p0 = first + int64_t(r0 / group), p1 = first + int64_t(r1 / group);
+    KeyRange k;
+    k.hi = p1 < 0 ? 0u : uint32_t(p1 + 1);
+    k.lo = window > 0 && p0 >= int64_t(window) ? uint32_t(p0 - window + 1) : 0u;
+    const uint32_t box = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
+    k.begin = k.lo & ~(box - 1);
+    const uint32_t tiles = k.hi > k.begin ? (k.hi - k.begin + kTileKeys - 1) / kTileKeys : 0u;
+    k.units = tiles > 0 ? tiles : 1u;
+    return k;
+}
+
+struct Walk {
+    uint64_t unit, end;    // this CTA's line segment still to do
+    uint64_t item0;        // first unit of the current item
+    uint64_t total;        // units in all
+    uint32_t ctas;         // CTAs that have work
+    uint32_t kv_head, b, tile;
+    Sequence s;
+    KeyRange k;
+};
+
+// The CTA that holds `unit`.
+__device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t total, uint64_t ctas) {
+    return uint32_t(((unit + 1) * ctas - 1) / total);
+}
+
+// Positions every thread of the CTA at its first item. `cost` is shared
+// scratch of one u64 per sequence, `out` one Walk in shared memory; both may
+// be reused after the call. False when the CTA has no work.
+template <int M>
+static __device__ bool walk_begin(const View & v, uint32_t group, uint32_t window, uint64_t * cost, Walk * out, Walk & w) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    // units of each sequence: a thread per sequence; the lanes of the warp
+    // share the row tiles of a sequence that has many
+    for (uint32_t base = warp * 32; base < v.sequences; base += warps * 32) {
+        const uint32_t b = base + lane;
+        Sequence s = {0, 0, 0};
+        uint32_t tiles = 0;
+        uint64_t units = 0;
+        if (b < v.sequences) {
+            s = load_sequence(v, b);
+            tiles = row_tiles<M>(s, group);
+            if (tiles <= 4) {
+                for (uint32_t t = 0; t < tiles; ++t) units += key_range<M>(v, s, group, window, t).units;
+            }
+        }
+        uint32_t many = __ballot_sync(0xffffffffu, tiles > 4);
+        while (many != 0) {
+            const int src = __ffs(many) - 1;
+            many &= many - 1;
+            Sequence o;
+            o.q0 = 0;
+            o.count = __shfl_sync(0xffffffffu, s.count, src);
+            o.kv = __shfl_sync(0xffffffffu, s.kv, src);
+            const uint32_t n = __shfl_sync(0xffffffffu, tiles, src);
+            unsigned long long sum = 0;
+            for (uint32_t t = lane; t < n; t += 32) sum += key_range<M>(v, o, group, window, t).units;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (int(lane) == src) units = sum;
+        }
+        if (b < v.sequences) cost[b] = units;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        unsigned long long per_head = 0;
+        for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
+        Walk x;
+        x.total = uint64_t(per_head) * v.kv_heads;
+        x.ctas = uint64_t(gridDim.x) < x.total ? gridDim.x : uint32_t(x.total);
+        const bool work = blockIdx.x < x.ctas;
+        if (work) {
+            x.unit = uint64_t(blockIdx.x) * x.total / x.ctas;
+            x.end = uint64_t(blockIdx.x + 1) * x.total / x.ctas;
+            x.kv_head = uint32_t(x.unit / per_head);
+            unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;  // within the head's line
+            // the sequence: 32 prefix sums at a time
+            uint32_t b = 0;
+            for (uint32_t base = 0; base < v.sequences; base += 32) {
+                const unsigned long long mine = base + lane < v.sequences ? cost[base + lane] : 0ull;
+                unsigned long long upto = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (int(lane) >= d) upto += o;
+                }
+                const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
+                if (over != 0) {
+                    const int src = __ffs(over) - 1;
+                    b = base + src;
+                    left -= __shfl_sync(0xffffffffu, upto - mine, src);
+                    break;
+                }
+                left -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+            x.b = b;
+            x.s = load_sequence(v, b);
+            // the row tile, the same way
+            const uint32_t tiles = row_tiles<M>(x.s, group);
+            x.tile = 0;
+            for (uint32_t base = 0; base < tiles; base += 32) {
+                const unsigned long long mine =
+                    base + lane < tiles ? key_range<M>(v, x.s, group, window, base + lane).units : 0ull;
+                unsigned long long upto = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (int(lane) >= d) upto += o;
+                }
+                const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
+                if (over != 0) {
+                    const int src = __ffs(over) - 1;
+                    x.tile = base + src;
+                    left -= __shfl_sync(0xffffffffu, upto - mine, src);
+                    break;
+                }
+                left -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+            x.item0 = x.unit - left;
+            x.k = key_range<M>(v, x.s, group, window, x.tile);
+        } else {
+            x.unit = x.end = 0;
+        }
+        if (lane == 0) *out = x;
+    }
+    __syncthreads();
+    w = *out;
+    __syncthreads();
+    return w.unit < w.end;
+}
+
+// Key tiles [t0, t1) of the current item that this CTA does.
+__device__ __forceinline__ void walk_segment(const Walk & w, uint32_t & t0, uint32_t & t1) {
+    t0 = uint32_t(w.unit - w.item0);
+    const uint64_t left = w.end - w.unit;
+    t1 = left < w.k.units - t0 ? t0 + uint32_t(left) : w.k.units;
+}
+
+// Moves past the current segment; false at the end of the CTA's line.
+template <int M>
+__device__ __forceinline__ bool walk_next(const View & v, uint32_t group, uint32_t window, Walk & w) {
+    const uint64_t item_end = w.item0 + w.k.units;
+    w.unit = item_end < w.end ? item_end : w.end;
+    if (w.unit >= w.end) return false;
+    w.item0 = w.unit;
+    ++w.tile;
+    while (w.tile >= row_tiles<M>(w.s, group)) {
+        w.tile = 0;
+        if (++w.b >= v.sequences) {
+            w.b = 0;
+            ++w.kv_head;
+        }
+        w.s = load_sequence(v, w.b);
+    }
+    w.k = key_range<M>(v, w.s, group, window, w.tile);
+    return true;
+}
+
+// ---- number types -------------------------------------------------------------------
+
+template <typename T>
+struct Num;
+template <>
+struct Num<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2 *>(&u)); }
+};
+template <>
+struct Num<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) {
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// ---- host side ------------------------------------------------------------------------
+
+inline jfb_status check_cache(const jfb_paged_cache * c) {
+    if (c == nullptr || c->k == nullptr || c->v == nullptr) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged cache pools are required");
+    }
+    if (c->dtype != JFB_DTYPE_F16 && c->dtype != JFB_DTYPE_BF16) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged cache dtype must be F16 or BF16");
+    }
+    if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "page_size %u is not a power of two from 8 to 1024", c->page_size);
+    }
+    if (c->head_dim < 8 || c->head_dim > 128 || c->head_dim % 8 != 0) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged head_dim %u is not a multiple of 8 up to 128", c->head_dim);
+    }
+    if (c->pages == 0 || c->pages > 0x7fffffffu || c->kv_heads == 0 || c->kv_heads > 65535u) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged cache needs pages and kv heads");
+    }
+    const uint64_t strides[3] = {c->page_stride, c->token_stride, c->head_stride};
+    for (uint64_t s : strides) {
+        if (s == 0 || s % 8 != 0 || s >= (1ull << 39)) {
+            return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged cache strides must be positive multiples of 8 elements");
+        }
+    }
+    if (c->token_stride < c->head_dim || c->head_stride < c->head_dim || c->page_stride < c->head_dim) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged cache strides make elements share addresses");
+    }
+    if ((reinterpret_cast<uintptr_t>(c->k) & 15u) != 0 || (reinterpret_cast<uintptr_t>(c->v) & 15u) != 0) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged cache pools must be 16-byte aligned");
+    }
+    return status_ok();
+}
+
+inline jfb_status check_batch(const jfb_paged_batch * b, bool rows) {
+    if (b == nullptr || (rows && b->q_start == nullptr) || b->kv_len == nullptr || b->page_table == nullptr) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged batch arrays are required");
+    }
+    if (b->sequences > JFB_PAGED_MAX_SEQUENCES) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "a paged call takes at most %d sequences", JFB_PAGED_MAX_SEQUENCES);
+    }
+    if (b->table_width == 0 || b->table_stride < b->table_width) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "page_table rows hold %u of a stride of %llu", b->table_width,
+                            static_cast<unsigned long long>(b->table_stride));
+    }
+    return status_ok();
+}
+
+inline View make_view(const jfb_paged_cache & c, const jfb_paged_batch & b, uint32_t rows, int32_t * error) {
+    View v;
+    v.q_start = b.q_start;
+    v.kv_len = b.kv_len;
+    v.table = b.page_table;
+    v.table_stride = b.table_stride;
+    v.page_stride = c.page_stride;
+    v.token_stride = c.token_stride;
+    v.head_stride = c.head_stride;
+    v.sequences = b.sequences;
+    v.table_width = b.table_width;
+    v.pages = c.pages;
+    v.page_size = c.page_size;
+    v.page_shift = uint32_t(__builtin_ctz(c.page_size));
+    v.kv_heads = c.kv_heads;
+    v.head_dim = c.head_dim;
+    v.rows = rows;
+    v.error = error;
+    return v;
+}
+
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void * f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess) {
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+        }
+    });
+    return fn;
+}
+
+// Pool as (head_dim, token, head, page): boxes of 64 elements x min(page_size,
+// 128) tokens in the 128-byte swizzle; elements beyond head_dim and pages
+// beyond the pool read as zeros.
+inline bool pool_map(CUtensorMap & map, const void * pool, const jfb_paged_cache & c) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[4] = {c.head_dim, c.page_size, c.kv_heads, c.pages};
+    const cuuint64_t strides[3] = {c.token_stride * 2, c.head_stride * 2, c.page_stride * 2};
+    const cuuint32_t box[4] = {64, c.page_size < uint32_t(kTileKeys) ? c.page_size : uint32_t(kTileKeys), 1, 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    std::memset(&map, 0, sizeof(map));
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(pool), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// SMs of the current device.
+inline uint32_t device_sms() {
+    int device = 0, n = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+    return n > 0 ? uint32_t(n) : 0u;
+}
+
+// Largest dynamic shared memory of a kernel, set once per device.
+template <typename K>
+inline cudaError_t allow_smem(K kernel, uint32_t bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+}
+
+}  // namespace paged
+}  // namespace jfb
