@@ -111,7 +111,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t * bar, uint32_t parity, u
 
 // False when the phase has not completed within kWaitNs (recorded in *error)
 // or another thread of the CTA has given up.
-static __device__ __noinline__ bool mbar_wait_slow(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
+__device__ __forceinline__ bool mbar_wait_slow(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
     const uint64_t t0 = global_ns();
     for (;;) {
         if (mbar_try_wait(bar, parity, kSuspendNs)) return true;
@@ -136,7 +136,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volat
 }
 
 // After an abort: waits (bounded by itself) for a copy in flight.
-static __device__ __noinline__ void mbar_drain(uint64_t * bar, uint32_t parity) {
+__device__ __forceinline__ void mbar_drain(uint64_t * bar, uint32_t parity) {
     const uint64_t t0 = global_ns();
     while (!mbar_try_wait(bar, parity, kSuspendNs) && global_ns() - t0 < kWaitNs) {}
 }

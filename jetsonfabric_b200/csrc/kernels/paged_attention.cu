@@ -377,7 +377,7 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a positive finite scale and a window below 2^31");
     }
     const uint32_t sms = device_sms();
-    if (sms == 0 || sms * sizeof(uint32_t) > kCounterBytes) {
+    if (sms == 0 || sms * 2 * sizeof(uint32_t) > kCounterBytes) {
         return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: no usable device");
     }
     const uint64_t need = kCounterBytes + uint64_t(sms) * 2 * kSlotFloats * sizeof(float);
@@ -405,6 +405,7 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     }
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
+    if (uint64_t(rows) * p.group > 32ull * batch->sequences) return launch_attention_tc(half, cache->head_dim, mk, mv, p, sms, s);
     if (cache->head_dim <= 64) {
         return half ? launch_rows<__half, 64>(mk, mv, p, sms, s) : launch_rows<__nv_bfloat16, 64>(mk, mv, p, sms, s);
     }

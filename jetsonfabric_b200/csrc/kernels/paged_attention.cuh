@@ -7,8 +7,8 @@
 namespace jfb {
 namespace paged {
 
-// Workspace: one arrival counter per CTA (an item split over CTAs counts at
-// its first one), then two slots per CTA for the parts of the items that
+// Workspace: two arrival counters per CTA (an item split over CTAs counts at
+// its first one, in the tcgen05 kernel per row tile), then two slots per CTA for the parts of the items that
 // begin before it and that end behind it: [256 rows][128] sums and [256]
 // (maximum, sum), f32.
 constexpr uint64_t kCounterBytes = 4096;
@@ -65,6 +65,10 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+// The tcgen05 kernel of paged_attention_tc.cu.
+jfb_status launch_attention_tc(bool half, uint32_t head_dim, const CUtensorMap & k, const CUtensorMap & v, const AttentionParams & p,
+                               uint32_t sms, cudaStream_t s);
 
 // Query-shaped rows [rows][heads x head_dim] of 16-bit numbers.
 inline jfb_status check_rows(const char * what, const void * x, uint64_t stride, uint32_t rows, uint32_t heads,
