@@ -29,7 +29,10 @@ struct View {
     uint32_t sequences, table_width;
     uint32_t pages, page_size, page_shift;
     uint32_t kv_heads, head_dim;
-    uint32_t rows;  // rows of the call's row arrays
+    uint32_t rows;       // rows of the call's row arrays
+    uint32_t group;      // query heads per kv head
+    uint32_t window;     // 0: none
+    uint32_t item_rows;  // packed rows of one item of the attention work
     int32_t * error;
 };
 
@@ -110,8 +113,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t * bar, uint32_t parity, u
 }
 
 // False when the phase has not completed within kWaitNs (recorded in *error)
-// or another thread of the CTA has given up.
-__device__ __forceinline__ bool mbar_wait_slow(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
+// or another thread of the CTA has given up. Waiting threads are suspended:
+// spinning ones would take issue slots from the others.
+__device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
+    if (mbar_try_wait(bar, parity, kSuspendNs)) return true;
     const uint64_t t0 = global_ns();
     for (;;) {
         if (mbar_try_wait(bar, parity, kSuspendNs)) return true;
@@ -121,18 +126,6 @@ __device__ __forceinline__ bool mbar_wait_slow(uint64_t * bar, uint32_t parity, 
     *abort_flag = 1;
     flag_error(error, JFB_PAGED_ERROR_TIMEOUT);
     return false;
-}
-
-__device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0 || mbar_wait_slow(bar, parity, abort_flag, error);
 }
 
 // After an abort: waits (bounded by itself) for a copy in flight.
@@ -154,38 +147,61 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap * 
         : "memory");
 }
 
+// Box (64 elements, heads, rows) of query rows (no multicast); x as above.
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap * map, int32_t x, int32_t head, int32_t row,
+                                              uint64_t * bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // Bytes of a tile of kTileKeys keys of D elements, stored as D / 64 halves of
 // [key][64] in the 128-byte swizzle (16-byte chunk c of key r at c ^ (r % 8)).
 template <int D>
 constexpr uint32_t kTileBytes = kTileKeys * D * 2;
 
-// The calling warp loads the pages of keys [key0, key1) (key1 - key0 <= 128,
-// key0 a multiple of min(page_size, 128)) of one sequence and kv head. Every
-// lane fetches one page's id and issues its boxes; lane 0 announces the bytes
-// first. Ids outside the pool are turned into one that reads as zeros: the
-// tensor map fills coordinates outside the pool.
-template <int D>
-__device__ __forceinline__ void load_tile(const View & v, const CUtensorMap * map, const int32_t * row, uint32_t head,
-                                          uint32_t key0, uint32_t key1, uint32_t dst, uint64_t * bar) {
+// A tile's load by one warp, a box (a page, or 128 keys of a larger one) per
+// lane, in two steps: the page ids are fetched while the tile's place in the
+// ring is still in use, their latency being most of the way to issuing.
+struct TileLoad {
+    int32_t page;      // of this lane's box
+    uint32_t token;    // its first token within the page
+    uint32_t boxes, step;
+};
+
+// Boxes of keys [key0, key1) (at most 128, key0 a multiple of the box) of the
+// sequence whose table row is `row`. A page id outside the pool becomes one
+// that reads as zeros: the tensor map fills coordinates outside the pool.
+__device__ __forceinline__ TileLoad tile_pages(const View & v, const int32_t * row, uint32_t key0, uint32_t key1) {
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t step = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
-    const uint32_t boxes = (key1 - key0 + step - 1) / step;
-    int32_t page = 0;
-    const uint32_t key = key0 + lane * step;
-    if (lane < boxes) {
-        page = row[key >> v.page_shift];
-        if (page < 0 || uint32_t(page) >= v.pages) {
+    TileLoad l;
+    l.step = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
+    l.boxes = (key1 - key0 + l.step - 1) / l.step;
+    const uint32_t key = key0 + lane * l.step;
+    l.token = key & (v.page_size - 1);
+    l.page = 0;
+    if (lane < l.boxes) {
+        l.page = row[key >> v.page_shift];
+        if (l.page < 0 || uint32_t(l.page) >= v.pages) {
             flag_error(v.error, JFB_PAGED_ERROR_RANGE);
-            page = int32_t(v.pages);
+            l.page = int32_t(v.pages);
         }
     }
-    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * step * D * 2);
+    return l;
+}
+
+// Lane 0 announces the bytes, then every lane issues its boxes.
+template <int D>
+__device__ __forceinline__ void tile_issue(const TileLoad & l, const CUtensorMap * map, uint32_t head, uint32_t dst, uint64_t * bar) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (lane == 0) mbar_arrive_expect_tx(bar, l.boxes * l.step * D * 2);
     __syncwarp();
-    if (lane < boxes) {
-        const uint32_t to = dst + lane * step * 128;
+    if (lane < l.boxes) {
+        const uint32_t to = dst + lane * l.step * 128;
 #pragma unroll
         for (int h = 0; h < D / 64; ++h) {
-            tma_load_page(to + h * (kTileKeys * 128), map, h * 64, int32_t(key & (v.page_size - 1)), int32_t(head), page, bar);
+            tma_load_page(to + h * (kTileKeys * 128), map, h * 64, int32_t(l.token), int32_t(head), l.page, bar);
         }
     }
     __syncwarp();
@@ -194,41 +210,37 @@ __device__ __forceinline__ void load_tile(const View & v, const CUtensorMap * ma
 // ---- division of the attention work ------------------------------------------------
 //
 // The (row, head of the group) pairs of one sequence and kv head are packed
-// into rows i * G + g and cut into row tiles of M; an item is one (kv head,
-// sequence, row tile), its units the key tiles that any of its rows sees (one
-// for an item that sees none, which then writes zeros). The units of all
-// items, kv head outermost, form one line that the persistent CTAs divide
-// evenly, so long contexts are split, short ones gathered and causal tiles
-// balanced by the same rule from lengths that only the device knows. The
-// parts of an item that spans CTAs are joined in CTA order by the last one
-// to arrive.
+// into rows i * G + g and cut into row tiles of item_rows; an item is one (kv head,
+// sequence, row tile) with the key tiles that any of its rows sees (one for an
+// item that sees none, which then writes zeros). It takes E units for its
+// start and end and one per key tile. The units of all items, kv head
+// outermost, form one line that the persistent CTAs divide evenly, so long
+// contexts are split, short ones gathered and causal tiles balanced by the
+// same rule from lengths that only the device knows. The parts of an item that
+// spans CTAs are joined in CTA order by the last one to arrive.
 
 struct KeyRange {
     uint32_t lo, hi;   // keys [lo, hi) are seen by some row of the tile
     uint32_t begin;    // first tile's first key: lo rounded down to a box
-    uint32_t units;    // max(1, tiles of [begin, hi))
+    uint32_t tiles;    // max(1, tiles of [begin, hi))
 };
 
-template <int M>
-__device__ __forceinline__ uint32_t row_tiles(const Sequence & s, uint32_t group) {
-    return uint32_t((uint64_t(s.count) * group + M - 1) / M);
+__device__ __forceinline__ uint32_t row_tiles(const View & v, const Sequence & s) {
+    return uint32_t((uint64_t(s.count) * v.group + v.item_rows - 1) / v.item_rows);
 }
 
-template <int M>
-__device__ __forceinline__ KeyRange key_range(const View & v, const Sequence & s, uint32_t group, uint32_t window,
-                                              uint32_t tile) {
-    const uint64_t packed = uint64_t(s.count) * group;
-    const uint64_t r0 = uint64_t(tile) * M;
-    const uint64_t r1 = (r0 + M < packed ? r0 + M : packed) - 1;
+__device__ __forceinline__ KeyRange key_range(const View & v, const Sequence & s, uint32_t tile) {
+    const uint64_t packed = uint64_t(s.count) * v.group;
+    const uint64_t r0 = uint64_t(tile) * v.item_rows;
+    const uint64_t r1 = (r0 + v.item_rows < packed ? r0 + v.item_rows : packed) - 1;
     const int64_t first = int64_t(s.kv) - s.count;
-    const int64_t p0 = first + int64_t(r0 / group), p1 = first + int64_t(r1 / group);
+    const int64_t p0 = first + int64_t(uint32_t(r0) / v.group), p1 = first + int64_t(uint32_t(r1) / v.group);
     KeyRange k;
     k.hi = p1 < 0 ? 0u : uint32_t(p1 + 1);
-    k.lo = window > 0 && p0 >= int64_t(window) ? uint32_t(p0 - window + 1) : 0u;
+    k.lo = v.window > 0 && p0 >= int64_t(v.window) ? uint32_t(p0 - v.window + 1) : 0u;
     const uint32_t box = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
     k.begin = k.lo & ~(box - 1);
-    const uint32_t tiles = k.hi > k.begin ? (k.hi - k.begin + kTileKeys - 1) / kTileKeys : 0u;
-    k.units = tiles > 0 ? tiles : 1u;
+    k.tiles = k.hi > k.begin ? (k.hi - k.begin + kTileKeys - 1) / kTileKeys : 1u;
     return k;
 }
 
@@ -247,11 +259,56 @@ __device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t total, uint64
     return uint32_t(((unit + 1) * ctas - 1) / total);
 }
 
-// Positions every thread of the CTA at its first item. `cost` is shared
-// scratch of one u64 per sequence, `out` one Walk in shared memory; both may
-// be reused after the call. False when the CTA has no work.
-template <int M>
-static __device__ bool walk_begin(const View & v, uint32_t group, uint32_t window, uint64_t * cost, Walk * out, Walk & w) {
+// Key tiles [t0, t1) of the current item that this CTA does.
+template <int E>
+__device__ __forceinline__ void walk_segment(const Walk & w, uint32_t & t0, uint32_t & t1) {
+    const uint64_t a = w.unit - w.item0, b = w.end - w.item0;
+    t0 = a > E ? uint32_t(a - E) : 0u;
+    t1 = b <= E ? 0u : b - E < w.k.tiles ? uint32_t(b - E) : w.k.tiles;
+}
+
+// Moves to the CTA's next segment with tiles; false at the end of its line.
+template <int E>
+__device__ __forceinline__ bool walk_next(const View & v, Walk & w) {
+    const uint64_t item_end = w.item0 + w.k.tiles + E;
+    // what is left of the line, if not tiles of another item, is the start of one
+    if (item_end + E >= w.end) return false;
+    w.unit = w.item0 = item_end;
+    ++w.tile;
+    while (w.tile >= row_tiles(v, w.s)) {
+        w.tile = 0;
+        if (++w.b >= v.sequences) {
+            w.b = 0;
+            ++w.kv_head;
+        }
+        w.s = load_sequence(v, w.b);
+    }
+    w.k = key_range(v, w.s, w.tile);
+    return true;
+}
+
+// walk_next of a warp's own copy in shared memory (registers are scarce in the
+// kernels): lane 0 moves it.
+template <int E>
+__device__ __forceinline__ bool walk_warp_next(const View & v, Walk * w) {
+    __syncwarp();
+    int more = 0;
+    if ((threadIdx.x & 31) == 0) more = walk_next<E>(v, *w);
+    return __shfl_sync(0xffffffffu, more, 0) != 0;
+}
+
+// The CTAs that hold the first and the last tile of the current item.
+template <int E>
+__device__ __forceinline__ void walk_owners(const Walk & w, uint32_t & c0, uint32_t & c1) {
+    c0 = cta_of(w.item0 + E, w.total, w.ctas);
+    c1 = cta_of(w.item0 + E + w.k.tiles - 1, w.total, w.ctas);
+}
+
+// Positions `copies` (up to 32) Walks in shared memory at the CTA's first
+// segment. `cost` is shared scratch of one u64 per sequence, free
+// after the call. False when the CTA has no work.
+template <int E>
+static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks, uint32_t copies) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     // units of each sequence: a thread per sequence; the lanes of the warp
     // share the row tiles of a sequence that has many
@@ -262,9 +319,9 @@ static __device__ bool walk_begin(const View & v, uint32_t group, uint32_t windo
         uint64_t units = 0;
         if (b < v.sequences) {
             s = load_sequence(v, b);
-            tiles = row_tiles<M>(s, group);
+            tiles = row_tiles(v, s);
             if (tiles <= 4) {
-                for (uint32_t t = 0; t < tiles; ++t) units += key_range<M>(v, s, group, window, t).units;
+                for (uint32_t t = 0; t < tiles; ++t) units += key_range(v, s, t).tiles + E;
             }
         }
         uint32_t many = __ballot_sync(0xffffffffu, tiles > 4);
@@ -277,7 +334,7 @@ static __device__ bool walk_begin(const View & v, uint32_t group, uint32_t windo
             o.kv = __shfl_sync(0xffffffffu, s.kv, src);
             const uint32_t n = __shfl_sync(0xffffffffu, tiles, src);
             unsigned long long sum = 0;
-            for (uint32_t t = lane; t < n; t += 32) sum += key_range<M>(v, o, group, window, t).units;
+            for (uint32_t t = lane; t < n; t += 32) sum += key_range(v, o, t).tiles + E;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (int(lane) == src) units = sum;
@@ -321,11 +378,11 @@ static __device__ bool walk_begin(const View & v, uint32_t group, uint32_t windo
             x.b = b;
             x.s = load_sequence(v, b);
             // the row tile, the same way
-            const uint32_t tiles = row_tiles<M>(x.s, group);
+            const uint32_t tiles = row_tiles(v, x.s);
             x.tile = 0;
             for (uint32_t base = 0; base < tiles; base += 32) {
                 const unsigned long long mine =
-                    base + lane < tiles ? key_range<M>(v, x.s, group, window, base + lane).units : 0ull;
+                    base + lane < tiles ? key_range(v, x.s, base + lane).tiles + E : 0ull;
                 unsigned long long upto = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -342,43 +399,21 @@ static __device__ bool walk_begin(const View & v, uint32_t group, uint32_t windo
                 left -= __shfl_sync(0xffffffffu, upto, 31);
             }
             x.item0 = x.unit - left;
-            x.k = key_range<M>(v, x.s, group, window, x.tile);
+            x.k = key_range(v, x.s, x.tile);
         } else {
             x.unit = x.end = 0;
         }
-        if (lane == 0) *out = x;
-    }
-    __syncthreads();
-    w = *out;
-    __syncthreads();
-    return w.unit < w.end;
-}
-
-// Key tiles [t0, t1) of the current item that this CTA does.
-__device__ __forceinline__ void walk_segment(const Walk & w, uint32_t & t0, uint32_t & t1) {
-    t0 = uint32_t(w.unit - w.item0);
-    const uint64_t left = w.end - w.unit;
-    t1 = left < w.k.units - t0 ? t0 + uint32_t(left) : w.k.units;
-}
-
-// Moves past the current segment; false at the end of the CTA's line.
-template <int M>
-__device__ __forceinline__ bool walk_next(const View & v, uint32_t group, uint32_t window, Walk & w) {
-    const uint64_t item_end = w.item0 + w.k.units;
-    w.unit = item_end < w.end ? item_end : w.end;
-    if (w.unit >= w.end) return false;
-    w.item0 = w.unit;
-    ++w.tile;
-    while (w.tile >= row_tiles<M>(w.s, group)) {
-        w.tile = 0;
-        if (++w.b >= v.sequences) {
-            w.b = 0;
-            ++w.kv_head;
+        bool any = x.unit < x.end;
+        if (any) {
+            uint32_t t0, t1;
+            walk_segment<E>(x, t0, t1);
+            any = t0 < t1 || walk_next<E>(v, x);
         }
-        w.s = load_sequence(v, w.b);
+        if (!any) x.unit = x.end = 0;
+        if (lane < copies) walks[lane] = x;
     }
-    w.k = key_range<M>(v, w.s, group, window, w.tile);
-    return true;
+    __syncthreads();
+    return walks[0].unit < walks[0].end;
 }
 
 // ---- number types -------------------------------------------------------------------
@@ -460,7 +495,8 @@ inline jfb_status check_batch(const jfb_paged_batch * b, bool rows) {
     return status_ok();
 }
 
-inline View make_view(const jfb_paged_cache & c, const jfb_paged_batch & b, uint32_t rows, int32_t * error) {
+inline View make_view(const jfb_paged_cache & c, const jfb_paged_batch & b, uint32_t rows, uint32_t group, uint32_t window,
+                      int32_t * error) {
     View v;
     v.q_start = b.q_start;
     v.kv_len = b.kv_len;
@@ -477,6 +513,9 @@ inline View make_view(const jfb_paged_cache & c, const jfb_paged_batch & b, uint
     v.kv_heads = c.kv_heads;
     v.head_dim = c.head_dim;
     v.rows = rows;
+    v.group = group;
+    v.window = window;
+    v.item_rows = 0;
     v.error = error;
     return v;
 }

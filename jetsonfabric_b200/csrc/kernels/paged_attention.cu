@@ -26,6 +26,7 @@ namespace {
 // segment, in shared memory.
 
 constexpr int kRowsM = 16;
+constexpr int kItemRows = 0;  // units of an item's start and end
 constexpr int kConsumers = 8;
 constexpr int kThreadsRows = (kConsumers + 2) * 32;
 
@@ -37,7 +38,7 @@ struct RowsSmem {
     static constexpr uint32_t kMl = kMerge + kConsumers * kRowsM * 64 * 4;     // [8][16] (m, l)
     static constexpr uint32_t kBars = kMl + kConsumers * kRowsM * 8;           // full K, full V, empty
     static constexpr uint32_t kWalk = kBars + 3 * kStages * 8;
-    static constexpr uint32_t kFlags = kWalk + (sizeof(Walk) + 15) / 16 * 16;  // abort, last
+    static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(Walk);  // abort, last
     static constexpr uint32_t kBytes = kFlags + 16 + 1024;                     // + alignment
 };
 static_assert(RowsSmem<128>::kBytes <= 232448 && RowsSmem<64>::kBytes <= 232448);
@@ -81,10 +82,9 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     pdl_trigger();
     pdl_wait();
     const View & v = p.view;
-    Walk w;
-    const bool work = walk_begin<kRowsM>(v, p.group, p.window, reinterpret_cast<uint64_t *>(smem),
-                                         reinterpret_cast<Walk *>(smem + L::kWalk), w);
-    if (!work) return;
+    Walk * walks = reinterpret_cast<Walk *>(smem + L::kWalk);
+    if (!walk_begin<kItemRows>(v, reinterpret_cast<uint64_t *>(smem), walks, kThreadsRows / 32)) return;
+    Walk & w = walks[warp];
     fence_proxy_async();  // the ring held the walk's scratch
     __syncthreads();
 
@@ -96,18 +96,23 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         bool ok = true;
         do {
             uint32_t t0, t1;
-            walk_segment(w, t0, t1);
+            walk_segment<kItemRows>(w, t0, t1);
             const int32_t * row = v.table + uint64_t(w.b) * v.table_stride;
-            for (uint32_t t = t0; t < t1 && ok; ++t, ++n) {
+            const uint32_t begin = w.k.begin, hi = w.k.hi, head = w.kv_head;
+            auto pages_of = [&](uint32_t t) {
+                const uint32_t key0 = begin + t * kTileKeys;
+                return tile_pages(v, row, key0, hi <= key0 ? key0 : min(hi, key0 + uint32_t(kTileKeys)));
+            };
+            TileLoad next = pages_of(t0);
+            for (uint32_t t = t0; t < t1; ++t, ++n) {
+                const TileLoad load = next;
+                if (t + 1 < t1) next = pages_of(t + 1);
                 const uint32_t st = n % L::kStages, turn = n / L::kStages;
                 if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
                 if (!ok) break;
-                const uint32_t key0 = w.k.begin + t * kTileKeys;
-                const uint32_t key1 = w.k.hi <= key0 ? key0 : min(w.k.hi, key0 + uint32_t(kTileKeys));
-                load_tile<D>(v, map, row, w.kv_head, key0, key1,
-                             smem_u32(smem) + st * L::kStage + (is_v ? kTileBytes<D> : 0u), full + st);
+                tile_issue<D>(load, map, head, smem_u32(smem) + st * L::kStage + (is_v ? kTileBytes<D> : 0u), full + st);
             }
-        } while (ok && walk_next<kRowsM>(v, p.group, p.window, w));
+        } while (ok && walk_warp_next<kItemRows>(v, &w));
         if (flags[0]) {
             for (uint32_t i = n > uint32_t(L::kStages) ? n - L::kStages : 0u; i < n; ++i) {
                 mbar_drain(full + i % L::kStages, (i / L::kStages) & 1);
@@ -118,14 +123,14 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
 
     // consumers
     const uint32_t grp = lane >> 2, tig = lane & 3;
-    const uint32_t G = p.group, hd = v.head_dim;
+    const uint32_t G = v.group, hd = v.head_dim;
     const float scale2 = p.scale * kLog2e;
     float * merge = reinterpret_cast<float *>(smem + L::kMerge);
     float2 * ml = reinterpret_cast<float2 *>(smem + L::kMl);
     uint32_t n = 0;
     do {
         uint32_t t0, t1;
-        walk_segment(w, t0, t1);
+        walk_segment<kItemRows>(w, t0, t1);
         const uint32_t packed = w.s.count * G;  // rows of an item: below 2^32 (checked on the host)
         const uint32_t row0 = w.tile * kRowsM;
         const int64_t first = int64_t(w.s.kv) - w.s.count;
@@ -182,13 +187,13 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 mma_16816<T>(s[0], qa[kk], b[0], b[1]);
                 mma_16816<T>(s[1], qa[kk], b[2], b[3]);
             }
-            if (key + 15 > pos_first || (p.window > 0 && key <= pos_last - int32_t(p.window))) {
+            if (key + 15 > pos_first || (v.window > 0 && key <= pos_last - int32_t(v.window))) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int32_t k = key + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
-                        if (k > q || (p.window > 0 && k <= q - int32_t(p.window))) s[j][e] = -INFINITY;
+                        if (k > q || (v.window > 0 && k <= q - int32_t(v.window))) s[j][e] = -INFINITY;
                     }
                 }
             }
@@ -271,8 +276,9 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             const float2 a = ml[x * kRowsM + orow];
             sum += a.x == -INFINITY ? 0.0f : a.y * exp2_approx(a.x - top);
         }
-        const RowsOut<T> out(p, w, row0 + orow);
-        const bool whole = t0 == 0 && t1 == w.k.units;
+        const uint32_t r = row0 + orow;
+        const RowsOut<T> out(p, r < packed, w.s.q0 + r / G, w.kv_head * G + r % G);
+        const bool whole = t0 == 0 && t1 == w.k.tiles;
         float * slot = p.partial + uint64_t(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * kSlotFloats;
 #pragma unroll
         for (int h = 0; h < D / 64; ++h) {
@@ -302,7 +308,8 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         } else {
             if ((threadIdx.x & 15) == 0) __stcg(reinterpret_cast<float2 *>(slot + kRowsM * D + 2 * orow), make_float2(top, sum));
             // the last CTA of the item to arrive joins the parts, in CTA order
-            const uint32_t c0 = cta_of(w.item0, w.total, w.ctas), c1 = cta_of(w.item0 + w.k.units - 1, w.total, w.ctas);
+            uint32_t c0, c1;
+            walk_owners<kItemRows>(w, c0, c1);
             __threadfence();
             bar_consumers();
             if (threadIdx.x == 0) {
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             }
             bar_consumers();
         }
-    } while (walk_next<kRowsM>(v, p.group, p.window, w));
+    } while (walk_warp_next<kItemRows>(v, &w));
 }
 
 template <typename T, int D>
@@ -387,15 +394,14 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     }
     if (rows == 0 || batch->sequences == 0) return status_ok();
     AttentionParams p;
-    p.view = make_view(*cache, *batch, rows, error_flag);
+    p.view = make_view(*cache, *batch, rows, heads / cache->kv_heads, window, error_flag);
+    p.view.item_rows = kRowsM;
     p.q = q;
     p.out = out;
     p.lse = lse;
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.heads = heads;
-    p.group = heads / cache->kv_heads;
-    p.window = window;
     p.scale = scale;
     p.counters = static_cast<uint32_t *>(workspace);
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);
@@ -405,7 +411,8 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     }
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
-    if (uint64_t(rows) * p.group > 32ull * batch->sequences) return launch_attention_tc(half, cache->head_dim, mk, mv, p, sms, s);
+    const uint32_t group = p.view.group;
+    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_attention_tc(*cache, mk, mv, p, sms, s);
     if (cache->head_dim <= 64) {
         return half ? launch_rows<__half, 64>(mk, mv, p, sms, s) : launch_rows<__nv_bfloat16, 64>(mk, mv, p, sms, s);
     }

@@ -20,20 +20,18 @@ struct AttentionParams {
     void * out;
     float * lse;
     uint64_t q_stride, out_stride;
-    uint32_t heads, group, window;
+    uint32_t heads;
     float scale;
     uint32_t * counters;
     float * partial;
 };
 
-// Where packed row r of the walk's item goes.
+// Where a result row goes.
 template <typename T>
 struct RowsOut {
     T * out;  // nullptr: no such row
     uint64_t at;
-    __device__ __forceinline__ RowsOut(const AttentionParams & p, const Walk & w, uint32_t r) {
-        const bool valid = r < w.s.count * p.group;
-        const uint32_t row = w.s.q0 + (valid ? r / p.group : 0u), head = w.kv_head * p.group + (valid ? r % p.group : 0u);
+    __device__ __forceinline__ RowsOut(const AttentionParams & p, bool valid, uint32_t row, uint32_t head) {
         out = valid ? static_cast<T *>(p.out) + uint64_t(row) * p.out_stride + uint64_t(head) * p.view.head_dim : nullptr;
         at = uint64_t(row) * p.heads + head;
     }
@@ -42,6 +40,22 @@ struct RowsOut {
         if (out == nullptr || d >= head_dim) return;
         const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
         *reinterpret_cast<uint2 *>(out + d) = make_uint2(Num<T>::pack(a.x * f, a.y * f), Num<T>::pack(a.z * f, a.w * f));
+    }
+    // sixteen columns, as one 32-byte sector where rows are aligned to it
+    __device__ __forceinline__ void store16(uint32_t d, const float * a, float sum, uint32_t head_dim, bool sectors) const {
+        if (out == nullptr || d >= head_dim) return;
+        const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = Num<T>::pack(a[2 * i] * f, a[2 * i + 1] * f);
+        if (sectors && d + 16 <= head_dim) {
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + d), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                         "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        } else {
+            *reinterpret_cast<uint4 *>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (d + 8 < head_dim) *reinterpret_cast<uint4 *>(out + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
     }
     // top is the maximum in units of log 2
     __device__ __forceinline__ void store_lse(const AttentionParams & p, float top, float sum) const {
@@ -67,7 +81,7 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const ui
 }
 
 // The tcgen05 kernel of paged_attention_tc.cu.
-jfb_status launch_attention_tc(bool half, uint32_t head_dim, const CUtensorMap & k, const CUtensorMap & v, const AttentionParams & p,
+jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap & k, const CUtensorMap & v, AttentionParams p,
                                uint32_t sms, cudaStream_t s);
 
 // Query-shaped rows [rows][heads x head_dim] of 16-bit numbers.

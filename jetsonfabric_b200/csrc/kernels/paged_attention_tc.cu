@@ -1,17 +1,22 @@
 // Attention of chunks over a cache in pages on the tcgen05 tensor cores.
 //
-// An item is 256 packed rows (token, head of the group) of one sequence and kv
-// head, two tiles of 128, and its keys come in tiles of 128. One CTA per SM
+// An item is two row tiles of one sequence and kv head, each the packed rows
+// (token, head of the group) of 128 / G whole tokens, so that the tile's
+// queries are one box of TMA; its keys come in tiles of 128. One CTA per SM
 // walks its share of the units (walk_begin):
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, a thread per row: scores from
 //                   tensor memory, running maximum and sum, probabilities back
-//                   over the scores as the 16-bit A operand, results out;
-//   warp 8          MMA: S_x = Q_x K^T and O_x += P_x V, so that one row tile's
-//                   products run under the other's softmax;
-//   warps 9, 10     K and V tiles, page by page through TMA, into one ring.
-// Tensor memory (512 columns): S_0, S_1, O_0, O_1 of 128 f32 columns; P_x
-// takes the first 64 columns of S_x. An MMA chain executes in issue order, so
-// S_x of the next tile is issued right behind the P_x V that still reads P_x.
+//                   as the 16-bit A operand, results out;
+//   warps 8, 11     the MMAs, S_x = Q_x K^T from one and O_x += P_x V from the
+//                   other, each waiting only for what its own chain needs;
+//   warp 9          K and V tiles, page by page through TMA, into one ring;
+//   warp 10         the queries of the next item, as soon as the last scores of
+//                   this one are formed.
+// Tensor memory (512 columns): O_0 and O_1 of 128 f32 columns, P_0 and P_1 of
+// 64 columns of 16-bit pairs, and one S of 128. The row tiles take turns with
+// S: a softmax thread moves its row into registers at once, which frees S for
+// the other tile's scores while it works, so the scores a row tile needs next
+// are formed during its current exponentials.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one its sums refer to (the sums stay far inside f32's range and the
@@ -24,34 +29,39 @@ namespace jfb {
 namespace paged {
 namespace {
 
-constexpr int kRowsTc = 256;
+constexpr int kItemTc = 2;  // units of an item's start and end
 constexpr int kThreadsTc = 384;
-constexpr int kMmaWarp = 8, kWarpK = 9, kWarpV = 10;
-constexpr uint32_t kColS = 0, kColO = 256;  // of row tile 0; tile 1 is 128 columns further
-constexpr float kSlack = 8.0f;              // growth of the maximum (log 2) that a rescale waits for
+constexpr int kWarpS = 8, kWarpKV = 9, kWarpQ = 10;  // warp 11 issues P V
+constexpr uint32_t kColO = 0, kColP = 256, kColS = 384;  // O_1 is 128 and P_1 64 columns further
+constexpr float kSlack = 8.0f;                           // growth of the maximum (log 2) that a rescale waits for
 
 template <int D>
 struct TcSmem {
     static constexpr int kStages = D == 128 ? 5 : 10;
-    static constexpr uint32_t kQ = 2 * 128 * D * 2;
+    static constexpr uint32_t kQ = 2 * kTileBytes<D>;
     static constexpr uint32_t kBars = kQ + kStages * kTileBytes<D>;
-    static constexpr uint32_t kNumBars = 2 * kStages + 8;  // full, empty; s, p, o, q of both row tiles
+    static constexpr uint32_t kNumBars = 2 * kStages + 11;  // full, empty; s, p, o, q full and q free of both row tiles; S free
     static constexpr uint32_t kWalk = kBars + kNumBars * 8;
-    static constexpr uint32_t kFlags = kWalk + (sizeof(Walk) + 15) / 16 * 16;  // abort, last of tile 0 and 1, tmem
-    static constexpr uint32_t kBytes = kFlags + 32 + 1024;
+    static constexpr uint32_t kFlags = kWalk + kThreadsTc / 32 * sizeof(Walk);  // abort, last of tile 0 and 1, tmem
+    static constexpr uint32_t kBytes = kFlags + 32;
 };
 static_assert(TcSmem<128>::kBytes <= 232448 && TcSmem<64>::kBytes <= 232448);
 static_assert(TcSmem<64>::kBars >= JFB_PAGED_MAX_SEQUENCES * 8);
 
-template <typename T>
-__device__ __forceinline__ const T * query_row(const AttentionParams & p, const Walk & w, uint32_t r) {
-    if (r >= w.s.count * p.group) return nullptr;
-    return static_cast<const T *>(p.q) + uint64_t(w.s.q0 + r / p.group) * p.q_stride +
-           uint64_t(w.kv_head * p.group + r % p.group) * p.view.head_dim;
-}
+// First token of row tile x of the walk's item, and whether the item has a second one.
+__device__ __forceinline__ uint32_t first_token(const Walk & w, uint32_t tokens, uint32_t x) { return (w.tile * 2 + x) * tokens; }
+__device__ __forceinline__ bool two_tiles(const Walk & w, uint32_t tokens) { return w.s.count > first_token(w, tokens, 1); }
 
-__device__ __forceinline__ bool two_tiles(const AttentionParams & p, const Walk & w) {
-    return w.s.count * p.group > w.tile * kRowsTc + 128;
+// The calling warp zeroes rows [a, b) of a tile (a <= b <= 128).
+template <int D>
+__device__ __forceinline__ void clear_rows(uint32_t tile, uint32_t a, uint32_t b) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t i = a * 8 + lane; i < b * 8; i += 32) {
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + h * kHalfBytes + i * 16), "r"(0) : "memory");
+        }
+    }
 }
 
 // The 128 threads of one row tile's softmax.
@@ -60,18 +70,23 @@ __device__ __forceinline__ void bar_tile(uint32_t x) {
     else asm volatile("bar.sync 2, 128;" ::: "memory");
 }
 
+struct TcMaps {
+    CUtensorMap k, v, q;
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreadsTc, 1)
-    paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
-    extern __shared__ uint8_t smem_raw[];
+__global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_constant__ TcMaps maps, const AttentionParams p,
+                                                                 const uint32_t tokens, const bool sectors) {
+    extern __shared__ __align__(1024) uint8_t smem[];
     using L = TcSmem<D>;
-    uint8_t * smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t * full = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t * empty = full + L::kStages;
     uint64_t * s_full = empty + L::kStages;
     uint64_t * p_full = s_full + 2;
     uint64_t * o_full = p_full + 2;
     uint64_t * q_full = o_full + 2;
+    uint64_t * q_free = q_full + 2;
+    uint64_t * s_free = q_free + 2;
     volatile int * flags = reinterpret_cast<volatile int *>(smem + L::kFlags);
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kFlags + 16);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -84,20 +99,27 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             mbar_init(s_full + x, 1);
             mbar_init(p_full + x, 4);
             mbar_init(o_full + x, 1);
-            mbar_init(q_full + x, 4);
+            mbar_init(q_full + x, 1);
+            mbar_init(q_free + x, 1);
         }
+        mbar_init(s_free, 4);
         flags[0] = 0;
         mbar_init_fence();
     }
     pdl_trigger();
     pdl_wait();
     const View & v = p.view;
-    Walk w;
-    if (!walk_begin<kRowsTc>(v, p.group, p.window, reinterpret_cast<uint64_t *>(smem), reinterpret_cast<Walk *>(smem + L::kWalk), w)) {
+    if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it
+        if (threadIdx.x == 0) flag_error(v.error, JFB_PAGED_ERROR_TIMEOUT);
         return;
     }
-    fence_proxy_async();  // the ring held the walk's scratch
-    if (warp == kMmaWarp) tmem_alloc(tmem_slot);
+    Walk * walks = reinterpret_cast<Walk *>(smem + L::kWalk);
+    if (!walk_begin<kItemTc>(v, reinterpret_cast<uint64_t *>(smem), walks, kThreadsTc / 32)) return;
+    Walk & w = walks[warp];
+    // rows that no query fills stay zero (and this held the walk's scratch)
+    for (uint32_t i = threadIdx.x; i < L::kQ / 16; i += kThreadsTc) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+    if (warp == kWarpS) tmem_alloc(tmem_slot);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -105,129 +127,148 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     const uint32_t ring = smem_u32(smem) + L::kQ;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == kWarpK || warp == kWarpV) {
-            const bool is_v = warp == kWarpV;
-            const CUtensorMap * map = is_v ? &map_v : &map_k;
-            uint32_t n = is_v ? 1 : 0;  // ring slots alternate K, V
-            bool ok = true;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        bool ok = true;
+        auto wait = [&](uint64_t * bar, uint32_t parity) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, flags, v.error));
+            return ok;
+        };
+        if (warp == kWarpKV) {
+            uint32_t n = 0;  // ring slots alternate K, V
             do {
                 uint32_t t0, t1;
-                walk_segment(w, t0, t1);
+                walk_segment<kItemTc>(w, t0, t1);
                 const int32_t * row = v.table + uint64_t(w.b) * v.table_stride;
-                for (uint32_t t = t0; t < t1; ++t, n += 2) {
-                    const uint32_t st = n % L::kStages, turn = n / L::kStages;
-                    if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
-                    if (!ok) break;
-                    const uint32_t key0 = w.k.begin + t * kTileKeys;
-                    const uint32_t key1 = w.k.hi <= key0 ? key0 : min(w.k.hi, key0 + uint32_t(kTileKeys));
-                    load_tile<D>(v, map, row, w.kv_head, key0, key1, ring + st * kTileBytes<D>, full + st);
+                const uint32_t begin = w.k.begin, kv = w.s.kv, head = w.kv_head;
+                auto pages_of = [&](uint32_t t) {
+                    const uint32_t key0 = begin + t * kTileKeys;
+                    return tile_pages(v, row, key0, kv <= key0 ? key0 : min(kv, key0 + uint32_t(kTileKeys)));
+                };
+                TileLoad next = pages_of(t0);
+                for (uint32_t t = t0; ok && t < t1; ++t) {
+                    const TileLoad load = next;
+                    if (t + 1 < t1) next = pages_of(t + 1);
+                    for (uint32_t is_v = 0; is_v < 2; ++is_v, ++n) {
+                        const uint32_t st = n % L::kStages, turn = n / L::kStages;
+                        if (turn > 0 && !wait(empty + st, (turn - 1) & 1)) break;
+                        tile_issue<D>(load, is_v ? &maps.v : &maps.k, head, ring + st * kTileBytes<D>, full + st);
+                    }
                 }
-            } while (ok && walk_next<kRowsTc>(v, p.group, p.window, w));
+            } while (ok && walk_warp_next<kItemTc>(v, &w));
             if (flags[0]) {
-                for (uint32_t i = n >= 2u * L::kStages ? n - 2u * L::kStages : (is_v ? 1u : 0u); i < n; i += 2) {
+                for (uint32_t i = n > uint32_t(L::kStages) ? n - L::kStages : 0u; i < n; ++i) {
                     mbar_drain(full + i % L::kStages, (i / L::kStages) & 1);
                 }
             }
-        } else if (warp == kMmaWarp) {
-            constexpr uint32_t idesc_s = instr_desc<T>(kTileKeys, false), idesc_o = instr_desc<T>(D, true);
+        } else if (warp == kWarpQ) {
+            uint32_t items[2] = {0, 0};
+            do {
+                const uint32_t two = two_tiles(w, tokens) ? 1 : 0;
+                for (uint32_t x = 0; ok && x <= two; ++x) {
+                    if (items[x] > 0 && !wait(q_free + x, (items[x] - 1) & 1)) break;
+                    ++items[x];
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(q_full + x, tokens * v.group * D * 2);
+                        for (int h = 0; h < D / 64; ++h) {
+                            tma_load_rows(smem_u32(smem) + x * kTileBytes<D> + h * kHalfBytes, &maps.q, h * 64, int32_t(w.kv_head * v.group),
+                                          int32_t(w.s.q0 + first_token(w, tokens, x)), q_full + x);
+                        }
+                    }
+                    __syncwarp();
+                }
+            } while (ok && walk_warp_next<kItemTc>(v, &w));
+            if (flags[0]) {
+                for (uint32_t x = 0; x < 2; ++x) {
+                    if (items[x] > 0) mbar_drain(q_full + x, (items[x] - 1) & 1);
+                }
+            }
+        } else {
+            // steps j of a segment are (key tile j >> two, row tile j & two)
+            const bool scores = warp == kWarpS;
             const uint32_t q_addr = smem_u32(smem);
             uint32_t tiles[2] = {0, 0}, items[2] = {0, 0};
-            uint32_t g = 0;  // key tiles so far
-            bool ok = true;
-            auto wait = [&](uint64_t * bar, uint32_t parity) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, flags, v.error));
-                return ok;
-            };
+            uint32_t g = 0;      // key tiles before this segment
+            uint32_t moved = 0;  // times S was used
             auto full_of = [&](uint32_t n) { return wait(full + n % L::kStages, (n / L::kStages) & 1); };
-            auto issue_s = [&](uint32_t x, uint32_t n) {
-                const uint32_t k_addr = ring + (n % L::kStages) * kTileBytes<D>;
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t at = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-                    mma_ss(tmem + kColS + x * 128, desc_k_major(q_addr + x * (128 * D * 2) + at), desc_k_major(k_addr + at), idesc_s, kk > 0);
-                }
-                mma_commit(s_full + x);
-            };
             do {
                 uint32_t t0, t1;
-                walk_segment(w, t0, t1);
-                const uint32_t last = two_tiles(p, w) ? 1 : 0;
-                if (!full_of(2 * g)) break;
-                for (uint32_t x = 0; x <= last; ++x) {
-                    if (!wait(q_full + x, items[x]++ & 1)) break;
-                    tc_fence_after();
-                    issue_s(x, 2 * g);
-                }
-                if (!ok) break;
-                mma_commit(empty + (2 * g) % L::kStages);
-                for (uint32_t t = t0; ok && t < t1; ++t, ++g) {
-                    const uint32_t vs = (2 * g + 1) % L::kStages;
-                    const uint32_t v_addr = ring + vs * kTileBytes<D>;
-                    for (uint32_t x = 0; x <= last; ++x) {
-                        if (!wait(p_full + x, tiles[x]++ & 1)) break;
+                walk_segment<kItemTc>(w, t0, t1);
+                const uint32_t two = two_tiles(w, tokens) ? 1 : 0;
+                const uint32_t steps = (t1 - t0) << two;
+                const uint32_t begin = w.k.begin, kv = w.s.kv;
+                // first slot that the sequence's first new row sees
+                const uint32_t seen_from = v.window > 0 && kv > w.s.count + (v.window - 1) ? kv - w.s.count - (v.window - 1) : 0u;
+                for (uint32_t j = 0; j < steps; ++j) {
+                    const uint32_t x = j & two, n = 2 * (g + (j >> two)) + (scores ? 0 : 1);
+                    const uint32_t addr = ring + (n % L::kStages) * kTileBytes<D>;
+                    if (scores) {
+                        if (x == 0 && !full_of(n)) break;
+                        if (j <= two && !wait(q_full + x, items[x]++ & 1)) break;
+                        if (moved > 0 && !wait(s_free, (moved - 1) & 1)) break;
+                        ++moved;
+                        tc_fence_after();
+                        const uint32_t qx = q_addr + x * kTileBytes<D>;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t at = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+                            mma_ss(tmem + kColS, desc_k_major(qx + at), desc_k_major(addr + at), instr_desc<T>(kTileKeys, false), kk > 0);
+                        }
+                        mma_commit(s_full + x);
+                        if (j + two >= steps - 1) mma_commit(q_free + x);
+                    } else {
+                        const uint32_t t = t0 + (j >> two);
                         if (x == 0) {
-                            if (!full_of(2 * g + 1)) break;
-                            // what no row sees may hold anything: its probability is 0, but 0 x NaN is not
-                            const uint32_t key0 = w.k.begin + t * kTileKeys;
-                            if (key0 < w.k.lo || key0 + kTileKeys > w.k.hi) {
-                                for (uint32_t r = 0; r < uint32_t(kTileKeys); ++r) {
-                                    if (key0 + r >= w.k.lo && key0 + r < w.k.hi) continue;
-                                    if (lane < D / 8) {
-                                        const uint32_t at = v_addr + (lane >> 3) * kHalfBytes + r * 128 + ((lane & 7) << 4);
-                                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                                    }
-                                }
+                            if (!full_of(n)) break;
+                            // Slots that no row of the sequence sees may hold anything: their
+                            // probability is 0, but 0 x NaN is not.
+                            const uint32_t key0 = begin + t * kTileKeys;
+                            const uint32_t from = key0 < seen_from ? min(seen_from - key0, uint32_t(kTileKeys)) : 0u;
+                            const uint32_t to = kv > key0 ? min(kv - key0, uint32_t(kTileKeys)) : 0u;
+                            if (from > 0 || to < uint32_t(kTileKeys)) {
+                                clear_rows<D>(addr, 0, from);
+                                clear_rows<D>(addr, to, kTileKeys);
                                 fence_proxy_async();
                                 __syncwarp();
                             }
                         }
+                        if (!wait(p_full + x, tiles[x]++ & 1)) break;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-                            mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + kk * 8, desc_mn_major(v_addr + kk * 2048), idesc_o,
-                                   t > t0 || kk > 0);
+                            mma_ts(tmem + kColO + x * 128, tmem + kColP + x * 64 + kk * 8, desc_mn_major(addr + kk * 2048),
+                                   instr_desc<T>(D, true), t > t0 || kk > 0);
                         }
                         mma_commit(o_full + x);
-                        if (x == last) mma_commit(empty + vs);
-                        if (t + 1 < t1) {
-                            if (x == 0 && !full_of(2 * g + 2)) break;
-                            issue_s(x, 2 * g + 2);
-                            if (x == last) mma_commit(empty + (2 * g + 2) % L::kStages);
-                        }
                     }
+                    if (x == two) mma_commit(empty + n % L::kStages);
                 }
-            } while (ok && walk_next<kRowsTc>(v, p.group, p.window, w));
+                g += t1 - t0;
+            } while (ok && walk_warp_next<kItemTc>(v, &w));
             if (flags[0]) {  // MMAs in flight finish before tensor memory is given back
                 const uint64_t t = global_ns();
-                mma_commit(q_full);
                 while (global_ns() - t < 10000000ull) __nanosleep(1000);
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t x = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
-        const uint32_t t_s = lanes + kColS + x * 128, t_o = lanes + kColO + x * 128;
+        const uint32_t t_s = lanes + kColS, t_p = lanes + kColP + x * 64, t_o = lanes + kColO + x * 128;
         const float scale2 = p.scale * kLog2e;
-        uint32_t n = 0;  // tiles of this row tile so far
-        auto load_q = [&]() {
-            store_row<T, D>(smem + x * (128 * D * 2), row, query_row<T>(p, w, w.tile * kRowsTc + x * 128 + row), v.head_dim);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full + x);
-        };
+        const uint32_t token = row / v.group, head = row - token * v.group;  // within the tile and the group
+        uint32_t n = 0;                                                      // tiles of this row tile so far
         bool more = true;
-        while (more && x == 1 && !two_tiles(p, w)) more = walk_next<kRowsTc>(v, p.group, p.window, w);
-        if (more) load_q();
-        while (more) {
+        do {
+            if (x == 1 && !two_tiles(w, tokens)) {
+                more = walk_warp_next<kItemTc>(v, &w);
+                continue;
+            }
             uint32_t t0, t1;
-            walk_segment(w, t0, t1);
-            const uint32_t packed = w.s.count * p.group, r0 = w.tile * kRowsTc + x * 128;
-            const int64_t first = int64_t(w.s.kv) - w.s.count;
-            const int32_t pos = int32_t(first + (r0 + row) / p.group);
-            const int32_t pos_first = int32_t(first + r0 / p.group);
-            const int32_t pos_last = int32_t(first + (min(r0 + 128, packed) - 1) / p.group);
+            walk_segment<kItemTc>(w, t0, t1);
+            const uint32_t token0 = first_token(w, tokens, x);
+            const int32_t pos_first = int32_t(int64_t(w.s.kv) - w.s.count + token0), pos = pos_first + int32_t(token);
+            const int32_t pos_last = pos_first + int32_t(min(tokens, w.s.count - token0)) - 1;
+            const uint32_t begin = w.k.begin;
             float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
             for (uint32_t t = t0; t < t1; ++t, ++n) {
                 // after a wait that gave up the tiles are skipped; the warps still meet at the barriers below
@@ -237,19 +278,29 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, s + c * 32);
                 tmem_wait_ld();
-                const int32_t key0 = int32_t(w.k.begin + t * kTileKeys);
-                if (key0 + kTileKeys - 1 > pos_first || (p.window > 0 && key0 <= pos_last - int32_t(p.window))) {
-                    const int32_t hi = pos - key0, lo = p.window > 0 ? hi - int32_t(p.window) : -1;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free);
+                const int32_t key0 = int32_t(begin + t * kTileKeys);
+                if (key0 + kTileKeys - 1 > pos_first || (v.window > 0 && key0 <= pos_last - int32_t(v.window))) {
+                    const int32_t hi = pos - key0, lo = v.window > 0 ? hi - int32_t(v.window) : -1;
 #pragma unroll
                     for (int i = 0; i < 128; ++i) s[i] = i <= hi && i > lo ? s[i] : -INFINITY;
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < 128; i += 4) {
+                for (int i = 4; i + 8 <= 128; i += 8) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[i + e]);
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale2;
+                // P and O are free again when the previous product is done
+                if (t > t0) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(o_full + x, (n - 1) & 1, flags, v.error))) continue;
+                    tc_fence_after();
+                }
                 const bool grow = top > m + kSlack;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float next = grow ? top : m;
@@ -258,16 +309,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     l0 *= f;
                     l1 *= f;
                     if (t > t0) {
-                        if (!__all_sync(0xffffffffu, mbar_wait(o_full + x, (n - 1) & 1, flags, v.error))) continue;
-                        tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            float o[32];
-                            tmem_ld32(t_o + c * 32, o);
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            tmem_ld16(t_o + c, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= f;
-                            tmem_st32(t_o + c * 32, reinterpret_cast<const uint32_t *>(o));
+                            for (int i = 0; i < 16; ++i) o[i] *= f;
+                            tmem_st16(t_o + c, reinterpret_cast<const uint32_t *>(o));
                         }
                     }
                 }
@@ -284,46 +333,46 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         add2(l0, l1, a, b);
                         pk[i / 2] = Num<T>::pack(a, b);
                     }
-                    tmem_st16(t_s + c * 16, pk);
+                    tmem_st16(t_p + c * 16, pk);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + x);
             }
-            // the segment's results; the next item's rows are fetched first, so its products can start
-            const RowsOut<T> out(p, w, r0 + row);
-            const bool whole = t0 == 0 && t1 == w.k.units;
-            const uint32_t c0 = cta_of(w.item0, w.total, w.ctas), c1 = cta_of(w.item0 + w.k.units - 1, w.total, w.ctas);
-            do {
-                more = walk_next<kRowsTc>(v, p.group, p.window, w);
-            } while (more && x == 1 && !two_tiles(p, w));
-            if (more) load_q();
-            const bool ok = __all_sync(0xffffffffu, flags[0] == 0 && mbar_wait(o_full + x, (n - 1) & 1, flags, v.error));
-            tc_fence_after();
+            // the segment's results
             const float sum = l0 + l1;
+            const bool whole = t0 == 0 && t1 == w.k.tiles;
+            const RowsOut<T> out(p, token < min(tokens, w.s.count - token0), w.s.q0 + token0 + token, w.kv_head * v.group + head);
             // parts are stored as [4 columns][row] so that a warp's stores are contiguous
             float * slot = p.partial + uint64_t(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * kSlotFloats;
-            if (ok) {
+            if (__all_sync(0xffffffffu, flags[0] == 0 && mbar_wait(o_full + x, (n - 1) & 1, flags, v.error))) {
+                tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float o[32];
-                    tmem_ld32(t_o + c * 32, o);
+                for (int c = 0; c < D; c += 64) {
+                    float o[64];
+                    tmem_ld32(t_o + c, o);
+                    tmem_ld32(t_o + c + 32, o + 32);
                     tmem_wait_ld();
+                    if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 a = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        const uint32_t d = c * 32 + i;
-                        if (whole) out.store4(d, a, sum, v.head_dim);
-                        else __stcg(reinterpret_cast<float4 *>(slot) + (d / 4) * kRowsTc + x * 128 + row, a);
+                        for (int i = 0; i < 64; i += 16) out.store16(c + i, o + i, sum, v.head_dim, sectors);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            __stcg(reinterpret_cast<float4 *>(slot) + ((c + i) / 4) * 256 + x * 128 + row,
+                                   make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                        }
                     }
                 }
                 if (whole) out.store_lse(p, m, sum);
-                else __stcg(reinterpret_cast<float2 *>(slot + kRowsTc * D) + x * 128 + row, make_float2(m, sum));
+                else __stcg(reinterpret_cast<float2 *>(slot + 256 * D) + x * 128 + row, make_float2(m, sum));
             }
             tc_fence_before();
             if (!whole) {
                 // the last CTA of the item to arrive joins this row tile's parts, in CTA order
+                uint32_t c0, c1;
+                walk_owners<kItemTc>(w, c0, c1);
                 __threadfence();
                 bar_tile(x);
                 if (row == 0) {
@@ -335,60 +384,86 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 if (flags[1 + x]) {
                     __threadfence();
                     auto part_of = [&](uint32_t c) { return p.partial + uint64_t(2 * c + (c == c0 ? 1 : 0)) * kSlotFloats; };
-                    auto ml_of = [&](uint32_t c) { return __ldcg(reinterpret_cast<const float2 *>(part_of(c) + kRowsTc * D) + x * 128 + row); };
+                    auto ml_of = [&](uint32_t c) { return __ldcg(reinterpret_cast<const float2 *>(part_of(c) + 256 * D) + x * 128 + row); };
                     float jtop = -INFINITY, jsum = 0.0f;
                     for (uint32_t c = c0; c <= c1; ++c) jtop = fmaxf(jtop, ml_of(c).x);
                     for (uint32_t c = c0; c <= c1; ++c) {
                         const float2 a = ml_of(c);
                         jsum = fmaf(a.y, a.x == -INFINITY ? 0.0f : exp2_approx(a.x - jtop), jsum);
                     }
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 64) {
+                        float acc[64];
 #pragma unroll
-                    for (int d = 0; d < D; d += 32) {
-                        float4 acc[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
                         for (uint32_t c = c0; c <= c1; ++c) {
                             const float a = ml_of(c).x;
                             const float f = a == -INFINITY ? 0.0f : exp2_approx(a - jtop);
-                            const float4 * from = reinterpret_cast<const float4 *>(part_of(c)) + (d / 4) * kRowsTc + x * 128 + row;
+                            const float4 * from = reinterpret_cast<const float4 *>(part_of(c)) + (d / 4) * 256 + x * 128 + row;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float4 y = __ldcg(from + i * kRowsTc);
-                                acc[i].x = fmaf(y.x, f, acc[i].x);
-                                acc[i].y = fmaf(y.y, f, acc[i].y);
-                                acc[i].z = fmaf(y.z, f, acc[i].z);
-                                acc[i].w = fmaf(y.w, f, acc[i].w);
+                            for (int i = 0; i < 16; ++i) {
+                                const float4 y = __ldcg(from + i * 256);
+                                acc[4 * i] = fmaf(y.x, f, acc[4 * i]);
+                                acc[4 * i + 1] = fmaf(y.y, f, acc[4 * i + 1]);
+                                acc[4 * i + 2] = fmaf(y.z, f, acc[4 * i + 2]);
+                                acc[4 * i + 3] = fmaf(y.w, f, acc[4 * i + 3]);
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) out.store4(d + i * 4, acc[i], jsum, v.head_dim);
+                        for (int i = 0; i < 64; i += 16) out.store16(d + i, acc + i, jsum, v.head_dim, sectors);
                     }
                     out.store_lse(p, jtop, jsum);
                 }
                 bar_tile(x);
             }
-        }
+            more = walk_warp_next<kItemTc>(v, &w);
+        } while (more);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) tmem_free(tmem);
+    if (warp == kWarpS) tmem_free(tmem);
+}
+
+// Query rows as (head_dim, heads, rows): boxes of 64 elements x the group x whole tokens.
+bool query_map(CUtensorMap & map, const AttentionParams & p, uint32_t tokens) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[3] = {p.view.head_dim, p.heads, p.view.rows};
+    const cuuint64_t strides[2] = {uint64_t(p.view.head_dim) * 2, p.q_stride * 2};
+    const cuuint32_t box[3] = {64, p.view.group, tokens};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    std::memset(&map, 0, sizeof(map));
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(p.q), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D>
-jfb_status launch(const CUtensorMap & k, const CUtensorMap & v, const AttentionParams & p, uint32_t sms, cudaStream_t s) {
+jfb_status launch(const TcMaps & maps, const AttentionParams & p, uint32_t tokens, uint32_t sms, cudaStream_t s) {
+    // rows of whole 32-byte sectors
+    const bool sectors = ((reinterpret_cast<uintptr_t>(p.out) | p.out_stride * 2 | p.view.head_dim * 2) & 31u) == 0;
     auto kernel = paged_tc_kernel<T, D>;
     cudaError_t e = allow_smem(kernel, TcSmem<D>::kBytes);
-    if (e == cudaSuccess) e = launch_k(kernel, dim3(sms), dim3(kThreadsTc), TcSmem<D>::kBytes, s, k, v, p);
+    if (e == cudaSuccess) e = launch_k(kernel, dim3(sms), dim3(kThreadsTc), TcSmem<D>::kBytes, s, maps, p, tokens, sectors);
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_attention");
 }
 
 }  // namespace
 
-jfb_status launch_attention_tc(bool half, uint32_t head_dim, const CUtensorMap & k, const CUtensorMap & v, const AttentionParams & p,
+jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap & k, const CUtensorMap & v, AttentionParams p,
                                uint32_t sms, cudaStream_t s) {
-    if (head_dim <= 64) return half ? launch<__half, 64>(k, v, p, sms, s) : launch<__nv_bfloat16, 64>(k, v, p, sms, s);
-    return half ? launch<__half, 128>(k, v, p, sms, s) : launch<__nv_bfloat16, 128>(k, v, p, sms, s);
+    const uint32_t tokens = 128 / p.view.group;
+    p.view.item_rows = 2 * tokens * p.view.group;
+    TcMaps maps;
+    maps.k = k;
+    maps.v = v;
+    if (!query_map(maps.q, p, tokens)) {
+        return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: could not encode a TMA tensor map");
+    }
+    const bool half = cache.dtype == JFB_DTYPE_F16;
+    if (cache.head_dim <= 64) return half ? launch<__half, 64>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 64>(maps, p, tokens, sms, s);
+    return half ? launch<__half, 128>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 128>(maps, p, tokens, sms, s);
 }
 
 }  // namespace paged

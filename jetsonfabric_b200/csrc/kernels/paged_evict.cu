@@ -250,7 +250,7 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     }
     if (batch->sequences == 0) return status_ok();
     EvictParams p;
-    p.view = make_view(*cache, *batch, 0, error_flag);
+    p.view = make_view(*cache, *batch, 0, 1, 0, error_flag);
     p.mass = mass;
     p.mass_out = mass_out;
     p.keep = keep;

@@ -17,7 +17,7 @@ struct MassParams {
     const float * mass_in;
     float * mass_out;
     uint64_t q_stride, mass_stride;
-    uint32_t heads, group, window;
+    uint32_t heads;
     float scale;
 };
 
@@ -161,15 +161,21 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     if (warp == kConsumers) {
         uint32_t n = 0;
         bool ok = true;
-        do {
+        auto pages_of = [&](const KeyWalk & a) {
+            const uint32_t key0 = a.tile * kTileKeys;
+            return tile_pages(v, v.table + uint64_t(a.b) * v.table_stride, key0, min(a.limit, key0 + uint32_t(kTileKeys)));
+        };
+        TileLoad next = pages_of(w);
+        for (bool more = true; more; ++n) {
+            const TileLoad load = next;
+            const uint32_t head = w.kv_head;
+            more = key_walk_next(v, p.mass_stride, w);
+            if (more) next = pages_of(w);
             const uint32_t st = n % L::kStages, turn = n / L::kStages;
             if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
             if (!ok) break;
-            const uint32_t key0 = w.tile * kTileKeys;
-            load_tile<D>(v, &map_k, v.table + uint64_t(w.b) * v.table_stride, w.kv_head, key0,
-                         min(w.limit, key0 + uint32_t(kTileKeys)), smem_u32(smem) + st * kTileBytes<D>, full + st);
-            ++n;
-        } while (key_walk_next(v, p.mass_stride, w));
+            tile_issue<D>(load, &map_k, head, smem_u32(smem) + st * kTileBytes<D>, full + st);
+        }
         if (flags[0]) {
             for (uint32_t i = n > uint32_t(L::kStages) ? n - L::kStages : 0u; i < n; ++i) {
                 mbar_drain(full + i % L::kStages, (i / L::kStages) & 1);
@@ -179,7 +185,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     }
 
     const uint32_t grp = lane >> 2, tig = lane & 3;
-    const uint32_t G = p.group, hd = v.head_dim;
+    const uint32_t G = v.group, hd = v.head_dim;
     const float scale2 = p.scale * kLog2e;
     uint32_t n = 0;
     do {
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         if (key < w.limit) {
             const int64_t first = int64_t(w.s.kv) - w.s.count;
             uint32_t r0, r1;
-            seeing_rows(w.s, G, p.window, key, min(w.limit, key + 16), r0, r1);
+            seeing_rows(w.s, G, v.window, key, min(w.limit, key + 16), r0, r1);
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (uint32_t base = r0; base < r1; base += 16) {
                 float s[2][4];
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int32_t k = int32_t(key) + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
-                        const bool seen = k <= q && (p.window == 0 || k > q - int32_t(p.window));
+                        const bool seen = k <= q && (v.window == 0 || k > q - int32_t(v.window));
                         if (seen) acc[j * 2 + (e & 1)] += exp2_approx(fmaf(s[j][e], scale2, -lse2[e >> 1]));
                     }
                 }
@@ -303,7 +309,7 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     if (sms == 0) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no usable device");
     if (batch->sequences == 0) return status_ok();
     MassParams p;
-    p.view = make_view(*cache, *batch, rows, error_flag);
+    p.view = make_view(*cache, *batch, rows, heads / cache->kv_heads, window, error_flag);
     p.q = q;
     p.lse = lse;
     p.mass_in = mass_in;
@@ -311,8 +317,6 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     p.q_stride = q_stride;
     p.mass_stride = mass_stride;
     p.heads = heads;
-    p.group = heads / cache->kv_heads;
-    p.window = window;
     p.scale = scale;
     CUtensorMap mk;
     if (!pool_map(mk, cache->k, *cache)) {

@@ -316,7 +316,7 @@ extern "C" jfb_status jfb_rope_paged_append(const void * q, const void * k, cons
     if (rows > 0x7fffffffu) return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_rope_paged_append: too many rows");
     if (rows == 0 || batch->sequences == 0) return status_ok();
     RopeParams p;
-    p.view = make_view(*cache, *batch, rows, error_flag);
+    p.view = make_view(*cache, *batch, rows, 1, 0, error_flag);
     p.q = q;
     p.k = k;
     p.v = v;

@@ -85,12 +85,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float * r) {
         : JFB_R8(r, 0), JFB_R8(r, 8), JFB_R8(r, 16), JFB_R8(r, 24)
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t * r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float * r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        JFB_W8(r, 0), JFB_W8(r, 8), JFB_W8(r, 16), JFB_W8(r, 24)
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : JFB_R8(r, 0), JFB_R8(r, 8)
+        : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t * r) {
     asm volatile(
@@ -119,19 +118,10 @@ __device__ __forceinline__ void add2(float & d0, float & d1, float a0, float a1)
         : "f"(a0), "f"(a1));
 }
 
-// The row (token i, head g of the group) of packed row r, as 16-byte pieces in
-// the K-major swizzled layout: row `at` of the [128][64] halves at `smem`.
-template <typename T, int D>
-__device__ __forceinline__ void store_row(uint8_t * smem, uint32_t at, const T * src, uint32_t head_dim) {
-    uint4 x[D / 8];
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-        x[c] = src != nullptr && uint32_t(c * 8) < head_dim ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-        *reinterpret_cast<uint4 *>(smem + (c >> 3) * kHalfBytes + at * 128 + (((c & 7) ^ (at & 7)) << 4)) = x[c];
-    }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 }  // namespace paged
