@@ -33,6 +33,7 @@ struct View {
     uint32_t group;      // query heads per kv head
     uint32_t window;     // 0: none
     uint32_t item_rows;  // packed rows of one item of the attention work
+    uint64_t slots;      // masses kept per sequence and kv head
     int32_t * error;
 };
 
@@ -244,15 +245,24 @@ __device__ __forceinline__ KeyRange key_range(const View & v, const Sequence & s
     return k;
 }
 
-struct Walk {
+// Items of a sequence and their parts: row tiles with their key tiles.
+struct RowItems {
+    using Part = KeyRange;
+    static __device__ __forceinline__ uint32_t count(const View & v, const Sequence & s) { return row_tiles(v, s); }
+    static __device__ __forceinline__ Part part(const View & v, const Sequence & s, uint32_t item) { return key_range(v, s, item); }
+};
+
+template <class Items>
+struct WalkOf {
     uint64_t unit, end;    // this CTA's line segment still to do
     uint64_t item0;        // first unit of the current item
     uint64_t total;        // units in all
     uint32_t ctas;         // CTAs that have work
     uint32_t kv_head, b, tile;
     Sequence s;
-    KeyRange k;
+    typename Items::Part k;
 };
+using Walk = WalkOf<RowItems>;
 
 // The CTA that holds `unit`.
 __device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t total, uint64_t ctas) {
@@ -267,15 +277,12 @@ __device__ __forceinline__ void walk_segment(const Walk & w, uint32_t & t0, uint
     t1 = b <= E ? 0u : b - E < w.k.tiles ? uint32_t(b - E) : w.k.tiles;
 }
 
-// Moves to the CTA's next segment with tiles; false at the end of its line.
-template <int E>
-__device__ __forceinline__ bool walk_next(const View & v, Walk & w) {
-    const uint64_t item_end = w.item0 + w.k.tiles + E;
-    // what is left of the line, if not tiles of another item, is the start of one
-    if (item_end + E >= w.end) return false;
-    w.unit = w.item0 = item_end;
+// Moves to the following item.
+template <int E, class Items>
+__device__ __forceinline__ void walk_item(const View & v, WalkOf<Items> & w) {
+    w.unit = w.item0 = w.item0 + w.k.tiles + E;
     ++w.tile;
-    while (w.tile >= row_tiles(v, w.s)) {
+    while (w.tile >= Items::count(v, w.s)) {
         w.tile = 0;
         if (++w.b >= v.sequences) {
             w.b = 0;
@@ -283,7 +290,15 @@ __device__ __forceinline__ bool walk_next(const View & v, Walk & w) {
         }
         w.s = load_sequence(v, w.b);
     }
-    w.k = key_range(v, w.s, w.tile);
+    w.k = Items::part(v, w.s, w.tile);
+}
+
+// Moves to the CTA's next segment with tiles; false at the end of its line.
+template <int E>
+__device__ __forceinline__ bool walk_next(const View & v, Walk & w) {
+    // what is left of the line, if not tiles of another item, is the start of one
+    if (w.item0 + w.k.tiles + 2 * E >= w.end) return false;
+    walk_item<E>(v, w);
     return true;
 }
 
@@ -304,27 +319,27 @@ __device__ __forceinline__ void walk_owners(const Walk & w, uint32_t & c0, uint3
     c1 = cta_of(w.item0 + E + w.k.tiles - 1, w.total, w.ctas);
 }
 
-// Positions `copies` (up to 32) Walks in shared memory at the CTA's first
-// segment. `cost` is shared scratch of one u64 per sequence, free
-// after the call. False when the CTA has no work.
-template <int E>
-static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks, uint32_t copies) {
+// Positions `x` (every lane of warp 0 gets it) at the unit where the line of
+// worker `index` of `workers` begins; unit == end when it has no work. All
+// threads call it; `cost` is shared scratch of one u64 per sequence.
+template <int E, class Items>
+__device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uint32_t index, uint32_t workers, WalkOf<Items> & x) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     // units of each sequence: a thread per sequence; the lanes of the warp
-    // share the row tiles of a sequence that has many
+    // share the items of a sequence that has many
     for (uint32_t base = warp * 32; base < v.sequences; base += warps * 32) {
         const uint32_t b = base + lane;
         Sequence s = {0, 0, 0};
-        uint32_t tiles = 0;
+        uint32_t items = 0;
         uint64_t units = 0;
         if (b < v.sequences) {
             s = load_sequence(v, b);
-            tiles = row_tiles(v, s);
-            if (tiles <= 4) {
-                for (uint32_t t = 0; t < tiles; ++t) units += key_range(v, s, t).tiles + E;
+            items = Items::count(v, s);
+            if (items <= 4) {
+                for (uint32_t i = 0; i < items; ++i) units += Items::part(v, s, i).tiles + E;
             }
         }
-        uint32_t many = __ballot_sync(0xffffffffu, tiles > 4);
+        uint32_t many = __ballot_sync(0xffffffffu, items > 4);
         while (many != 0) {
             const int src = __ffs(many) - 1;
             many &= many - 1;
@@ -332,9 +347,9 @@ static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks,
             o.q0 = 0;
             o.count = __shfl_sync(0xffffffffu, s.count, src);
             o.kv = __shfl_sync(0xffffffffu, s.kv, src);
-            const uint32_t n = __shfl_sync(0xffffffffu, tiles, src);
+            const uint32_t n = __shfl_sync(0xffffffffu, items, src);
             unsigned long long sum = 0;
-            for (uint32_t t = lane; t < n; t += 32) sum += key_range(v, o, t).tiles + E;
+            for (uint32_t i = lane; i < n; i += 32) sum += Items::part(v, o, i).tiles + E;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (int(lane) == src) units = sum;
@@ -342,67 +357,56 @@ static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks,
         if (b < v.sequences) cost[b] = units;
     }
     __syncthreads();
-    if (warp == 0) {
-        unsigned long long per_head = 0;
-        for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
+    if (warp != 0) return;
+    unsigned long long per_head = 0;
+    for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
-        Walk x;
-        x.total = uint64_t(per_head) * v.kv_heads;
-        x.ctas = uint64_t(gridDim.x) < x.total ? gridDim.x : uint32_t(x.total);
-        const bool work = blockIdx.x < x.ctas;
-        if (work) {
-            x.unit = uint64_t(blockIdx.x) * x.total / x.ctas;
-            x.end = uint64_t(blockIdx.x + 1) * x.total / x.ctas;
-            x.kv_head = uint32_t(x.unit / per_head);
-            unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;  // within the head's line
-            // the sequence: 32 prefix sums at a time
-            uint32_t b = 0;
-            for (uint32_t base = 0; base < v.sequences; base += 32) {
-                const unsigned long long mine = base + lane < v.sequences ? cost[base + lane] : 0ull;
-                unsigned long long upto = mine;
+    for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
+    x.total = uint64_t(per_head) * v.kv_heads;
+    x.ctas = uint64_t(workers) < x.total ? workers : uint32_t(x.total);
+    x.unit = x.end = 0;
+    if (index >= x.ctas) return;
+    x.unit = uint64_t(index) * x.total / x.ctas;
+    x.end = uint64_t(index + 1) * x.total / x.ctas;
+    x.kv_head = uint32_t(x.unit / per_head);
+    // the first entry of a list whose running sum exceeds what is left: 32 at a time
+    unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;
+    const auto find = [&](uint32_t n, auto value) {
+        uint32_t at = 0;
+        for (uint32_t base = 0; base < n; base += 32) {
+            const unsigned long long mine = base + lane < n ? value(base + lane) : 0ull;
+            unsigned long long upto = mine;
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (int(lane) >= d) upto += o;
-                }
-                const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
-                if (over != 0) {
-                    const int src = __ffs(over) - 1;
-                    b = base + src;
-                    left -= __shfl_sync(0xffffffffu, upto - mine, src);
-                    break;
-                }
-                left -= __shfl_sync(0xffffffffu, upto, 31);
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
+                if (int(lane) >= d) upto += o;
             }
-            x.b = b;
-            x.s = load_sequence(v, b);
-            // the row tile, the same way
-            const uint32_t tiles = row_tiles(v, x.s);
-            x.tile = 0;
-            for (uint32_t base = 0; base < tiles; base += 32) {
-                const unsigned long long mine =
-                    base + lane < tiles ? key_range(v, x.s, base + lane).tiles + E : 0ull;
-                unsigned long long upto = mine;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (int(lane) >= d) upto += o;
-                }
-                const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
-                if (over != 0) {
-                    const int src = __ffs(over) - 1;
-                    x.tile = base + src;
-                    left -= __shfl_sync(0xffffffffu, upto - mine, src);
-                    break;
-                }
-                left -= __shfl_sync(0xffffffffu, upto, 31);
+            const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
+            if (over != 0) {
+                const int src = __ffs(over) - 1;
+                at = base + src;
+                left -= __shfl_sync(0xffffffffu, upto - mine, src);
+                break;
             }
-            x.item0 = x.unit - left;
-            x.k = key_range(v, x.s, x.tile);
-        } else {
-            x.unit = x.end = 0;
+            left -= __shfl_sync(0xffffffffu, upto, 31);
         }
+        return at;
+    };
+    x.b = find(v.sequences, [&](uint32_t b) { return (unsigned long long)(cost[b]); });
+    x.s = load_sequence(v, x.b);
+    x.tile = find(Items::count(v, x.s), [&](uint32_t i) { return (unsigned long long)(Items::part(v, x.s, i).tiles + E); });
+    x.item0 = x.unit - left;
+    x.k = Items::part(v, x.s, x.tile);
+}
+
+// Positions `copies` (up to 32) Walks in shared memory at the CTA's first
+// segment. `cost` is shared scratch of one u64 per sequence, free after the
+// call. False when the CTA has no work.
+template <int E>
+static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks, uint32_t copies) {
+    Walk x;
+    walk_locate<E>(v, cost, blockIdx.x, gridDim.x, x);
+    if (threadIdx.x < 32) {
         bool any = x.unit < x.end;
         if (any) {
             uint32_t t0, t1;
@@ -410,7 +414,7 @@ static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks,
             any = t0 < t1 || walk_next<E>(v, x);
         }
         if (!any) x.unit = x.end = 0;
-        if (lane < copies) walks[lane] = x;
+        if (threadIdx.x < copies) walks[threadIdx.x] = x;
     }
     __syncthreads();
     return walks[0].unit < walks[0].end;
@@ -516,6 +520,7 @@ inline View make_view(const jfb_paged_cache & c, const jfb_paged_batch & b, uint
     v.group = group;
     v.window = window;
     v.item_rows = 0;
+    v.slots = 0;
     v.error = error;
     return v;
 }

@@ -207,12 +207,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                         if (moved > 0 && !wait(s_free, (moved - 1) & 1)) break;
                         ++moved;
                         tc_fence_after();
-                        const uint32_t qx = q_addr + x * kTileBytes<D>;
-#pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t at = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-                            mma_ss(tmem + kColS, desc_k_major(qx + at), desc_k_major(addr + at), instr_desc<T>(kTileKeys, false), kk > 0);
-                        }
+                        mma_scores<T, D>(tmem + kColS, q_addr + x * kTileBytes<D>, addr);
                         mma_commit(s_full + x);
                         if (j + two >= steps - 1) mma_commit(q_free + x);
                     } else {
@@ -424,20 +419,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
     if (warp == kWarpS) tmem_free(tmem);
 }
 
-// Query rows as (head_dim, heads, rows): boxes of 64 elements x the group x whole tokens.
-bool query_map(CUtensorMap & map, const AttentionParams & p, uint32_t tokens) {
-    PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
-    if (encode == nullptr) return false;
-    const cuuint64_t dims[3] = {p.view.head_dim, p.heads, p.view.rows};
-    const cuuint64_t strides[2] = {uint64_t(p.view.head_dim) * 2, p.q_stride * 2};
-    const cuuint32_t box[3] = {64, p.view.group, tokens};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    std::memset(&map, 0, sizeof(map));
-    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(p.q), dims, strides, box, elem,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int D>
 jfb_status launch(const TcMaps & maps, const AttentionParams & p, uint32_t tokens, uint32_t sms, cudaStream_t s) {
     // rows of whole 32-byte sectors
@@ -458,7 +439,7 @@ jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap 
     TcMaps maps;
     maps.k = k;
     maps.v = v;
-    if (!query_map(maps.q, p, tokens)) {
+    if (!query_map(maps.q, p.view, p.q, p.q_stride, p.heads, tokens)) {
         return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: could not encode a TMA tensor map");
     }
     const bool half = cache.dtype == JFB_DTYPE_F16;

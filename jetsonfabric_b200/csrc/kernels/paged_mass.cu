@@ -5,21 +5,11 @@
 // same key, and the order of every sum is fixed.
 #include "paged.cuh"
 #include "paged_attention.cuh"
+#include "paged_mass.cuh"
 
 namespace jfb {
 namespace paged {
 namespace {
-
-struct MassParams {
-    View view;
-    const void * q;
-    const float * lse;
-    const float * mass_in;
-    float * mass_out;
-    uint64_t q_stride, mass_stride;
-    uint32_t heads;
-    float scale;
-};
 
 // ---- few rows -----------------------------------------------------------------------
 //
@@ -154,7 +144,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     pdl_wait();
     const View & v = p.view;
     KeyWalk w;
-    if (!key_walk_begin(v, p.mass_stride, reinterpret_cast<uint32_t *>(smem), reinterpret_cast<KeyWalk *>(smem + L::kWalk), w)) return;
+    if (!key_walk_begin(v, v.slots, reinterpret_cast<uint32_t *>(smem), reinterpret_cast<KeyWalk *>(smem + L::kWalk), w)) return;
     fence_proxy_async();  // the ring held the walk's scratch
     __syncthreads();
 
@@ -169,7 +159,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         for (bool more = true; more; ++n) {
             const TileLoad load = next;
             const uint32_t head = w.kv_head;
-            more = key_walk_next(v, p.mass_stride, w);
+            more = key_walk_next(v, v.slots, w);
             if (more) next = pages_of(w);
             const uint32_t st = n % L::kStages, turn = n / L::kStages;
             if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
@@ -260,7 +250,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor_sync(0xffffffffu, acc[x], d);
             }
             if (grp == 0) {
-                const uint64_t line = (uint64_t(w.b) * v.kv_heads + w.kv_head) * p.mass_stride;
+                const uint64_t line = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const uint32_t k = key + (x >> 1) * 8 + tig * 2 + (x & 1);
@@ -271,7 +261,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 }
             }
         }
-    } while (key_walk_next(v, p.mass_stride, w));
+    } while (key_walk_next(v, v.slots, w));
 }
 
 template <typename T, int D>
@@ -310,12 +300,12 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     if (batch->sequences == 0) return status_ok();
     MassParams p;
     p.view = make_view(*cache, *batch, rows, heads / cache->kv_heads, window, error_flag);
+    p.view.slots = mass_stride;
     p.q = q;
     p.lse = lse;
     p.mass_in = mass_in;
     p.mass_out = mass_out;
     p.q_stride = q_stride;
-    p.mass_stride = mass_stride;
     p.heads = heads;
     p.scale = scale;
     CUtensorMap mk;
@@ -324,6 +314,8 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     }
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
+    const uint32_t group = p.view.group;
+    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_mass_tc(*cache, mk, p, sms, s);
     if (cache->head_dim <= 64) {
         return half ? launch_rows<__half, 64>(mk, p, sms, s) : launch_rows<__nv_bfloat16, 64>(mk, p, sms, s);
     }

@@ -1,0 +1,433 @@
+// The attention weight each cached key received from chunks of new tokens, on
+// the tcgen05 tensor cores.
+//
+// The keys are the M side, so that every sum over rows stays in one thread: an
+// item is 128 keys of one sequence and kv head, its steps the row tiles (128 / G
+// whole tokens) that see any of them, S^T = K Q^T of a step 128 x 128 scores. A
+// step costs one exponential per score, 1024 cycles of the unit against 512 of
+// the tensor pipe, so the exponentials bound the time. A cluster of 4 CTAs
+// takes an item, every fourth step each, and adds the four sums over
+// distributed shared memory: few long items still fill the SMs, and no
+// workspace or order of arrival is involved. Clusters take whole items off the
+// evenly divided line of units (walk_locate).
+//   warps 0-3, 4-7  sums of the even and the odd steps, a thread per key;
+//   warp 8          the MMAs, up to four steps ahead (S takes all of the 512
+//                   columns of tensor memory);
+//   warp 9          K tiles and queries through TMA;
+//   warp 10         each row's -lse and slot.
+#include "paged_attention.cuh"
+#include "paged_mass.cuh"
+#include "paged_tc.cuh"
+
+namespace jfb {
+namespace paged {
+namespace {
+
+constexpr int kItemMass = 8;  // units of an item's start and end
+constexpr int kThreadsMass = 384;
+constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpLse = 10;
+constexpr uint32_t kCluster = 4;
+constexpr uint32_t kScores = 4;   // S tiles in tensor memory
+constexpr uint32_t kLseRing = 8;  // steps of row data ahead
+
+// Items of a sequence: its key tiles with the row tiles that see them.
+struct KeyItems {
+    struct Part {
+        uint32_t first, tiles;  // row tiles [first, first + tiles)
+    };
+    static __device__ __forceinline__ uint32_t limit(const View & v, const Sequence & s) {
+        if (s.kv <= v.slots) return s.kv;
+        flag_error(v.error, JFB_PAGED_ERROR_RANGE);
+        return uint32_t(v.slots);
+    }
+    static __device__ __forceinline__ uint32_t count(const View & v, const Sequence & s) {
+        return (limit(v, s) + kTileKeys - 1) / kTileKeys;
+    }
+    static __device__ __forceinline__ Part part(const View & v, const Sequence & s, uint32_t item) {
+        const uint32_t tokens = v.item_rows / v.group;
+        const int64_t first = int64_t(s.kv) - s.count, key0 = int64_t(item) * kTileKeys;
+        const int64_t key1 = key0 + kTileKeys < limit(v, s) ? key0 + kTileKeys : limit(v, s);
+        const int64_t i0 = key0 > first ? key0 - first : 0;  // tokens [i0, i1) see some key of the tile
+        int64_t i1 = s.count;
+        if (v.window > 0 && key1 - 1 + v.window - first < i1) i1 = key1 - 1 + v.window - first;
+        Part p = {0, 0};
+        if (i0 < i1) {
+            p.first = uint32_t(i0) / tokens;
+            p.tiles = (uint32_t(i1) + tokens - 1) / tokens - p.first;
+        }
+        return p;
+    }
+};
+using KeyTileWalk = WalkOf<KeyItems>;
+
+template <int D>
+struct MassTcSmem {
+    static constexpr uint32_t kQStages = D == 128 ? 4 : 8;
+    static constexpr uint32_t kQ = 2 * kTileBytes<D>;  // two K tiles first
+    static constexpr uint32_t kRows = kQ + kQStages * kTileBytes<D>;  // [ring][128] (-lse log2 e, slot)
+    static constexpr uint32_t kSums = kRows + kLseRing * 128 * 8;     // [2][cluster][128], and [128] of the odd steps
+    static constexpr uint32_t kBars = kSums + (2 * kCluster + 1) * 128 * 4;
+    static constexpr uint32_t kNumBars = 4 + 2 * kQStages + 2 * kScores + 2 * kLseRing + 4;
+    static constexpr uint32_t kWalk = kBars + kNumBars * 8;
+    static constexpr uint32_t kFlags = kWalk + kThreadsMass / 32 * sizeof(KeyTileWalk);  // abort, tmem
+    static constexpr uint32_t kBytes = kFlags + 32;
+};
+static_assert(MassTcSmem<128>::kBytes <= 232448 && MassTcSmem<64>::kBytes <= 232448);
+static_assert(MassTcSmem<64>::kBars >= JFB_PAGED_MAX_SEQUENCES * 8);
+
+struct MassMaps {
+    CUtensorMap k, q;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address of `p` in the CTA of cluster rank `rank`.
+__device__ __forceinline__ uint32_t remote(const void * p, uint32_t rank) {
+    uint32_t out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_u32(p)), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ void remote_store(const float * p, uint32_t rank, float x) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(p, rank)), "f"(x) : "memory");
+}
+// Releases the calling thread's (and, after a warp barrier and fence, its warp's) accesses.
+__device__ __forceinline__ void remote_arrive(uint64_t * bar, uint32_t rank) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(bar, rank)) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int32_t * error) {
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
+            : "memory");
+        if (ok != 0) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitNs) break;
+    }
+    *abort_flag = 1;
+    flag_error(error, JFB_PAGED_ERROR_TIMEOUT);
+    return false;
+}
+
+// The next item whose first unit lies in the cluster's part of the line.
+__device__ __forceinline__ bool next_item(const View & v, KeyTileWalk * w) {
+    __syncwarp();
+    int more = 0;
+    if ((threadIdx.x & 31) == 0 && w->item0 + w->k.tiles + kItemMass < w->end) {
+        walk_item<kItemMass>(v, *w);
+        more = 1;
+    }
+    return __shfl_sync(0xffffffffu, more, 0) != 0;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreadsMass, 1)
+    mass_tc_kernel(const __grid_constant__ MassMaps maps, const MassParams p, const uint32_t tokens) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    using L = MassTcSmem<D>;
+    uint64_t * k_full = reinterpret_cast<uint64_t *>(smem + L::kBars);
+    uint64_t * k_free = k_full + 2;
+    uint64_t * q_full = k_free + 2;
+    uint64_t * q_free = q_full + L::kQStages;
+    uint64_t * s_full = q_free + L::kQStages;
+    uint64_t * s_free = s_full + kScores;
+    uint64_t * r_full = s_free + kScores;
+    uint64_t * r_free = r_full + kLseRing;
+    uint64_t * sum_full = r_free + kLseRing;  // of the leader: the cluster's sums of an even or odd item are in
+    uint64_t * sum_free = sum_full + 2;       // of every CTA: the leader has used them
+    volatile int * flags = reinterpret_cast<volatile int *>(smem + L::kFlags);
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kFlags + 16);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(k_full + i, 1);
+            mbar_init(k_free + i, 1);
+            mbar_init(sum_full + i, 4 * kCluster);
+            mbar_init(sum_free + i, 1);
+        }
+        for (uint32_t i = 0; i < L::kQStages; ++i) {
+            mbar_init(q_full + i, 1);
+            mbar_init(q_free + i, 1);
+        }
+        for (uint32_t i = 0; i < kScores; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(s_free + i, 4);
+        }
+        for (uint32_t i = 0; i < kLseRing; ++i) {
+            mbar_init(r_full + i, 1);
+            mbar_init(r_free + i, 4);
+        }
+        flags[0] = 0;
+        mbar_init_fence();
+    }
+    pdl_trigger();
+    pdl_wait();
+    const View & v = p.view;
+    KeyTileWalk * walks = reinterpret_cast<KeyTileWalk *>(smem + L::kWalk);
+    KeyTileWalk start;
+    walk_locate<kItemMass>(v, reinterpret_cast<uint64_t *>(smem), blockIdx.x / kCluster, gridDim.x / kCluster, start);
+    if (warp == 0) {
+        if (start.unit < start.end && start.item0 < start.unit) {  // that item began in another cluster's part
+            if (start.item0 + start.k.tiles + kItemMass < start.end) walk_item<kItemMass>(v, start);
+            else start.unit = start.end;
+        }
+        if (lane < kThreadsMass / 32) walks[lane] = start;
+    }
+    __syncthreads();
+    KeyTileWalk & w = walks[warp];
+    const bool work = walks[0].unit < walks[0].end && (smem_u32(smem) & 1023u) == 0;
+    // rows that no query fills stay zero (and this held the walk's scratch)
+    for (uint32_t i = threadIdx.x; i < L::kRows / 16; i += kThreadsMass) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+    if (warp == kWarpMma) tmem_alloc(tmem_slot);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    cluster_sync();  // every CTA's barriers are initialised before any remote arrival
+    const uint32_t tmem = *tmem_slot;
+    bool ok = work;
+    auto wait = [&](uint64_t * bar, uint32_t parity) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, flags, v.error));
+        return ok;
+    };
+    // this CTA's steps of an item are row tiles k.first + rank, + kCluster, ...; s counts its steps over all items
+    uint32_t s = 0;
+
+    if (warp == kWarpLoad) {
+        uint32_t item = 0;
+        for (bool more = work; ok && more; ++item) {
+            const uint32_t kb = item & 1, turn = item >> 1, key0 = w.tile * kTileKeys;
+            const uint32_t key1 = min(KeyItems::limit(v, w.s), key0 + uint32_t(kTileKeys));
+            const TileLoad load = tile_pages(v, v.table + uint64_t(w.b) * v.table_stride, key0, key1);
+            if (turn > 0 && !wait(k_free + kb, (turn - 1) & 1)) break;
+            tile_issue<D>(load, &maps.k, w.kv_head, smem_u32(smem) + kb * kTileBytes<D>, k_full + kb);
+            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+                const uint32_t st = s % L::kQStages;
+                if (s >= L::kQStages && !wait(q_free + st, (s / L::kQStages - 1) & 1)) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(q_full + st, tokens * v.group * D * 2);
+                    for (int h = 0; h < D / 64; ++h) {
+                        tma_load_rows(smem_u32(smem) + L::kQ + st * kTileBytes<D> + h * kHalfBytes, &maps.q, h * 64,
+                                      int32_t(w.kv_head * v.group), int32_t(w.s.q0 + (w.k.first + i) * tokens), q_full + st);
+                    }
+                }
+                __syncwarp();
+            }
+            more = next_item(v, &w);
+        }
+        if (flags[0]) {
+            for (uint32_t i = item >= 2 ? item - 2 : 0u; i < item; ++i) mbar_drain(k_full + (i & 1), (i >> 1) & 1);
+            for (uint32_t i = s >= L::kQStages ? s - L::kQStages : 0u; i < s; ++i) {
+                mbar_drain(q_full + i % L::kQStages, (i / L::kQStages) & 1);
+            }
+        }
+    } else if (warp == kWarpMma) {
+        uint32_t item = 0;
+        for (bool more = work; ok && more; ++item) {
+            const uint32_t kb = item & 1;
+            if (!wait(k_full + kb, (item >> 1) & 1)) break;
+            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+                const uint32_t st = s % L::kQStages, buf = s % kScores;
+                if (!wait(q_full + st, (s / L::kQStages) & 1)) break;
+                if (s >= kScores && !wait(s_free + buf, (s / kScores - 1) & 1)) break;
+                tc_fence_after();
+                mma_scores<T, D>(tmem + buf * 128, smem_u32(smem) + kb * kTileBytes<D>, smem_u32(smem) + L::kQ + st * kTileBytes<D>);
+                mma_commit(s_full + buf);
+                mma_commit(q_free + st);
+            }
+            mma_commit(k_free + kb);
+            more = next_item(v, &w);
+        }
+        if (flags[0]) {  // MMAs in flight finish before tensor memory is given back
+            const uint64_t t = global_ns();
+            while (global_ns() - t < 10000000ull) __nanosleep(1000);
+        }
+    } else if (warp == kWarpLse) {
+        float2 * ring = reinterpret_cast<float2 *>(smem + L::kRows);
+        uint32_t token[4], head[4];  // of this lane's four rows
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            token[e] = (lane + 32 * e) / v.group;
+            head[e] = lane + 32 * e - token[e] * v.group;
+        }
+        for (bool more = work; ok && more;) {
+            const int64_t first = int64_t(w.s.kv) - w.s.count;
+            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+                const uint32_t st = s % kLseRing, token0 = (w.k.first + i) * tokens;
+                float2 x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // rows of no token: weight 0, and before every slot
+                    const bool valid = token[e] < tokens && token0 + token[e] < w.s.count;
+                    x[e].x = valid ? -kLog2e * p.lse[uint64_t(w.s.q0 + token0 + token[e]) * p.heads + w.kv_head * v.group + head[e]] : -INFINITY;
+                    x[e].y = __int_as_float(valid ? int32_t(first + token0 + token[e]) : -1);
+                }
+                if (s >= kLseRing && !wait(r_free + st, (s / kLseRing - 1) & 1)) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ring[st * 128 + lane + 32 * e] = x[e];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(r_full + st);
+            }
+            more = next_item(v, &w);
+        }
+    } else if (warp < 8) {
+        const uint32_t odd = warp >> 2, key = threadIdx.x & 127;
+        const uint32_t lanes = tmem + ((warp & 3) << 21);
+        const float scale2 = p.scale * kLog2e;
+        const float2 * ring = reinterpret_cast<const float2 *>(smem + L::kRows);
+        float * sums = reinterpret_cast<float *>(smem + L::kSums);
+        float * odd_sums = sums + 2 * kCluster * 128;
+        uint32_t item = 0;
+        for (bool more = work; more; ++item) {
+            const int64_t first = int64_t(w.s.kv) - w.s.count;
+            const uint32_t key0 = w.tile * kTileKeys, at = key0 + key;
+            float total = 0.0f;
+            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+                // after a wait that gave up the steps are skipped; the warps still meet at the barriers below
+                if ((s & 1) != odd || !ok) continue;
+                const uint32_t buf = s % kScores, st = s % kLseRing;
+                const uint32_t token0 = (w.k.first + i) * tokens;
+                const int64_t pos0 = first + token0, pos1 = pos0 + tokens - 1;
+                const bool edge = token0 + tokens > w.s.count || pos0 < int64_t(key0) + kTileKeys - 1 ||
+                                  (v.window > 0 && int64_t(key0) <= pos1 - int64_t(v.window));
+                if (!wait(r_full + st, (s / kLseRing) & 1) || !wait(s_full + buf, (s / kScores) & 1)) continue;
+                tc_fence_after();
+                const float4 * rows = reinterpret_cast<const float4 *>(ring + st * 128);
+                float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[32];
+                    tmem_ld32(lanes + buf * 128 + c * 32, x);
+                    tmem_wait_ld();
+                    if (c == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_free + buf);
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float4 r = rows[c * 16 + j / 2];
+                            float e0, e1;
+                            fma2(e0, e1, x[j], x[j + 1], scale2, r.x, r.z);
+                            e0 = exp2_approx(e0);
+                            e1 = exp2_approx(e1);
+                            const int32_t p0 = __float_as_int(r.y), p1 = __float_as_int(r.w), k = int32_t(at);
+                            e0 = k <= p0 && (v.window == 0 || k > p0 - int32_t(v.window)) ? e0 : 0.0f;
+                            e1 = k <= p1 && (v.window == 0 || k > p1 - int32_t(v.window)) ? e1 : 0.0f;
+                            add2(a0, a1, e0, e1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float4 r = rows[c * 16 + j / 2];
+                            float e0, e1;
+                            fma2(e0, e1, x[j], x[j + 1], scale2, r.x, r.z);
+                            add2(a0, a1, exp2_approx(e0), exp2_approx(e1));
+                        }
+                    }
+                }
+                total += a0 + a1;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(r_free + st);
+            }
+            // odd steps' sums to the even ones' threads, theirs to the leader's
+            const uint32_t q = item & 1, turn = item >> 1;
+            if (odd) odd_sums[key] = total;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (!odd) {
+                total += odd_sums[key];
+                if (turn > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(sum_free + q, (turn - 1) & 1, flags, v.error));
+                if (ok) {
+                    remote_store(sums + (q * kCluster + rank) * 128 + key, 0, total);
+                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) remote_arrive(sum_full + q, 0);
+                }
+                if (rank == 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait_cluster(sum_full + q, turn & 1, flags, v.error));
+                if (rank == 0) {
+                    if (ok && at < KeyItems::limit(v, w.s)) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (uint32_t r = 0; r < kCluster; ++r) sum += sums[(q * kCluster + r) * 128 + key];
+                        const uint64_t to = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots + at;
+                        const float before = p.mass_in != nullptr && int64_t(at) < first ? p.mass_in[to] : 0.0f;
+                        p.mass_out[to] = before + sum;
+                    }
+                    asm volatile("bar.sync 2, 128;" ::: "memory");
+                    if (warp == 0 && lane < kCluster) remote_arrive(sum_free + q, lane);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // odd_sums may be written again
+            more = next_item(v, &w);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kWarpMma) tmem_free(tmem);
+    cluster_sync();  // no CTA leaves while another may still reach its shared memory
+}
+
+template <typename T, int D>
+jfb_status launch(const MassMaps & maps, const MassParams & p, uint32_t tokens, uint32_t sms, cudaStream_t s) {
+    auto kernel = mass_tc_kernel<T, D>;
+    cudaError_t e = allow_smem(kernel, MassTcSmem<D>::kBytes);
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreadsMass);
+    cfg.dynamicSmemBytes = MassTcSmem<D>::kBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    // as many clusters as the GPCs hold at once: the line is divided evenly among them
+    cfg.gridDim = dim3(sms / kCluster * kCluster);
+    if (e == cudaSuccess) {
+        static std::mutex mu;
+        static int known[64] = {0};  // per device
+        int device = 0;
+        e = cudaGetDevice(&device);
+        const std::lock_guard<std::mutex> lock(mu);
+        int n = device >= 0 && device < 64 ? known[device] : 0;
+        if (e == cudaSuccess && n == 0) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        if (e == cudaSuccess && n < 1) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no room for a cluster");
+        if (device >= 0 && device < 64) known[device] = n;
+        cfg.gridDim = dim3(uint32_t(n) < sms / kCluster ? uint32_t(n) * kCluster : sms / kCluster * kCluster);
+    }
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, maps, p, tokens);
+    if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: %s", cudaGetErrorString(e));
+    return launch_status("jfb_paged_attention_mass");
+}
+
+}  // namespace
+
+jfb_status launch_mass_tc(const jfb_paged_cache & cache, const CUtensorMap & k, MassParams p, uint32_t sms, cudaStream_t s) {
+    const uint32_t tokens = 128 / p.view.group;
+    p.view.item_rows = tokens * p.view.group;
+    MassMaps maps;
+    maps.k = k;
+    if (!query_map(maps.q, p.view, p.q, p.q_stride, p.heads, tokens)) {
+        return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: could not encode a TMA tensor map");
+    }
+    const bool half = cache.dtype == JFB_DTYPE_F16;
+    if (cache.head_dim <= 64) return half ? launch<__half, 64>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 64>(maps, p, tokens, sms, s);
+    return half ? launch<__half, 128>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 128>(maps, p, tokens, sms, s);
+}
+
+}  // namespace paged
+}  // namespace jfb

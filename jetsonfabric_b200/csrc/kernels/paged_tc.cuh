@@ -74,6 +74,16 @@ __device__ __forceinline__ void mma_commit(uint64_t * bar) {
         : "memory");
 }
 
+// The 128 x 128 scores of two K-major tiles of D columns.
+template <typename T, int D>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t at = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+        mma_ss(d, desc_k_major(a + at), desc_k_major(b + at), instr_desc<T>(kTileKeys, false), kk > 0);
+    }
+}
+
 #define JFB_R8(r, i) "=f"(r[i]), "=f"(r[i + 1]), "=f"(r[i + 2]), "=f"(r[i + 3]), "=f"(r[i + 4]), "=f"(r[i + 5]), "=f"(r[i + 6]), "=f"(r[i + 7])
 #define JFB_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
 
@@ -110,6 +120,13 @@ __device__ __forceinline__ void fma2(float & d0, float & d1, float a0, float a1,
         : "=f"(d0), "=f"(d1)
         : "f"(a0), "f"(a1), "f"(b), "f"(c));
 }
+__device__ __forceinline__ void fma2(float & d0, float & d1, float a0, float a1, float b, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %6};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ void add2(float & d0, float & d1, float a0, float a1) {
     asm("{\n\t.reg .b64 a, d;\n\t"
         "mov.b64 a, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\t"
@@ -122,6 +139,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+// Query rows as (head_dim, heads, rows): boxes of 64 elements x the group x
+// `tokens` rows, so a box's rows are packed rows (token, head of the group).
+inline bool query_map(CUtensorMap & map, const View & v, const void * q, uint64_t q_stride, uint32_t heads, uint32_t tokens) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[3] = {v.head_dim, heads, v.rows};
+    const cuuint64_t strides[2] = {uint64_t(v.head_dim) * 2, q_stride * 2};
+    const cuuint32_t box[3] = {64, v.group, tokens};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    std::memset(&map, 0, sizeof(map));
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(q), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace paged
