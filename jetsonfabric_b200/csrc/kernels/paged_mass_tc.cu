@@ -2,16 +2,18 @@
 // the tcgen05 tensor cores.
 //
 // The keys are the M side, so that every sum over rows stays in one thread: an
-// item is 128 keys of one sequence and kv head, its steps the row tiles (128 / G
-// whole tokens) that see any of them, S^T = K Q^T of a step 128 x 128 scores. A
-// step costs one exponential per score, 1024 cycles of the unit against 512 of
-// the tensor pipe, so the exponentials bound the time. A cluster of 4 CTAs
-// takes an item, every fourth step each, and adds the four sums over
-// distributed shared memory: few long items still fill the SMs, and no
-// workspace or order of arrival is involved. Clusters take whole items off the
-// evenly divided line of units (walk_locate).
-//   warps 0-3, 4-7  sums of the even and the odd steps, a thread per key;
-//   warp 8          the MMAs, up to four steps ahead (S takes all of the 512
+// item is 256 keys of one sequence and kv head, two key tiles, its steps the
+// row tiles (128 / G whole tokens) that see any of them, S^T = K Q^T of a step
+// 2 x 128 x 128 scores. A step costs one exponential per score, 2048 cycles of
+// the unit against 1024 of the tensor pipe and 32 KB of queries, so the
+// exponentials bound the time (with 128 keys an item the queries' way from L2
+// did: 250 us instead of @@). A cluster of 4 CTAs takes an item, every fourth
+// step each, and adds the four sums over distributed shared memory: few long
+// items still fill the SMs, and no workspace or order of arrival is involved.
+// Clusters take whole items off the evenly divided line of units
+// (walk_locate), each the items whose middle lies in its part.
+//   warps 0-3, 4-7  sums of key tile 0 and 1, a thread per key;
+//   warp 8          the MMAs, up to two steps ahead (S takes all of the 512
 //                   columns of tensor memory);
 //   warp 9          K tiles and queries through TMA;
 //   warp 10         each row's -lse and slot.
@@ -27,10 +29,10 @@ constexpr int kItemMass = 8;  // units of an item's start and end
 constexpr int kThreadsMass = 384;
 constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpLse = 10;
 constexpr uint32_t kCluster = 4;
-constexpr uint32_t kScores = 4;   // S tiles in tensor memory
+constexpr uint32_t kItemKeys = 2 * kTileKeys;
 constexpr uint32_t kLseRing = 8;  // steps of row data ahead
 
-// Items of a sequence: its key tiles with the row tiles that see them.
+// Items of a sequence: its pairs of key tiles with the row tiles that see them.
 struct KeyItems {
     struct Part {
         uint32_t first, tiles;  // row tiles [first, first + tiles)
@@ -41,12 +43,12 @@ struct KeyItems {
         return uint32_t(v.slots);
     }
     static __device__ __forceinline__ uint32_t count(const View & v, const Sequence & s) {
-        return (limit(v, s) + kTileKeys - 1) / kTileKeys;
+        return (limit(v, s) + kItemKeys - 1) / kItemKeys;
     }
     static __device__ __forceinline__ Part part(const View & v, const Sequence & s, uint32_t item) {
         const uint32_t tokens = v.item_rows / v.group;
-        const int64_t first = int64_t(s.kv) - s.count, key0 = int64_t(item) * kTileKeys;
-        const int64_t key1 = key0 + kTileKeys < limit(v, s) ? key0 + kTileKeys : limit(v, s);
+        const int64_t first = int64_t(s.kv) - s.count, key0 = int64_t(item) * kItemKeys;
+        const int64_t key1 = key0 + kItemKeys < limit(v, s) ? key0 + kItemKeys : limit(v, s);
         const int64_t i0 = key0 > first ? key0 - first : 0;  // tokens [i0, i1) see some key of the tile
         int64_t i1 = s.count;
         if (v.window > 0 && key1 - 1 + v.window - first < i1) i1 = key1 - 1 + v.window - first;
@@ -63,11 +65,11 @@ using KeyTileWalk = WalkOf<KeyItems>;
 template <int D>
 struct MassTcSmem {
     static constexpr uint32_t kQStages = D == 128 ? 4 : 8;
-    static constexpr uint32_t kQ = 2 * kTileBytes<D>;  // two K tiles first
+    static constexpr uint32_t kQ = 2 * kTileBytes<D>;  // the two K tiles first
     static constexpr uint32_t kRows = kQ + kQStages * kTileBytes<D>;  // [ring][128] (-lse log2 e, slot)
-    static constexpr uint32_t kSums = kRows + kLseRing * 128 * 8;     // [2][cluster][128], and [128] of the odd steps
-    static constexpr uint32_t kBars = kSums + (2 * kCluster + 1) * 128 * 4;
-    static constexpr uint32_t kNumBars = 4 + 2 * kQStages + 2 * kScores + 2 * kLseRing + 4;
+    static constexpr uint32_t kSums = kRows + kLseRing * 128 * 8;     // [key tile][2][cluster][128]
+    static constexpr uint32_t kBars = kSums + 2 * 2 * kCluster * 128 * 4;
+    static constexpr uint32_t kNumBars = 2 + 2 * kQStages + 8 + 2 * kLseRing + 8;
     static constexpr uint32_t kWalk = kBars + kNumBars * 8;
     static constexpr uint32_t kFlags = kWalk + kThreadsMass / 32 * sizeof(KeyTileWalk);  // abort, tmem
     static constexpr uint32_t kBytes = kFlags + 32;
@@ -120,15 +122,21 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t * bar, uint32_t parit
     return false;
 }
 
-// The next item whose first unit lies in the cluster's part of the line.
+// The next item, if its middle lies in the cluster's part of the line.
+__device__ __forceinline__ bool step_item(const View & v, KeyTileWalk & w) {
+    if (w.item0 + w.k.tiles + kItemMass >= w.end) return false;
+    walk_item<kItemMass>(v, w);
+    return w.item0 + (w.k.tiles + kItemMass) / 2 < w.end;
+}
 __device__ __forceinline__ bool next_item(const View & v, KeyTileWalk * w) {
     __syncwarp();
     int more = 0;
-    if ((threadIdx.x & 31) == 0 && w->item0 + w->k.tiles + kItemMass < w->end) {
-        walk_item<kItemMass>(v, *w);
-        more = 1;
-    }
+    if ((threadIdx.x & 31) == 0) more = step_item(v, *w);
     return __shfl_sync(0xffffffffu, more, 0) != 0;
+}
+// Whether the item has keys in its second tile.
+__device__ __forceinline__ bool two_key_tiles(const View & v, const KeyTileWalk & w) {
+    return KeyItems::limit(v, w.s) > w.tile * kItemKeys + kTileKeys;
 }
 
 template <typename T, int D>
@@ -137,36 +145,34 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
     extern __shared__ __align__(1024) uint8_t smem[];
     using L = MassTcSmem<D>;
     uint64_t * k_full = reinterpret_cast<uint64_t *>(smem + L::kBars);
-    uint64_t * k_free = k_full + 2;
-    uint64_t * q_full = k_free + 2;
+    uint64_t * k_free = k_full + 1;
+    uint64_t * q_full = k_free + 1;
     uint64_t * q_free = q_full + L::kQStages;
-    uint64_t * s_full = q_free + L::kQStages;
-    uint64_t * s_free = s_full + kScores;
-    uint64_t * r_full = s_free + kScores;
+    uint64_t * s_full = q_free + L::kQStages;  // [key tile][2]
+    uint64_t * s_free = s_full + 4;
+    uint64_t * r_full = s_free + 4;
     uint64_t * r_free = r_full + kLseRing;
-    uint64_t * sum_full = r_free + kLseRing;  // of the leader: the cluster's sums of an even or odd item are in
-    uint64_t * sum_free = sum_full + 2;       // of every CTA: the leader has used them
+    uint64_t * sum_full = r_free + kLseRing;  // [key tile][2], of the leader: the cluster's sums of an even or odd item are in
+    uint64_t * sum_free = sum_full + 4;       // of every CTA: the leader has used them
     volatile int * flags = reinterpret_cast<volatile int *>(smem + L::kFlags);
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kFlags + 16);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank();
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(k_full + i, 1);
-            mbar_init(k_free + i, 1);
-            mbar_init(sum_full + i, 4 * kCluster);
-            mbar_init(sum_free + i, 1);
-        }
+        mbar_init(k_full, 2);  // both key tiles
+        mbar_init(k_free, 1);
         for (uint32_t i = 0; i < L::kQStages; ++i) {
             mbar_init(q_full + i, 1);
             mbar_init(q_free + i, 1);
         }
-        for (uint32_t i = 0; i < kScores; ++i) {
+        for (uint32_t i = 0; i < 4; ++i) {
             mbar_init(s_full + i, 1);
             mbar_init(s_free + i, 4);
+            mbar_init(sum_full + i, 4 * kCluster);
+            mbar_init(sum_free + i, 1);
         }
         for (uint32_t i = 0; i < kLseRing; ++i) {
             mbar_init(r_full + i, 1);
-            mbar_init(r_free + i, 4);
+            mbar_init(r_free + i, 8);
         }
         flags[0] = 0;
         mbar_init_fence();
@@ -178,9 +184,10 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
     KeyTileWalk start;
     walk_locate<kItemMass>(v, reinterpret_cast<uint64_t *>(smem), blockIdx.x / kCluster, gridDim.x / kCluster, start);
     if (warp == 0) {
-        if (start.unit < start.end && start.item0 < start.unit) {  // that item began in another cluster's part
-            if (start.item0 + start.k.tiles + kItemMass < start.end) walk_item<kItemMass>(v, start);
-            else start.unit = start.end;
+        if (start.unit < start.end) {
+            const uint64_t middle = start.item0 + (start.k.tiles + kItemMass) / 2;
+            // an item whose middle lies before or behind this part is another cluster's
+            if (middle >= start.end || (middle < start.unit && !step_item(v, start))) start.unit = start.end;
         }
         if (lane < kThreadsMass / 32) walks[lane] = start;
     }
@@ -207,11 +214,14 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
     if (warp == kWarpLoad) {
         uint32_t item = 0;
         for (bool more = work; ok && more; ++item) {
-            const uint32_t kb = item & 1, turn = item >> 1, key0 = w.tile * kTileKeys;
-            const uint32_t key1 = min(KeyItems::limit(v, w.s), key0 + uint32_t(kTileKeys));
-            const TileLoad load = tile_pages(v, v.table + uint64_t(w.b) * v.table_stride, key0, key1);
-            if (turn > 0 && !wait(k_free + kb, (turn - 1) & 1)) break;
-            tile_issue<D>(load, &maps.k, w.kv_head, smem_u32(smem) + kb * kTileBytes<D>, k_full + kb);
+            const uint32_t key0 = w.tile * kItemKeys, limit = KeyItems::limit(v, w.s);
+            const int32_t * row = v.table + uint64_t(w.b) * v.table_stride;
+            const TileLoad k0 = tile_pages(v, row, key0, min(limit, key0 + uint32_t(kTileKeys)));
+            const uint32_t key1 = min(limit, key0 + uint32_t(kTileKeys));
+            const TileLoad k1 = tile_pages(v, row, key1, min(limit, key0 + kItemKeys));
+            if (item > 0 && !wait(k_free, (item - 1) & 1)) break;
+            tile_issue<D>(k0, &maps.k, w.kv_head, smem_u32(smem), k_full);
+            tile_issue<D>(k1, &maps.k, w.kv_head, smem_u32(smem) + kTileBytes<D>, k_full);
             for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
                 const uint32_t st = s % L::kQStages;
                 if (s >= L::kQStages && !wait(q_free + st, (s / L::kQStages - 1) & 1)) break;
@@ -227,26 +237,29 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             more = next_item(v, &w);
         }
         if (flags[0]) {
-            for (uint32_t i = item >= 2 ? item - 2 : 0u; i < item; ++i) mbar_drain(k_full + (i & 1), (i >> 1) & 1);
+            if (item > 0) mbar_drain(k_full, (item - 1) & 1);
             for (uint32_t i = s >= L::kQStages ? s - L::kQStages : 0u; i < s; ++i) {
                 mbar_drain(q_full + i % L::kQStages, (i / L::kQStages) & 1);
             }
         }
     } else if (warp == kWarpMma) {
-        uint32_t item = 0;
+        uint32_t item = 0, s1 = 0;  // steps of items with a second key tile
         for (bool more = work; ok && more; ++item) {
-            const uint32_t kb = item & 1;
-            if (!wait(k_full + kb, (item >> 1) & 1)) break;
+            const bool two = two_key_tiles(v, w);
+            if (!wait(k_full, item & 1)) break;
             for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
-                const uint32_t st = s % L::kQStages, buf = s % kScores;
+                const uint32_t st = s % L::kQStages, q_addr = smem_u32(smem) + L::kQ + st * kTileBytes<D>;
                 if (!wait(q_full + st, (s / L::kQStages) & 1)) break;
-                if (s >= kScores && !wait(s_free + buf, (s / kScores - 1) & 1)) break;
-                tc_fence_after();
-                mma_scores<T, D>(tmem + buf * 128, smem_u32(smem) + kb * kTileBytes<D>, smem_u32(smem) + L::kQ + st * kTileBytes<D>);
-                mma_commit(s_full + buf);
+                for (uint32_t x = 0; x <= (two ? 1u : 0u); ++x) {
+                    const uint32_t n = x == 0 ? s : s1++, buf = 2 * x + (n & 1);
+                    if (n >= 2 && !wait(s_free + buf, (n / 2 - 1) & 1)) break;
+                    tc_fence_after();
+                    mma_scores<T, D>(tmem + buf * 128, smem_u32(smem) + x * kTileBytes<D>, q_addr);
+                    mma_commit(s_full + buf);
+                }
                 mma_commit(q_free + st);
             }
-            mma_commit(k_free + kb);
+            mma_commit(k_free);
             more = next_item(v, &w);
         }
         if (flags[0]) {  // MMAs in flight finish before tensor memory is given back
@@ -281,72 +294,75 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             more = next_item(v, &w);
         }
     } else if (warp < 8) {
-        const uint32_t odd = warp >> 2, key = threadIdx.x & 127;
+        const uint32_t x = warp >> 2, key = threadIdx.x & 127;
         const uint32_t lanes = tmem + ((warp & 3) << 21);
         const float scale2 = p.scale * kLog2e;
         const float2 * ring = reinterpret_cast<const float2 *>(smem + L::kRows);
-        float * sums = reinterpret_cast<float *>(smem + L::kSums);
-        float * odd_sums = sums + 2 * kCluster * 128;
-        uint32_t item = 0;
-        for (bool more = work; more; ++item) {
+        float * sums = reinterpret_cast<float *>(smem + L::kSums) + x * 2 * kCluster * 128;
+        sum_full += 2 * x;
+        sum_free += 2 * x;
+        uint32_t item = 0, n = 0;  // items and steps of this key tile
+        for (bool more = work; more;) {
             const int64_t first = int64_t(w.s.kv) - w.s.count;
-            const uint32_t key0 = w.tile * kTileKeys, at = key0 + key;
+            const uint32_t key0 = w.tile * kItemKeys + x * kTileKeys, at = key0 + key;
+            const bool mine = x == 0 || two_key_tiles(v, w);
             float total = 0.0f;
             for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+                const uint32_t st = s % kLseRing;
                 // after a wait that gave up the steps are skipped; the warps still meet at the barriers below
-                if ((s & 1) != odd || !ok) continue;
-                const uint32_t buf = s % kScores, st = s % kLseRing;
-                const uint32_t token0 = (w.k.first + i) * tokens;
-                const int64_t pos0 = first + token0, pos1 = pos0 + tokens - 1;
-                const bool edge = token0 + tokens > w.s.count || pos0 < int64_t(key0) + kTileKeys - 1 ||
-                                  (v.window > 0 && int64_t(key0) <= pos1 - int64_t(v.window));
-                if (!wait(r_full + st, (s / kLseRing) & 1) || !wait(s_full + buf, (s / kScores) & 1)) continue;
-                tc_fence_after();
-                const float4 * rows = reinterpret_cast<const float4 *>(ring + st * 128);
-                float a0 = 0.0f, a1 = 0.0f;
+                if (!wait(r_full + st, (s / kLseRing) & 1)) continue;
+                if (mine) {
+                    const uint32_t buf = 2 * x + (n & 1);
+                    const uint32_t token0 = (w.k.first + i) * tokens;
+                    const int64_t pos0 = first + token0, pos1 = pos0 + tokens - 1;
+                    const bool edge = token0 + tokens > w.s.count || pos0 < int64_t(key0) + kTileKeys - 1 ||
+                                      (v.window > 0 && int64_t(key0) <= pos1 - int64_t(v.window));
+                    if (!wait(s_full + buf, (n / 2) & 1)) continue;
+                    ++n;
+                    tc_fence_after();
+                    const float4 * rows = reinterpret_cast<const float4 *>(ring + st * 128);
+                    float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    tmem_ld32(lanes + buf * 128 + c * 32, x);
-                    tmem_wait_ld();
-                    if (c == 3) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(s_free + buf);
-                    }
-                    if (edge) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float4 r = rows[c * 16 + j / 2];
-                            float e0, e1;
-                            fma2(e0, e1, x[j], x[j + 1], scale2, r.x, r.z);
-                            e0 = exp2_approx(e0);
-                            e1 = exp2_approx(e1);
-                            const int32_t p0 = __float_as_int(r.y), p1 = __float_as_int(r.w), k = int32_t(at);
-                            e0 = k <= p0 && (v.window == 0 || k > p0 - int32_t(v.window)) ? e0 : 0.0f;
-                            e1 = k <= p1 && (v.window == 0 || k > p1 - int32_t(v.window)) ? e1 : 0.0f;
-                            add2(a0, a1, e0, e1);
+                    for (int c = 0; c < 4; ++c) {
+                        float y[32];
+                        tmem_ld32(lanes + buf * 128 + c * 32, y);
+                        tmem_wait_ld();
+                        if (c == 3) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(s_free + buf);
                         }
-                    } else {
+                        if (edge) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float4 r = rows[c * 16 + j / 2];
-                            float e0, e1;
-                            fma2(e0, e1, x[j], x[j + 1], scale2, r.x, r.z);
-                            add2(a0, a1, exp2_approx(e0), exp2_approx(e1));
+                            for (int j = 0; j < 32; j += 2) {
+                                const float4 r = rows[c * 16 + j / 2];
+                                float e0, e1;
+                                fma2(e0, e1, y[j], y[j + 1], scale2, r.x, r.z);
+                                e0 = exp2_approx(e0);
+                                e1 = exp2_approx(e1);
+                                const int32_t p0 = __float_as_int(r.y), p1 = __float_as_int(r.w), k = int32_t(at);
+                                e0 = k <= p0 && (v.window == 0 || k > p0 - int32_t(v.window)) ? e0 : 0.0f;
+                                e1 = k <= p1 && (v.window == 0 || k > p1 - int32_t(v.window)) ? e1 : 0.0f;
+                                add2(a0, a1, e0, e1);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) {
+                                const float4 r = rows[c * 16 + j / 2];
+                                float e0, e1;
+                                fma2(e0, e1, y[j], y[j + 1], scale2, r.x, r.z);
+                                add2(a0, a1, exp2_approx(e0), exp2_approx(e1));
+                            }
                         }
                     }
+                    total += a0 + a1;
                 }
-                total += a0 + a1;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(r_free + st);
             }
-            // odd steps' sums to the even ones' threads, theirs to the leader's
-            const uint32_t q = item & 1, turn = item >> 1;
-            if (odd) odd_sums[key] = total;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (!odd) {
-                total += odd_sums[key];
+            if (mine) {  // the cluster's sums to the leader, which writes them
+                const uint32_t q = item & 1, turn = item >> 1;
+                ++item;
                 if (turn > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(sum_free + q, (turn - 1) & 1, flags, v.error));
                 if (ok) {
                     remote_store(sums + (q * kCluster + rank) * 128 + key, 0, total);
@@ -354,8 +370,8 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                     __syncwarp();
                     if (lane == 0) remote_arrive(sum_full + q, 0);
                 }
-                if (rank == 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait_cluster(sum_full + q, turn & 1, flags, v.error));
                 if (rank == 0) {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(sum_full + q, turn & 1, flags, v.error));
                     if (ok && at < KeyItems::limit(v, w.s)) {
                         float sum = 0.0f;
 #pragma unroll
@@ -364,11 +380,11 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                         const float before = p.mass_in != nullptr && int64_t(at) < first ? p.mass_in[to] : 0.0f;
                         p.mass_out[to] = before + sum;
                     }
-                    asm volatile("bar.sync 2, 128;" ::: "memory");
-                    if (warp == 0 && lane < kCluster) remote_arrive(sum_free + q, lane);
+                    if (x == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+                    else asm volatile("bar.sync 2, 128;" ::: "memory");
+                    if ((warp & 3) == 0 && lane < kCluster) remote_arrive(sum_free + q, lane);
                 }
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // odd_sums may be written again
             more = next_item(v, &w);
         }
     }
