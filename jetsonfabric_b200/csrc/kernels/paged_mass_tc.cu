@@ -12,11 +12,13 @@
 // items still fill the SMs, and no workspace or order of arrival is involved.
 // Clusters take whole items off the evenly divided line of units
 // (walk_locate), each the items whose middle lies in its part.
-//   warps 0-3, 4-7  sums of key tile 0 and 1, a thread per key;
-//   warp 8          the MMAs, up to two steps ahead (S takes all of the 512
-//                   columns of tensor memory);
-//   warp 9          K tiles and queries through TMA;
-//   warp 10         each row's -lse and slot.
+//   warps 0-7, 8-15  sums of key tile 0 and 1, two threads per key, each half
+//                    of a step's rows (one thread per key, 8 warps, left the
+//                    exponentials' unit idle a quarter of the time: 197 us);
+//   warp 16          the MMAs, up to two steps ahead (S takes all of the 512
+//                    columns of tensor memory);
+//   warp 17          K tiles and queries through TMA;
+//   warp 18          each row's -lse and slot.
 #include "paged_attention.cuh"
 #include "paged_mass.cuh"
 #include "paged_tc.cuh"
@@ -26,8 +28,8 @@ namespace paged {
 namespace {
 
 constexpr int kItemMass = 8;  // units of an item's start and end
-constexpr int kThreadsMass = 384;
-constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpLse = 10;
+constexpr int kThreadsMass = 608;
+constexpr int kWarpMma = 16, kWarpLoad = 17, kWarpLse = 18;
 constexpr uint32_t kCluster = 4;
 constexpr uint32_t kItemKeys = 2 * kTileKeys;
 constexpr uint32_t kLseRing = 8;  // steps of row data ahead
@@ -68,7 +70,8 @@ struct MassTcSmem {
     static constexpr uint32_t kQ = 2 * kTileBytes<D>;  // the two K tiles first
     static constexpr uint32_t kRows = kQ + kQStages * kTileBytes<D>;  // [ring][128] (-lse log2 e, slot)
     static constexpr uint32_t kSums = kRows + kLseRing * 128 * 8;     // [key tile][2][cluster][128]
-    static constexpr uint32_t kBars = kSums + 2 * 2 * kCluster * 128 * 4;
+    static constexpr uint32_t kHalves = kSums + 2 * 2 * kCluster * 128 * 4;  // [key tile][2][128] of the second threads
+    static constexpr uint32_t kBars = kHalves + 2 * 2 * 128 * 4;
     static constexpr uint32_t kNumBars = 2 + 2 * kQStages + 8 + 2 * kLseRing + 8;
     static constexpr uint32_t kWalk = kBars + kNumBars * 8;
     static constexpr uint32_t kFlags = kWalk + kThreadsMass / 32 * sizeof(KeyTileWalk);  // abort, tmem
@@ -166,13 +169,13 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
         }
         for (uint32_t i = 0; i < 4; ++i) {
             mbar_init(s_full + i, 1);
-            mbar_init(s_free + i, 4);
+            mbar_init(s_free + i, 8);
             mbar_init(sum_full + i, 4 * kCluster);
             mbar_init(sum_free + i, 1);
         }
         for (uint32_t i = 0; i < kLseRing; ++i) {
             mbar_init(r_full + i, 1);
-            mbar_init(r_free + i, 8);
+            mbar_init(r_free + i, 16);
         }
         flags[0] = 0;
         mbar_init_fence();
@@ -293,12 +296,13 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             }
             more = next_item(v, &w);
         }
-    } else if (warp < 8) {
-        const uint32_t x = warp >> 2, key = threadIdx.x & 127;
+    } else if (warp < 16) {
+        const uint32_t x = warp >> 3, half = (warp >> 2) & 1, key = threadIdx.x & 127;
         const uint32_t lanes = tmem + ((warp & 3) << 21);
         const float scale2 = p.scale * kLog2e;
         const float2 * ring = reinterpret_cast<const float2 *>(smem + L::kRows);
         float * sums = reinterpret_cast<float *>(smem + L::kSums) + x * 2 * kCluster * 128;
+        float * halves = reinterpret_cast<float *>(smem + L::kHalves) + x * 256 + key;
         sum_full += 2 * x;
         sum_free += 2 * x;
         uint32_t item = 0, n = 0;  // items and steps of this key tile
@@ -320,14 +324,14 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                     if (!wait(s_full + buf, (n / 2) & 1)) continue;
                     ++n;
                     tc_fence_after();
-                    const float4 * rows = reinterpret_cast<const float4 *>(ring + st * 128);
+                    const float4 * rows = reinterpret_cast<const float4 *>(ring + st * 128 + half * 64);
                     float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         float y[32];
-                        tmem_ld32(lanes + buf * 128 + c * 32, y);
+                        tmem_ld32(lanes + buf * 128 + half * 64 + c * 32, y);
                         tmem_wait_ld();
-                        if (c == 3) {
+                        if (c == 1) {
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(s_free + buf);
@@ -363,6 +367,14 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             if (mine) {  // the cluster's sums to the leader, which writes them
                 const uint32_t q = item & 1, turn = item >> 1;
                 ++item;
+                if (half) halves[q * 128] = total;
+                if (x == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
+                else asm volatile("bar.sync 2, 256;" ::: "memory");
+                if (half) {
+                    more = next_item(v, &w);
+                    continue;
+                }
+                total += halves[q * 128];
                 if (turn > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(sum_free + q, (turn - 1) & 1, flags, v.error));
                 if (ok) {
                     remote_store(sums + (q * kCluster + rank) * 128 + key, 0, total);
@@ -380,8 +392,8 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                         const float before = p.mass_in != nullptr && int64_t(at) < first ? p.mass_in[to] : 0.0f;
                         p.mass_out[to] = before + sum;
                     }
-                    if (x == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-                    else asm volatile("bar.sync 2, 128;" ::: "memory");
+                    if (x == 0) asm volatile("bar.sync 3, 128;" ::: "memory");
+                    else asm volatile("bar.sync 4, 128;" ::: "memory");
                     if ((warp & 3) == 0 && lane < kCluster) remote_arrive(sum_free + q, lane);
                 }
             }
