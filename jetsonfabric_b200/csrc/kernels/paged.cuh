@@ -264,14 +264,21 @@ struct WalkOf {
 };
 using Walk = WalkOf<RowItems>;
 
-// The CTA that holds `unit`.
+// a * b / c, in 32 bits where that holds it (a 64-bit division takes hundreds of cycles).
+__device__ __forceinline__ uint64_t mul_div(uint64_t a, uint64_t b, uint64_t c) {
+    const uint64_t n = a * b;
+    return (n | c) >> 32 ? n / c : uint32_t(n) / uint32_t(c);
+}
+
+// The CTA that holds `unit`: the last c with c * total / ctas <= unit.
 __device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t total, uint64_t ctas) {
-    return uint32_t(((unit + 1) * ctas - 1) / total);
+    const uint64_t n = (unit + 1) * ctas - 1;
+    return (n | total) >> 32 ? uint32_t(n / total) : uint32_t(n) / uint32_t(total);
 }
 
 // Key tiles [t0, t1) of the current item that this CTA does.
-template <int E>
-__device__ __forceinline__ void walk_segment(const Walk & w, uint32_t & t0, uint32_t & t1) {
+template <int E, class Items>
+__device__ __forceinline__ void walk_segment(const WalkOf<Items> & w, uint32_t & t0, uint32_t & t1) {
     const uint64_t a = w.unit - w.item0, b = w.end - w.item0;
     t0 = a > E ? uint32_t(a - E) : 0u;
     t1 = b <= E ? 0u : b - E < w.k.tiles ? uint32_t(b - E) : w.k.tiles;
@@ -294,8 +301,8 @@ __device__ __forceinline__ void walk_item(const View & v, WalkOf<Items> & w) {
 }
 
 // Moves to the CTA's next segment with tiles; false at the end of its line.
-template <int E>
-__device__ __forceinline__ bool walk_next(const View & v, Walk & w) {
+template <int E, class Items>
+__device__ __forceinline__ bool walk_next(const View & v, WalkOf<Items> & w) {
     // what is left of the line, if not tiles of another item, is the start of one
     if (w.item0 + w.k.tiles + 2 * E >= w.end) return false;
     walk_item<E>(v, w);
@@ -304,8 +311,8 @@ __device__ __forceinline__ bool walk_next(const View & v, Walk & w) {
 
 // walk_next of a warp's own copy in shared memory (registers are scarce in the
 // kernels): lane 0 moves it.
-template <int E>
-__device__ __forceinline__ bool walk_warp_next(const View & v, Walk * w) {
+template <int E, class Items>
+__device__ __forceinline__ bool walk_warp_next(const View & v, WalkOf<Items> * w) {
     __syncwarp();
     int more = 0;
     if ((threadIdx.x & 31) == 0) more = walk_next<E>(v, *w);
@@ -313,31 +320,29 @@ __device__ __forceinline__ bool walk_warp_next(const View & v, Walk * w) {
 }
 
 // The CTAs that hold the first and the last tile of the current item.
-template <int E>
-__device__ __forceinline__ void walk_owners(const Walk & w, uint32_t & c0, uint32_t & c1) {
+template <int E, class Items>
+__device__ __forceinline__ void walk_owners(const WalkOf<Items> & w, uint32_t & c0, uint32_t & c1) {
     c0 = cta_of(w.item0 + E, w.total, w.ctas);
     c1 = cta_of(w.item0 + E + w.k.tiles - 1, w.total, w.ctas);
 }
 
-// Positions `x` (every lane of warp 0 gets it) at the unit where the line of
-// worker `index` of `workers` begins; unit == end when it has no work. All
-// threads call it; `cost` is shared scratch of one u64 per sequence.
+// Positions `walks`, one WalkOf per warp of the CTA in shared memory, at the
+// unit where the line of worker `index` of `workers` begins; unit == end when
+// it has no work. All threads call it; `cost` is shared scratch of one u64 per
+// sequence. Up to 128 sequences every warp works it out by itself from
+// registers, one load's latency long: it precedes the first copy of a call
+// that may be all latency. More go through `cost` and two CTA barriers.
 template <int E, class Items>
-__device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uint32_t index, uint32_t workers, WalkOf<Items> & x) {
+__device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uint32_t index, uint32_t workers, WalkOf<Items> * walks) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    // units of each sequence: a thread per sequence; the lanes of the warp
-    // share the items of a sequence that has many
-    for (uint32_t base = warp * 32; base < v.sequences; base += warps * 32) {
-        const uint32_t b = base + lane;
-        Sequence s = {0, 0, 0};
-        uint32_t items = 0;
-        uint64_t units = 0;
-        if (b < v.sequences) {
-            s = load_sequence(v, b);
-            items = Items::count(v, s);
-            if (items <= 4) {
-                for (uint32_t i = 0; i < items; ++i) units += Items::part(v, s, i).tiles + E;
-            }
+    constexpr uint32_t kOwn = 4;  // sequences per lane
+    const bool few = v.sequences <= 32 * kOwn;
+    // units of a sequence per lane; the lanes share the items of one that has many
+    const auto units_of = [&](const Sequence & s) {
+        const uint32_t items = Items::count(v, s);
+        unsigned long long units = 0;
+        if (items <= 4) {
+            for (uint32_t i = 0; i < items; ++i) units += Items::part(v, s, i).tiles + E;
         }
         uint32_t many = __ballot_sync(0xffffffffu, items > 4);
         while (many != 0) {
@@ -354,27 +359,43 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (int(lane) == src) units = sum;
         }
-        if (b < v.sequences) cost[b] = units;
-    }
-    __syncthreads();
-    if (warp != 0) return;
+        return units;
+    };
+    Sequence own[kOwn];
+    unsigned long long own_units[kOwn];
     unsigned long long per_head = 0;
-    for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
+    if (few) {
+#pragma unroll
+        for (uint32_t r = 0; r < kOwn; ++r) {
+            own[r] = Sequence{0, 0, 0};
+            if (r * 32 + lane < v.sequences) own[r] = load_sequence(v, r * 32 + lane);
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < kOwn; ++r) {
+            own_units[r] = r * 32 < v.sequences ? units_of(own[r]) : 0ull;
+            per_head += own_units[r];
+        }
+    } else {
+        for (uint32_t base = warp * 32; base < v.sequences; base += warps * 32) {
+            const uint32_t b = base + lane;
+            const unsigned long long units = units_of(b < v.sequences ? load_sequence(v, b) : Sequence{0, 0, 0});
+            if (b < v.sequences) cost[b] = units;
+        }
+        __syncthreads();
+        for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
+    WalkOf<Items> x = {};
     x.total = uint64_t(per_head) * v.kv_heads;
     x.ctas = uint64_t(workers) < x.total ? workers : uint32_t(x.total);
-    x.unit = x.end = 0;
-    if (index >= x.ctas) return;
-    x.unit = uint64_t(index) * x.total / x.ctas;
-    x.end = uint64_t(index + 1) * x.total / x.ctas;
-    x.kv_head = uint32_t(x.unit / per_head);
-    // the first entry of a list whose running sum exceeds what is left: 32 at a time
-    unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;
-    const auto find = [&](uint32_t n, auto value) {
-        uint32_t at = 0;
-        for (uint32_t base = 0; base < n; base += 32) {
-            const unsigned long long mine = base + lane < n ? value(base + lane) : 0ull;
+    if (index < x.ctas) {
+        x.unit = mul_div(index, x.total, x.ctas);
+        x.end = mul_div(index + 1, x.total, x.ctas);
+        x.kv_head = uint32_t(mul_div(x.unit, 1, per_head));
+        // the first entry of a list whose running sum exceeds what is left: 32 at a time
+        unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;
+        const auto find32 = [&](unsigned long long mine, int & src) {
             unsigned long long upto = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -382,42 +403,62 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
                 if (int(lane) >= d) upto += o;
             }
             const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
-            if (over != 0) {
-                const int src = __ffs(over) - 1;
-                at = base + src;
-                left -= __shfl_sync(0xffffffffu, upto - mine, src);
-                break;
+            src = __ffs(over) - 1;
+            left -= __shfl_sync(0xffffffffu, over != 0 ? upto - mine : upto, over != 0 ? src : 31);
+            return over != 0;
+        };
+        int src = 0;
+        if (few) {
+            bool found = false;
+#pragma unroll
+            for (uint32_t r = 0; r < kOwn; ++r) {
+                if (!found && r * 32 < v.sequences && find32(own_units[r], src)) {
+                    found = true;
+                    x.b = r * 32 + src;
+                    x.s.q0 = __shfl_sync(0xffffffffu, own[r].q0, src);
+                    x.s.count = __shfl_sync(0xffffffffu, own[r].count, src);
+                    x.s.kv = __shfl_sync(0xffffffffu, own[r].kv, src);
+                }
             }
-            left -= __shfl_sync(0xffffffffu, upto, 31);
+        } else {
+            for (uint32_t base = 0; base < v.sequences; base += 32) {
+                if (find32(base + lane < v.sequences ? cost[base + lane] : 0ull, src)) {
+                    x.b = base + src;
+                    break;
+                }
+            }
+            x.s = load_sequence(v, x.b);
         }
-        return at;
-    };
-    x.b = find(v.sequences, [&](uint32_t b) { return (unsigned long long)(cost[b]); });
-    x.s = load_sequence(v, x.b);
-    x.tile = find(Items::count(v, x.s), [&](uint32_t i) { return (unsigned long long)(Items::part(v, x.s, i).tiles + E); });
-    x.item0 = x.unit - left;
-    x.k = Items::part(v, x.s, x.tile);
+        const uint32_t items = Items::count(v, x.s);
+        if (items > 1) {
+            for (uint32_t base = 0; base < items; base += 32) {
+                if (find32(base + lane < items ? Items::part(v, x.s, base + lane).tiles + E : 0ull, src)) {
+                    x.tile = base + src;
+                    break;
+                }
+            }
+        }
+        x.item0 = x.unit - left;
+        x.k = Items::part(v, x.s, x.tile);
+    }
+    if (lane == 0) walks[warp] = x;
+    __syncwarp();
+    if (!few) {  // cost may be written again, by copies too
+        fence_proxy_async();
+        __syncthreads();
+    }
 }
 
-// Positions `copies` (up to 32) Walks in shared memory at the CTA's first
-// segment. `cost` is shared scratch of one u64 per sequence, free after the
-// call. False when the CTA has no work.
-template <int E>
-static __device__ bool walk_begin(const View & v, uint64_t * cost, Walk * walks, uint32_t copies) {
-    Walk x;
-    walk_locate<E>(v, cost, blockIdx.x, gridDim.x, x);
-    if (threadIdx.x < 32) {
-        bool any = x.unit < x.end;
-        if (any) {
-            uint32_t t0, t1;
-            walk_segment<E>(x, t0, t1);
-            any = t0 < t1 || walk_next<E>(v, x);
-        }
-        if (!any) x.unit = x.end = 0;
-        if (threadIdx.x < copies) walks[threadIdx.x] = x;
-    }
-    __syncthreads();
-    return walks[0].unit < walks[0].end;
+// The same for CTAs that share items: at the first segment that has tiles.
+// False when the CTA has no work.
+template <int E, class Items>
+__device__ __forceinline__ bool walk_begin(const View & v, uint64_t * cost, WalkOf<Items> * walks) {
+    walk_locate<E>(v, cost, blockIdx.x, gridDim.x, walks);
+    WalkOf<Items> * w = walks + (threadIdx.x >> 5);
+    if (w->unit >= w->end) return false;
+    uint32_t t0, t1;
+    walk_segment<E>(*w, t0, t1);
+    return t0 < t1 || walk_warp_next<E>(v, w);
 }
 
 // ---- number types -------------------------------------------------------------------

@@ -79,14 +79,13 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         flags[0] = 0;
         mbar_init_fence();
     }
+    __syncthreads();
     pdl_trigger();
     pdl_wait();
     const View & v = p.view;
     Walk * walks = reinterpret_cast<Walk *>(smem + L::kWalk);
-    if (!walk_begin<kItemRows>(v, reinterpret_cast<uint64_t *>(smem), walks, kThreadsRows / 32)) return;
+    if (!walk_begin<kItemRows>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
     Walk & w = walks[warp];
-    fence_proxy_async();  // the ring held the walk's scratch
-    __syncthreads();
 
     if (warp >= kConsumers) {
         const bool is_v = warp > kConsumers;

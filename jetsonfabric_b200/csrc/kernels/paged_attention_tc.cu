@@ -114,9 +114,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
         return;
     }
     Walk * walks = reinterpret_cast<Walk *>(smem + L::kWalk);
-    if (!walk_begin<kItemTc>(v, reinterpret_cast<uint64_t *>(smem), walks, kThreadsTc / 32)) return;
+    if (!walk_begin<kItemTc>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
     Walk & w = walks[warp];
-    // rows that no query fills stay zero (and this held the walk's scratch)
+    __syncthreads();
+    // rows that no query fills stay zero (and this may have held the walk's scratch)
     for (uint32_t i = threadIdx.x; i < L::kQ / 16; i += kThreadsTc) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
     if (warp == kWarpS) tmem_alloc(tmem_slot);

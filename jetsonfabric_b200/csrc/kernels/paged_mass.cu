@@ -21,94 +21,31 @@ namespace {
 constexpr int kConsumers = 8;
 constexpr int kThreadsRows = (kConsumers + 1) * 32;
 
+// A sequence and kv head is one item, its key tiles the units.
+struct SequenceItems {
+    struct Part {
+        uint32_t tiles;
+    };
+    static __device__ __forceinline__ uint32_t limit(const View & v, const Sequence & s) {
+        if (s.kv <= v.slots) return s.kv;
+        flag_error(v.error, JFB_PAGED_ERROR_RANGE);
+        return uint32_t(v.slots);
+    }
+    static __device__ __forceinline__ uint32_t count(const View & v, const Sequence & s) { return s.kv > 0 ? 1 : 0; }
+    static __device__ __forceinline__ Part part(const View & v, const Sequence & s, uint32_t) {
+        return Part{(limit(v, s) + kTileKeys - 1) / kTileKeys};
+    }
+};
+using SequenceWalk = WalkOf<SequenceItems>;
+
 template <int D>
 struct MassSmem {
     static constexpr int kStages = D == 128 ? 6 : 12;
     static constexpr uint32_t kBars = kStages * kTileBytes<D>;  // full, empty
     static constexpr uint32_t kWalk = kBars + 2 * kStages * 8;
-    static constexpr uint32_t kFlags = kWalk + 64;
+    static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(SequenceWalk);
     static constexpr uint32_t kBytes = kFlags + 16 + 1024;
 };
-
-// Key tiles of all sequences in one line, kv head outermost, divided evenly.
-struct KeyWalk {
-    uint64_t unit, end;
-    uint32_t kv_head, b, tile;
-    Sequence s;
-    uint32_t limit;  // keys of the sequence that are written
-};
-
-__device__ __forceinline__ uint32_t key_limit(const View & v, const Sequence & s, uint64_t mass_stride) {
-    if (s.kv > mass_stride) {
-        flag_error(v.error, JFB_PAGED_ERROR_RANGE);
-        return uint32_t(mass_stride);
-    }
-    return s.kv;
-}
-
-__device__ bool key_walk_begin(const View & v, uint64_t mass_stride, uint32_t * cost, KeyWalk * out, KeyWalk & w) {
-    for (uint32_t b = threadIdx.x; b < v.sequences; b += blockDim.x) {
-        cost[b] = (key_limit(v, load_sequence(v, b), mass_stride) + kTileKeys - 1) / kTileKeys;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const uint32_t lane = threadIdx.x;
-        unsigned long long per_head = 0;
-        for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
-        const unsigned long long total = per_head * v.kv_heads;
-        KeyWalk x;
-        x.unit = total * blockIdx.x / gridDim.x;
-        x.end = total * (blockIdx.x + 1) / gridDim.x;
-        x.kv_head = x.b = x.tile = x.limit = 0;
-        x.s = Sequence{0, 0, 0};
-        if (x.unit < x.end) {
-            x.kv_head = uint32_t(x.unit / per_head);
-            unsigned long long left = x.unit - per_head * x.kv_head;
-            for (uint32_t base = 0; base < v.sequences; base += 32) {
-                const unsigned long long mine = base + lane < v.sequences ? cost[base + lane] : 0u;
-                unsigned long long upto = mine;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (int(lane) >= d) upto += o;
-                }
-                const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
-                if (over != 0) {
-                    const int src = __ffs(over) - 1;
-                    x.b = base + src;
-                    left -= __shfl_sync(0xffffffffu, upto - mine, src);
-                    break;
-                }
-                left -= __shfl_sync(0xffffffffu, upto, 31);
-            }
-            x.tile = uint32_t(left);
-            x.s = load_sequence(v, x.b);
-            x.limit = key_limit(v, x.s, mass_stride);
-        }
-        if (lane == 0) *out = x;
-    }
-    __syncthreads();
-    w = *out;
-    __syncthreads();
-    return w.unit < w.end;
-}
-
-__device__ __forceinline__ bool key_walk_next(const View & v, uint64_t mass_stride, KeyWalk & w) {
-    if (++w.unit >= w.end) return false;
-    ++w.tile;
-    while (uint64_t(w.tile) * kTileKeys >= w.limit) {
-        w.tile = 0;
-        if (++w.b >= v.sequences) {
-            w.b = 0;
-            ++w.kv_head;
-        }
-        w.s = load_sequence(v, w.b);
-        w.limit = key_limit(v, w.s, mass_stride);
-    }
-    return true;
-}
 
 // Packed rows [r0, r1) that see some of keys [key0, key1).
 __device__ __forceinline__ void seeing_rows(const Sequence & s, uint32_t group, uint32_t window, uint32_t key0, uint32_t key1,
@@ -126,7 +63,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     mass_rows_kernel(const __grid_constant__ CUtensorMap map_k, const MassParams p) {
     extern __shared__ uint8_t smem_raw[];
     using L = MassSmem<D>;
-    static_assert(L::kBars >= JFB_PAGED_MAX_SEQUENCES * 4 && sizeof(KeyWalk) <= 64);
+    static_assert(L::kBars >= JFB_PAGED_MAX_SEQUENCES * 8);
     uint8_t * smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t * full = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t * empty = full + L::kStages;
@@ -140,32 +77,35 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         flags[0] = 0;
         mbar_init_fence();
     }
+    __syncthreads();
     pdl_trigger();
     pdl_wait();
     const View & v = p.view;
-    KeyWalk w;
-    if (!key_walk_begin(v, v.slots, reinterpret_cast<uint32_t *>(smem), reinterpret_cast<KeyWalk *>(smem + L::kWalk), w)) return;
-    fence_proxy_async();  // the ring held the walk's scratch
-    __syncthreads();
+    SequenceWalk * walks = reinterpret_cast<SequenceWalk *>(smem + L::kWalk);
+    if (!walk_begin<0>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
+    SequenceWalk & w = walks[warp];
 
     if (warp == kConsumers) {
         uint32_t n = 0;
         bool ok = true;
-        auto pages_of = [&](const KeyWalk & a) {
-            const uint32_t key0 = a.tile * kTileKeys;
-            return tile_pages(v, v.table + uint64_t(a.b) * v.table_stride, key0, min(a.limit, key0 + uint32_t(kTileKeys)));
-        };
-        TileLoad next = pages_of(w);
-        for (bool more = true; more; ++n) {
-            const TileLoad load = next;
-            const uint32_t head = w.kv_head;
-            more = key_walk_next(v, v.slots, w);
-            if (more) next = pages_of(w);
-            const uint32_t st = n % L::kStages, turn = n / L::kStages;
-            if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
-            if (!ok) break;
-            tile_issue<D>(load, &map_k, head, smem_u32(smem) + st * kTileBytes<D>, full + st);
-        }
+        do {
+            uint32_t t0, t1;
+            walk_segment<0>(w, t0, t1);
+            const int32_t * row = v.table + uint64_t(w.b) * v.table_stride;
+            const uint32_t limit = SequenceItems::limit(v, w.s), head = w.kv_head;
+            auto pages_of = [&](uint32_t t) {
+                return tile_pages(v, row, t * kTileKeys, min(limit, (t + 1) * uint32_t(kTileKeys)));
+            };
+            TileLoad next = pages_of(t0);
+            for (uint32_t t = t0; t < t1; ++t, ++n) {
+                const TileLoad load = next;
+                if (t + 1 < t1) next = pages_of(t + 1);
+                const uint32_t st = n % L::kStages, turn = n / L::kStages;
+                if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
+                if (!ok) break;
+                tile_issue<D>(load, &map_k, head, smem_u32(smem) + st * kTileBytes<D>, full + st);
+            }
+        } while (ok && walk_warp_next<0>(v, &w));
         if (flags[0]) {
             for (uint32_t i = n > uint32_t(L::kStages) ? n - L::kStages : 0u; i < n; ++i) {
                 mbar_drain(full + i % L::kStages, (i / L::kStages) & 1);
@@ -179,55 +119,72 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     const float scale2 = p.scale * kLog2e;
     uint32_t n = 0;
     do {
-        const uint32_t st = n % L::kStages, parity = (n / L::kStages) & 1;
-        ++n;
-        if (!__all_sync(0xffffffffu, mbar_wait(full + st, parity, flags, v.error))) return;  // no barrier joins these warps
-        // this warp's 16 keys as B fragments, then the stage is free
-        uint32_t kb[D / 16][4];
-        const uint32_t kbase = smem_u32(smem) + st * kTileBytes<D>;
-        const uint32_t krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
+        uint32_t t0, t1;
+        walk_segment<0>(w, t0, t1);
+        const int64_t first = int64_t(w.s.kv) - w.s.count;
+        const uint32_t limit = SequenceItems::limit(v, w.s);
+        const uint64_t line = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots;
+        // 16 packed rows as A fragments, their -lse and slots
+        uint32_t qa[D / 16][4];
+        float nlse[2];
+        int32_t pos[2];
+        const auto load_rows = [&](uint32_t base, uint32_t end) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t chunk = kk * 2 + ((lane >> 3) & 1);
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(kb[kk][0]), "=r"(kb[kk][1]), "=r"(kb[kk][2]), "=r"(kb[kk][3])
-                         : "r"(kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4))
-                         : "memory");
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty + st);
-        const uint32_t key = w.tile * kTileKeys + warp * 16;
-        if (key < w.limit) {
-            const int64_t first = int64_t(w.s.kv) - w.s.count;
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t r = base + grp + 8 * e;
+                const bool valid = r < end;
+                const uint32_t i = valid ? r / G : 0u, h = w.kv_head * G + (valid ? r % G : 0u);
+                const T * src = static_cast<const T *>(p.q) + uint64_t(w.s.q0 + i) * p.q_stride + uint64_t(h) * hd;
+                nlse[e] = valid ? -kLog2e * p.lse[uint64_t(w.s.q0 + i) * p.heads + h] : 0.0f;
+                pos[e] = valid ? int32_t(first + i) : -1;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t d = kk * 16 + x * 8;
+                        qa[kk][e + 2 * x] = valid && d < hd ? *reinterpret_cast<const uint32_t *>(src + d + tig * 2) : 0u;
+                    }
+                }
+            }
+        };
+        const uint32_t packed = w.s.count * G;
+        const bool once = packed <= 16;  // all rows fit: fetched once for the segment's tiles
+        if (once) load_rows(0, packed);
+        for (uint32_t t = t0; t < t1; ++t, ++n) {
+            const uint32_t st = n % L::kStages, parity = (n / L::kStages) & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(full + st, parity, flags, v.error))) return;  // no barrier joins these warps
+            // this warp's 16 keys as B fragments, then the stage is free
+            uint32_t kb[D / 16][4];
+            const uint32_t kbase = smem_u32(smem) + st * kTileBytes<D>;
+            const uint32_t krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t chunk = kk * 2 + ((lane >> 3) & 1);
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(kb[kk][0]), "=r"(kb[kk][1]), "=r"(kb[kk][2]), "=r"(kb[kk][3])
+                             : "r"(kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4))
+                             : "memory");
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + st);
+            const uint32_t key = t * kTileKeys + warp * 16;
+            if (key >= limit) continue;
+            float before[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of this lane's four keys, fetched while the products run
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t k = key + (x >> 1) * 8 + tig * 2 + (x & 1);
+                if (grp == 0 && p.mass_in != nullptr && k < limit && int64_t(k) < first) before[x] = p.mass_in[line + k];
+            }
             uint32_t r0, r1;
-            seeing_rows(w.s, G, v.window, key, min(w.limit, key + 16), r0, r1);
+            seeing_rows(w.s, G, v.window, key, min(limit, key + 16), r0, r1);
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t base = r0; base < r1; base += 16) {
+            for (uint32_t base = once ? 0u : r0; base < r1; base += 16) {
+                if (!once) load_rows(base, r1);
                 float s[2][4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
-                }
-                uint32_t qa[D / 16][4];
-                float lse2[2];
-                int32_t pos[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t r = base + grp + 8 * e;
-                    const bool valid = r < r1;
-                    const uint32_t i = valid ? r / G : 0u, h = w.kv_head * G + (valid ? r % G : 0u);
-                    const T * src = static_cast<const T *>(p.q) + uint64_t(w.s.q0 + i) * p.q_stride + uint64_t(h) * hd;
-                    lse2[e] = valid ? p.lse[uint64_t(w.s.q0 + i) * p.heads + h] * kLog2e : 0.0f;
-                    pos[e] = valid ? int32_t(first + i) : -1;
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t d = kk * 16 + x * 8;
-                            qa[kk][e + 2 * x] = valid && d < hd ? *reinterpret_cast<const uint32_t *>(src + d + tig * 2) : 0u;
-                        }
-                    }
                 }
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
@@ -240,7 +197,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                     for (int e = 0; e < 4; ++e) {
                         const int32_t k = int32_t(key) + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
                         const bool seen = k <= q && (v.window == 0 || k > q - int32_t(v.window));
-                        if (seen) acc[j * 2 + (e & 1)] += exp2_approx(fmaf(s[j][e], scale2, -lse2[e >> 1]));
+                        if (seen) acc[j * 2 + (e & 1)] += exp2_approx(fmaf(s[j][e], scale2, nlse[e >> 1]));
                     }
                 }
             }
@@ -250,18 +207,14 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor_sync(0xffffffffu, acc[x], d);
             }
             if (grp == 0) {
-                const uint64_t line = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const uint32_t k = key + (x >> 1) * 8 + tig * 2 + (x & 1);
-                    if (k < w.limit) {
-                        const float before = p.mass_in != nullptr && int64_t(k) < first ? p.mass_in[line + k] : 0.0f;
-                        p.mass_out[line + k] = before + acc[x];
-                    }
+                    if (k < limit) p.mass_out[line + k] = before[x] + acc[x];
                 }
             }
         }
-    } while (key_walk_next(v, v.slots, w));
+    } while (walk_warp_next<0>(v, &w));
 }
 
 template <typename T, int D>

@@ -27,7 +27,7 @@ namespace jfb {
 namespace paged {
 namespace {
 
-constexpr int kItemMass = 8;  // units of an item's start and end
+constexpr int kItemMass = 16; // units of an item's start and end
 constexpr int kThreadsMass = 608;
 constexpr int kWarpMma = 16, kWarpLoad = 17, kWarpLse = 18;
 constexpr uint32_t kCluster = 4;
@@ -184,20 +184,19 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
     pdl_wait();
     const View & v = p.view;
     KeyTileWalk * walks = reinterpret_cast<KeyTileWalk *>(smem + L::kWalk);
-    KeyTileWalk start;
-    walk_locate<kItemMass>(v, reinterpret_cast<uint64_t *>(smem), blockIdx.x / kCluster, gridDim.x / kCluster, start);
-    if (warp == 0) {
+    walk_locate<kItemMass>(v, reinterpret_cast<uint64_t *>(smem), blockIdx.x / kCluster, gridDim.x / kCluster, walks);
+    if (lane == 0) {
+        KeyTileWalk & start = walks[warp];
         if (start.unit < start.end) {
             const uint64_t middle = start.item0 + (start.k.tiles + kItemMass) / 2;
             // an item whose middle lies before or behind this part is another cluster's
             if (middle >= start.end || (middle < start.unit && !step_item(v, start))) start.unit = start.end;
         }
-        if (lane < kThreadsMass / 32) walks[lane] = start;
     }
     __syncthreads();
     KeyTileWalk & w = walks[warp];
-    const bool work = walks[0].unit < walks[0].end && (smem_u32(smem) & 1023u) == 0;
-    // rows that no query fills stay zero (and this held the walk's scratch)
+    const bool work = w.unit < w.end && (smem_u32(smem) & 1023u) == 0;
+    // rows that no query fills stay zero (and this may have held the walk's scratch)
     for (uint32_t i = threadIdx.x; i < L::kRows / 16; i += kThreadsMass) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
     if (warp == kWarpMma) tmem_alloc(tmem_slot);
