@@ -7,6 +7,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cstring>
 #include <mutex>
 
@@ -226,19 +227,18 @@ struct KeyRange {
     uint32_t tiles;    // max(1, tiles of [begin, hi))
 };
 
+// Packed rows of a sequence: the host refuses calls with 2^31 or more.
 __device__ __forceinline__ uint32_t row_tiles(const View & v, const Sequence & s) {
-    return uint32_t((uint64_t(s.count) * v.group + v.item_rows - 1) / v.item_rows);
+    return (s.count * v.group + v.item_rows - 1) / v.item_rows;
 }
 
 __device__ __forceinline__ KeyRange key_range(const View & v, const Sequence & s, uint32_t tile) {
-    const uint64_t packed = uint64_t(s.count) * v.group;
-    const uint64_t r0 = uint64_t(tile) * v.item_rows;
-    const uint64_t r1 = (r0 + v.item_rows < packed ? r0 + v.item_rows : packed) - 1;
-    const int64_t first = int64_t(s.kv) - s.count;
-    const int64_t p0 = first + int64_t(uint32_t(r0) / v.group), p1 = first + int64_t(uint32_t(r1) / v.group);
+    const uint32_t r0 = tile * v.item_rows, r1 = min(r0 + v.item_rows, s.count * v.group) - 1;
+    const int32_t first = int32_t(s.kv) - int32_t(s.count);
+    const int32_t p0 = first + int32_t(r0 / v.group), p1 = first + int32_t(r1 / v.group);
     KeyRange k;
     k.hi = p1 < 0 ? 0u : uint32_t(p1 + 1);
-    k.lo = v.window > 0 && p0 >= int64_t(v.window) ? uint32_t(p0 - v.window + 1) : 0u;
+    k.lo = v.window > 0 && p0 >= int32_t(v.window) ? uint32_t(p0) - v.window + 1 : 0u;
     const uint32_t box = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
     k.begin = k.lo & ~(box - 1);
     k.tiles = k.hi > k.begin ? (k.hi - k.begin + kTileKeys - 1) / kTileKeys : 1u;
@@ -596,18 +596,30 @@ inline bool pool_map(CUtensorMap & map, const void * pool, const jfb_paged_cache
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// SMs of the current device.
-inline uint32_t device_sms() {
-    int device = 0, n = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) return 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
-    return n > 0 ? uint32_t(n) : 0u;
+// The current device and its SMs (0 when there is none).
+struct Device {
+    int index;
+    uint32_t sms;
+};
+inline Device current_device() {
+    Device d = {0, 0};
+    int n = 0;
+    if (cudaGetDevice(&d.index) == cudaSuccess &&
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d.index) == cudaSuccess && n > 0) {
+        d.sms = uint32_t(n);
+    }
+    return d;
 }
 
-// Largest dynamic shared memory of a kernel, set once per device.
-template <typename K>
-inline cudaError_t allow_smem(K kernel, uint32_t bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+// Allows `Kernel` its dynamic shared memory, once per device.
+template <auto Kernel>
+inline cudaError_t allow_smem(const Device & d, uint32_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = d.index >= 0 && d.index < 64 ? 1ull << d.index : 0ull;
+    if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace paged

@@ -351,10 +351,10 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
 }
 
 template <typename T, int D>
-jfb_status launch_rows(const CUtensorMap & k, const CUtensorMap & v, const AttentionParams & p, uint32_t sms, cudaStream_t s) {
-    auto kernel = paged_rows_kernel<T, D>;
-    cudaError_t e = allow_smem(kernel, RowsSmem<D>::kBytes);
-    if (e == cudaSuccess) e = launch_k(kernel, dim3(sms), dim3(kThreadsRows), RowsSmem<D>::kBytes, s, k, v, p);
+jfb_status launch_rows(const CUtensorMap & k, const CUtensorMap & v, const AttentionParams & p, const Device & device,
+                       cudaStream_t s) {
+    cudaError_t e = allow_smem<paged_rows_kernel<T, D>>(device, RowsSmem<D>::kBytes);
+    if (e == cudaSuccess) e = launch_k(paged_rows_kernel<T, D>, dim3(device.sms), dim3(kThreadsRows), RowsSmem<D>::kBytes, s, k, v, p);
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_attention");
 }
@@ -367,7 +367,7 @@ using namespace jfb;
 using namespace jfb::paged;
 
 extern "C" uint64_t jfb_paged_attention_workspace_bytes(void) {
-    return kCounterBytes + uint64_t(device_sms()) * 2 * kSlotFloats * sizeof(float);
+    return kCounterBytes + uint64_t(current_device().sms) * 2 * kSlotFloats * sizeof(float);
 }
 
 extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uint32_t rows, uint32_t heads, float scale,
@@ -382,7 +382,8 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     if (!(scale > 0.0f) || scale > 3.0e38f || window > 0x7fffffffu) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a positive finite scale and a window below 2^31");
     }
-    const uint32_t sms = device_sms();
+    const Device device = current_device();
+    const uint32_t sms = device.sms;
     if (sms == 0 || sms * 2 * sizeof(uint32_t) > kCounterBytes) {
         return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: no usable device");
     }
@@ -411,9 +412,9 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
     const uint32_t group = p.view.group;
-    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_attention_tc(*cache, mk, mv, p, sms, s);
+    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_attention_tc(*cache, mk, mv, p, device, s);
     if (cache->head_dim <= 64) {
-        return half ? launch_rows<__half, 64>(mk, mv, p, sms, s) : launch_rows<__nv_bfloat16, 64>(mk, mv, p, sms, s);
+        return half ? launch_rows<__half, 64>(mk, mv, p, device, s) : launch_rows<__nv_bfloat16, 64>(mk, mv, p, device, s);
     }
-    return half ? launch_rows<__half, 128>(mk, mv, p, sms, s) : launch_rows<__nv_bfloat16, 128>(mk, mv, p, sms, s);
+    return half ? launch_rows<__half, 128>(mk, mv, p, device, s) : launch_rows<__nv_bfloat16, 128>(mk, mv, p, device, s);
 }

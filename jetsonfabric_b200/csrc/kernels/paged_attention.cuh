@@ -82,7 +82,7 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const ui
 
 // The tcgen05 kernel of paged_attention_tc.cu.
 jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap & k, const CUtensorMap & v, AttentionParams p,
-                               uint32_t sms, cudaStream_t s);
+                               const Device & device, cudaStream_t s);
 
 // Query-shaped rows [rows][heads x head_dim] of 16-bit numbers.
 inline jfb_status check_rows(const char * what, const void * x, uint64_t stride, uint32_t rows, uint32_t heads,

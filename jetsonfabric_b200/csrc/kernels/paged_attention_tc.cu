@@ -421,12 +421,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
 }
 
 template <typename T, int D>
-jfb_status launch(const TcMaps & maps, const AttentionParams & p, uint32_t tokens, uint32_t sms, cudaStream_t s) {
+jfb_status launch(const TcMaps & maps, const AttentionParams & p, uint32_t tokens, const Device & device, cudaStream_t s) {
     // rows of whole 32-byte sectors
     const bool sectors = ((reinterpret_cast<uintptr_t>(p.out) | p.out_stride * 2 | p.view.head_dim * 2) & 31u) == 0;
-    auto kernel = paged_tc_kernel<T, D>;
-    cudaError_t e = allow_smem(kernel, TcSmem<D>::kBytes);
-    if (e == cudaSuccess) e = launch_k(kernel, dim3(sms), dim3(kThreadsTc), TcSmem<D>::kBytes, s, maps, p, tokens, sectors);
+    cudaError_t e = allow_smem<paged_tc_kernel<T, D>>(device, TcSmem<D>::kBytes);
+    if (e == cudaSuccess) e = launch_k(paged_tc_kernel<T, D>, dim3(device.sms), dim3(kThreadsTc), TcSmem<D>::kBytes, s, maps, p, tokens, sectors);
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_attention");
 }
@@ -434,7 +433,7 @@ jfb_status launch(const TcMaps & maps, const AttentionParams & p, uint32_t token
 }  // namespace
 
 jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap & k, const CUtensorMap & v, AttentionParams p,
-                               uint32_t sms, cudaStream_t s) {
+                               const Device & device, cudaStream_t s) {
     const uint32_t tokens = 128 / p.view.group;
     p.view.item_rows = 2 * tokens * p.view.group;
     TcMaps maps;
@@ -444,8 +443,8 @@ jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap 
         return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention: could not encode a TMA tensor map");
     }
     const bool half = cache.dtype == JFB_DTYPE_F16;
-    if (cache.head_dim <= 64) return half ? launch<__half, 64>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 64>(maps, p, tokens, sms, s);
-    return half ? launch<__half, 128>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 128>(maps, p, tokens, sms, s);
+    if (cache.head_dim <= 64) return half ? launch<__half, 64>(maps, p, tokens, device, s) : launch<__nv_bfloat16, 64>(maps, p, tokens, device, s);
+    return half ? launch<__half, 128>(maps, p, tokens, device, s) : launch<__nv_bfloat16, 128>(maps, p, tokens, device, s);
 }
 
 }  // namespace paged

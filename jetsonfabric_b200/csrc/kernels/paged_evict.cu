@@ -1,25 +1,31 @@
 // Eviction: each sequence is cut, kv head by kv head, to its last `recent`
 // keys and the heaviest of the others, in their order.
 //
-// 1. select: a CTA per (sequence, kv head). The keys' masses become unsigned
-//    numbers that order like the floats; four passes over 8-bit digits find
-//    the threshold (the need-th largest), a last pass in slot order keeps all
-//    above it and the first of those that equal it, so ties fall to the lowest
-//    slot and the result is exact. The masses stay in L1/L2 between passes.
-// 2. move: K and V rows to their new slots, 16 bytes a thread, 8 in flight.
-//    Out of place, every (row range, sequence, head) is its own CTA. In place
-//    a CTA owns a column slice of one (sequence, head) and walks the rows in
-//    order, reading a whole step before it writes it: a row only moves to
-//    lower slots, so a step overwrites no later step's source.
+// 1. select: a CTA per (sequence, kv head) brings the masses into shared memory
+//    and orders them as unsigned numbers. The threshold (the need-th largest) is
+//    found two bits at a time by counting how many reach each of three
+//    candidates: sixteen passes without atomics on data, whose cost does not
+//    depend on how the masses are spread (counting digits in a histogram took
+//    three times as long on the usual few octaves). A last pass in slot order
+//    keeps all above it and the first of those that equal it, so ties fall to
+//    the lowest slot and the result is exact.
+// 2. move: K and V rows to their new slots, 16 bytes a thread. Out of place,
+//    every 64 rows of a (sequence, head) are a CTA of their own. In place a CTA
+//    owns a column slice of one (sequence, head) and walks the rows in order,
+//    reading a whole step before it writes it: a row only moves to lower
+//    slots, so a step overwrites no later step's source.
 #include "paged.cuh"
 
 namespace jfb {
 namespace paged {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kPieces = 8;  // 16-byte pieces in flight per thread of the move
+constexpr int kThreads = 1024;  // of the selection
+constexpr uint32_t kWarps = kThreads / 32;
+constexpr uint32_t kCached = 49152;  // masses that fit shared memory
+// threads of the move and 16-byte pieces in flight in each
+constexpr int kFarThreads = 256, kFarPieces = 4;
+constexpr int kNearThreads = 512, kNearPieces = 8;
 
 struct EvictParams {
     View view;
@@ -32,8 +38,8 @@ struct EvictParams {
     void * v;
     uint64_t mass_stride, mass_out_stride, table_out_stride;
     uint32_t budget, recent;
-    uint32_t slices, row_steps;  // of the move's grid
-    bool in_place;
+    uint32_t slices;  // columns of the move in place
+    uint32_t cached;  // masses that the selection's shared memory holds
 };
 
 // Unsigned numbers in the order of the floats; equal zeros, NaN least.
@@ -55,10 +61,9 @@ __device__ __forceinline__ uint32_t evict_length(const EvictParams & p, uint32_t
 }
 
 __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
-    __shared__ uint32_t hist[kWarps][256];
-    __shared__ uint32_t digits[256];
-    __shared__ uint32_t warp_above[kWarps], warp_equal[kWarps];
-    __shared__ uint32_t found, rest;
+    extern __shared__ float cache[];
+    __shared__ uint32_t counts[2][4];
+    __shared__ uint32_t above_of[kWarps], equal_of[kWarps];
     pdl_trigger();
     pdl_wait();
     const uint32_t b = blockIdx.x / p.view.kv_heads, t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -66,120 +71,127 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
     const float * mass = p.mass + uint64_t(blockIdx.x) * p.mass_stride;
     float * mass_out = p.mass_out + uint64_t(blockIdx.x) * p.mass_out_stride;
     int32_t * keep = p.keep + uint64_t(blockIdx.x) * p.budget;
-    uint32_t done = 0;  // kept so far
-    uint32_t tail = 0;  // from here on every slot is kept
-    if (len > p.budget) {
-        tail = len - p.recent;
-        const uint32_t need = p.budget - p.recent;
-        if (need > 0) {
-            // the need-th largest of slots [0, tail): need <= budget - recent < tail
-            uint32_t prefix = 0, left = need;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (uint32_t i = t; i < kWarps * 256; i += kThreads) (&hist[0][0])[i] = 0;
-                __syncthreads();
-                const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-                for (uint32_t j = t; j < tail; j += kThreads) {
-                    const uint32_t key = order_key(mass[j]);
-                    if ((key & mask) == prefix) atomicAdd(&hist[warp][(key >> shift) & 255u], 1u);
-                }
-                __syncthreads();
-                if (t < 256) {
-                    uint32_t sum = 0;
-                    for (int w = 0; w < kWarps; ++w) sum += hist[w][t];
-                    digits[t] = sum;
-                }
-                __syncthreads();
-                if (warp == 0) {
-                    // from the largest digit down: lane l holds digits 255 - 8l .. 248 - 8l
-                    uint32_t mine = 0;
-                    for (int i = 0; i < 8; ++i) mine += digits[255 - 8 * lane - i];
-                    uint32_t upto = mine;
-#pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
-                        if (int(lane) >= d) upto += o;
-                    }
-                    const uint32_t over = __ballot_sync(0xffffffffu, upto >= left);
-                    if (int(lane) == __ffs(over) - 1) {
-                        uint32_t r = left - (upto - mine);
-                        uint32_t d = 255 - 8 * lane;
-                        while (digits[d] < r) r -= digits[d--];
-                        found = d;
-                        rest = r;
-                    }
-                }
-                __syncthreads();
-                prefix |= found << shift;
-                left = rest;
-            }
-            // keep everything above the threshold and its first `left` equals
-            uint32_t equal_before = 0;
-            for (uint32_t base = 0; base < tail; base += kThreads) {
-                const uint32_t j = base + t;
-                const float x = j < tail ? mass[j] : 0.0f;
-                const uint32_t key = order_key(x);
-                const bool above = j < tail && key > prefix, equal = j < tail && key == prefix;
-                const uint32_t va = __ballot_sync(0xffffffffu, above), ve = __ballot_sync(0xffffffffu, equal);
-                if (lane == 0) {
-                    warp_above[warp] = __popc(va);
-                    warp_equal[warp] = __popc(ve);
-                }
-                __syncthreads();
-                uint32_t a = 0, e = 0, all_a = 0, all_e = 0;
-                for (int w = 0; w < kWarps; ++w) {
-                    const uint32_t ca = warp_above[w], ce = warp_equal[w];
-                    if (w < int(warp)) a += ca, e += ce;
-                    all_a += ca;
-                    all_e += ce;
-                }
-                const uint32_t below = (1u << lane) - 1u;
-                a += __popc(va & below);
-                e += equal_before + __popc(ve & below);
-                // kept before this slot: those above, and equals up to `left`
-                if (above || (equal && e < left)) {
-                    const uint32_t at = done + a + min(e, left) - min(equal_before, left);
-                    keep[at] = int32_t(j);
-                    mass_out[at] = x;
-                }
-                done += all_a + min(equal_before + all_e, left) - min(equal_before, left);
-                equal_before += all_e;
-                __syncthreads();
-            }
+    const uint32_t kept = min(len, p.budget);
+    for (uint32_t i = kept + t; i < p.budget; i += kThreads) keep[i] = -1;
+    if (len <= p.budget) {
+        for (uint32_t i = t; i < len; i += kThreads) {
+            keep[i] = int32_t(i);
+            mass_out[i] = mass[i];
         }
+        return;
     }
-    for (uint32_t base = tail; base < len; base += kThreads) {
-        const uint32_t j = base + t;
-        const float x = j < len ? mass[j] : 0.0f;
-        __syncthreads();  // in place: read before anything behind it is written
-        if (j < len) {
-            keep[done + (j - tail)] = int32_t(j);
-            mass_out[done + (j - tail)] = x;
+    const bool cached = len <= p.cached;
+    if (cached) {
+        for (uint32_t i = t; i < len; i += kThreads) cache[i] = mass[i];
+    }
+    if (t < 8) counts[t >> 2][t & 3] = 0;
+    __syncthreads();
+    const auto mass_of = [&](uint32_t j) { return cached ? cache[j] : mass[j]; };
+    const uint32_t tail = len - p.recent;  // from here on every slot is kept
+    const uint32_t need = p.budget - p.recent;
+    if (need > 0) {
+        // the need-th largest of slots [0, tail): need < tail
+        uint32_t threshold = 0, above = 0;  // above: how many exceed it
+        for (int shift = 30; shift >= 0; shift -= 2) {
+            const uint32_t c1 = threshold | (1u << shift), c2 = threshold | (2u << shift), c3 = threshold | (3u << shift);
+            uint32_t n1 = 0, n2 = 0, n3 = 0;
+            for (uint32_t j = t; j < tail; j += kThreads) {
+                const uint32_t k = order_key(mass_of(j));
+                n1 += k >= c1;
+                n2 += k >= c2;
+                n3 += k >= c3;
+            }
+            n1 = __reduce_add_sync(0xffffffffu, n1);
+            n2 = __reduce_add_sync(0xffffffffu, n2);
+            n3 = __reduce_add_sync(0xffffffffu, n3);
+            uint32_t * sum = counts[(shift >> 1) & 1];
+            if (lane == 0) {
+                atomicAdd(sum + 1, n1);
+                atomicAdd(sum + 2, n2);
+                atomicAdd(sum + 3, n3);
+            }
+            if (t < 4) counts[((shift >> 1) & 1) ^ 1][t] = 0;  // read by all before the barrier of the pass before
+            __syncthreads();
+            n1 = sum[1], n2 = sum[2], n3 = sum[3];
+            const uint32_t digit = n3 >= need ? 3u : n2 >= need ? 2u : n1 >= need ? 1u : 0u;
+            if (digit < 3) above = digit == 2 ? n3 : digit == 1 ? n2 : n1;
+            threshold |= digit << shift;
+            __syncthreads();
+        }
+        // keep everything above the threshold and the first `ties` that equal it: a warp per run of slots
+        const uint32_t ties = need - above;
+        const uint32_t run = (tail + kThreads - 1) / kThreads * 32, begin = min(tail, warp * run), end = min(tail, begin + run);
+        uint32_t na = 0, ne = 0;
+        for (uint32_t j = begin + lane; j < end; j += 32) {
+            const uint32_t k = order_key(mass_of(j));
+            na += k > threshold;
+            ne += k == threshold;
+        }
+        na = __reduce_add_sync(0xffffffffu, na);
+        ne = __reduce_add_sync(0xffffffffu, ne);
+        if (lane == 0) {
+            above_of[warp] = na;
+            equal_of[warp] = ne;
         }
         __syncthreads();
+        na = __reduce_add_sync(0xffffffffu, lane < warp ? above_of[lane] : 0u);  // before this run
+        ne = __reduce_add_sync(0xffffffffu, lane < warp ? equal_of[lane] : 0u);
+        const uint32_t below = (1u << lane) - 1u;
+        for (uint32_t base = begin; base < end; base += 32) {
+            const uint32_t j = base + lane;
+            const float x = j < end ? mass_of(j) : 0.0f;
+            const uint32_t k = order_key(x);
+            const uint32_t va = __ballot_sync(0xffffffffu, j < end && k > threshold);
+            const uint32_t ve = __ballot_sync(0xffffffffu, j < end && k == threshold);
+            const uint32_t a = na + __popc(va & below), e = ne + __popc(ve & below);
+            if (((va >> lane) & 1u) != 0 || (((ve >> lane) & 1u) != 0 && e < ties)) {
+                const uint32_t at = a + min(e, ties);
+                keep[at] = int32_t(j);
+                if (cached) mass_out[at] = x;
+            }
+            na += __popc(va);
+            ne += __popc(ve);
+        }
     }
-    for (uint32_t i = min(len, p.budget) + t; i < p.budget; i += kThreads) keep[i] = -1;
+    for (uint32_t j = tail + t; j < len; j += kThreads) {
+        keep[need + (j - tail)] = int32_t(j);
+        if (cached) mass_out[need + (j - tail)] = cache[j];
+    }
+    if (!cached) {
+        // the masses in order, each step read before it is written: they may move in place
+        __syncthreads();
+        for (uint32_t base = 0; base < kept; base += kThreads) {
+            const float x = base + t < kept ? mass[keep[base + t]] : 0.0f;
+            __syncthreads();
+            if (base + t < kept) mass_out[base + t] = x;
+            __syncthreads();
+        }
+    }
 }
 
-__global__ void __launch_bounds__(kThreads) move_kernel(const EvictParams p) {
+template <int THREADS, int PIECES, bool IN_PLACE>
+__global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
     pdl_trigger();
     pdl_wait();
     const View & v = p.view;
-    const uint32_t line = blockIdx.x >> 1, b = line / v.kv_heads, head = line % v.kv_heads;
+    const uint32_t line = blockIdx.x >> 1, b = line / v.kv_heads, head = line - b * v.kv_heads;
     uint16_t * pool = static_cast<uint16_t *>((blockIdx.x & 1) ? p.v : p.k);
     const int32_t * keep = p.keep + uint64_t(line) * p.budget;
     const int32_t * from = v.table + uint64_t(b) * v.table_stride;
     const int32_t * to = p.table_out + uint64_t(b) * p.table_out_stride;
-    const uint32_t width = v.head_dim / 8 / p.slices, first = blockIdx.y * width;  // pieces of a row
-    const uint32_t step = kThreads * kPieces / width;                                // rows read before they are written
-    const uint32_t len = evict_length(p, b);
-    const uint32_t kept = min(len, p.budget);
-    const uint32_t begin = p.in_place ? 0u : blockIdx.z * step, end = p.in_place ? kept : min(kept, begin + step);
+    const uint32_t width = v.head_dim / 8 / p.slices, first = blockIdx.z * width;  // pieces of a row
+    const uint32_t step = THREADS * PIECES / width;                                  // rows read before they are written
+    const uint32_t kept = min(evict_length(p, b), p.budget);
+    // The new length may replace the old one that other CTAs still read: they
+    // cut either to the same number of rows.
+    if (head == 0 && (blockIdx.x & 1) == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.kv_len_out[b] = int32_t(kept);
+    const uint32_t begin = IN_PLACE ? 0u : blockIdx.y * step, end = IN_PLACE ? kept : min(kept, begin + step);
     for (uint32_t row0 = begin; row0 < end; row0 += step) {
-        uint4 x[kPieces];
-        uint64_t dst[kPieces];
+        uint4 x[PIECES];
+        uint64_t dst[PIECES];
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
-            const uint32_t i = threadIdx.x + u * kThreads, r = i / width, c = (first + i - r * width) * 8;
+        for (int u = 0; u < PIECES; ++u) {
+            const uint32_t i = threadIdx.x + u * THREADS, r = i / width, c = (first + i - r * width) * 8;
             dst[u] = ~0ull;
             x[u] = make_uint4(0, 0, 0, 0);
             if (r < step && row0 + r < end) {
@@ -197,21 +209,13 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const EvictParams p) {
                 }
             }
         }
-        if (p.in_place) __syncthreads();
+        if (IN_PLACE) __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
+        for (int u = 0; u < PIECES; ++u) {
             if (dst[u] != ~0ull) *reinterpret_cast<uint4 *>(pool + dst[u]) = x[u];
         }
-        if (p.in_place) __syncthreads();
+        if (IN_PLACE) __syncthreads();
     }
-}
-
-// The new lengths, written last: kv_len_out may be the batch's kv_len.
-__global__ void __launch_bounds__(kThreads) length_kernel(const EvictParams p) {
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t b = blockIdx.x * kThreads + threadIdx.x;
-    if (b < p.view.sequences) p.kv_len_out[b] = int32_t(min(evict_length(p, b), p.budget));
 }
 
 }  // namespace
@@ -263,22 +267,26 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     p.table_out_stride = table_out_stride;
     p.budget = budget;
     p.recent = recent;
-    p.in_place = page_table_out == batch->page_table;
-    // column slices of at least 64 bytes (DRAM's granularity) while in-place CTAs do not fill the SMs
+    p.cached = mass_stride < kCached ? uint32_t(mass_stride) : kCached;
+    const bool in_place = page_table_out == batch->page_table;
     const uint32_t lines = batch->sequences * cache->kv_heads;
     const uint32_t pieces = cache->head_dim / 8;
+    // in place: column slices of at least 64 bytes (DRAM's granularity) while the CTAs do not fill the SMs four times
+    const Device device = current_device();
     p.slices = 1;
-    while (p.in_place && p.slices < 4 && pieces % (p.slices * 2) == 0 && pieces / (p.slices * 2) >= 4 && lines * 2 * p.slices < 4 * 148) {
+    while (in_place && p.slices < 4 && pieces % (p.slices * 2) == 0 && pieces / (p.slices * 2) >= 4 && lines * 2 * p.slices < 4 * device.sms) {
         p.slices *= 2;
     }
-    const uint32_t step = kThreads * kPieces / (pieces / p.slices);
-    const uint32_t steps = p.in_place ? 1u : (budget + step - 1) / step;
+    const uint32_t step = kFarThreads * kFarPieces / pieces;
+    const uint32_t steps = in_place ? 1u : (budget + step - 1) / step;
     if (steps > 65535u) return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: a budget of %u is too large", budget);
-    p.row_steps = steps;
     cudaStream_t s = as_stream(stream);
-    cudaError_t e = launch_k(select_kernel, dim3(lines), dim3(kThreads), 0, s, p);
-    if (e == cudaSuccess) e = launch_k(move_kernel, dim3(lines * 2, p.slices, steps), dim3(kThreads), 0, s, p);
-    if (e == cudaSuccess) e = launch_k(length_kernel, dim3((batch->sequences + kThreads - 1) / kThreads), dim3(kThreads), 0, s, p);
+    cudaError_t e = allow_smem<select_kernel>(device, kCached * sizeof(float));
+    if (e == cudaSuccess) e = launch_k(select_kernel, dim3(lines), dim3(kThreads), p.cached * sizeof(float), s, p);
+    if (e == cudaSuccess) {
+        e = in_place ? launch_k(move_kernel<kNearThreads, kNearPieces, true>, dim3(lines * 2, 1, p.slices), dim3(kNearThreads), 0, s, p)
+                     : launch_k(move_kernel<kFarThreads, kFarPieces, false>, dim3(lines * 2, steps), dim3(kFarThreads), 0, s, p);
+    }
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_evict: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_evict");
 }

@@ -218,10 +218,9 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
 }
 
 template <typename T, int D>
-jfb_status launch_rows(const CUtensorMap & k, const MassParams & p, uint32_t sms, cudaStream_t s) {
-    auto kernel = mass_rows_kernel<T, D>;
-    cudaError_t e = allow_smem(kernel, MassSmem<D>::kBytes);
-    if (e == cudaSuccess) e = launch_k(kernel, dim3(sms), dim3(kThreadsRows), MassSmem<D>::kBytes, s, k, p);
+jfb_status launch_rows(const CUtensorMap & k, const MassParams & p, const Device & device, cudaStream_t s) {
+    cudaError_t e = allow_smem<mass_rows_kernel<T, D>>(device, MassSmem<D>::kBytes);
+    if (e == cudaSuccess) e = launch_k(mass_rows_kernel<T, D>, dim3(device.sms), dim3(kThreadsRows), MassSmem<D>::kBytes, s, k, p);
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_attention_mass");
 }
@@ -248,8 +247,8 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
         return status_error(JFB_STATUS_INVALID_ARGUMENT,
                             "jfb_paged_attention_mass needs a positive finite scale and a window below 2^31");
     }
-    const uint32_t sms = device_sms();
-    if (sms == 0) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no usable device");
+    const Device device = current_device();
+    if (device.sms == 0) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no usable device");
     if (batch->sequences == 0) return status_ok();
     MassParams p;
     p.view = make_view(*cache, *batch, rows, heads / cache->kv_heads, window, error_flag);
@@ -268,9 +267,9 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
     const uint32_t group = p.view.group;
-    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_mass_tc(*cache, mk, p, sms, s);
+    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_mass_tc(*cache, mk, p, device, s);
     if (cache->head_dim <= 64) {
-        return half ? launch_rows<__half, 64>(mk, p, sms, s) : launch_rows<__nv_bfloat16, 64>(mk, p, sms, s);
+        return half ? launch_rows<__half, 64>(mk, p, device, s) : launch_rows<__nv_bfloat16, 64>(mk, p, device, s);
     }
-    return half ? launch_rows<__half, 128>(mk, p, sms, s) : launch_rows<__nv_bfloat16, 128>(mk, p, sms, s);
+    return half ? launch_rows<__half, 128>(mk, p, device, s) : launch_rows<__nv_bfloat16, 128>(mk, p, device, s);
 }

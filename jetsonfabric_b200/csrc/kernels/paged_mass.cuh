@@ -18,7 +18,7 @@ struct MassParams {
 };
 
 // The tcgen05 kernel of paged_mass_tc.cu.
-jfb_status launch_mass_tc(const jfb_paged_cache & cache, const CUtensorMap & k, MassParams p, uint32_t sms, cudaStream_t s);
+jfb_status launch_mass_tc(const jfb_paged_cache & cache, const CUtensorMap & k, MassParams p, const Device & device, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace jfb

@@ -406,9 +406,9 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
 }
 
 template <typename T, int D>
-jfb_status launch(const MassMaps & maps, const MassParams & p, uint32_t tokens, uint32_t sms, cudaStream_t s) {
-    auto kernel = mass_tc_kernel<T, D>;
-    cudaError_t e = allow_smem(kernel, MassTcSmem<D>::kBytes);
+jfb_status launch(const MassMaps & maps, const MassParams & p, uint32_t tokens, const Device & device, cudaStream_t s) {
+    constexpr auto kernel = mass_tc_kernel<T, D>;
+    cudaError_t e = allow_smem<mass_tc_kernel<T, D>>(device, MassTcSmem<D>::kBytes);
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kThreadsMass);
     cfg.dynamicSmemBytes = MassTcSmem<D>::kBytes;
@@ -423,19 +423,17 @@ jfb_status launch(const MassMaps & maps, const MassParams & p, uint32_t tokens, 
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     // as many clusters as the GPCs hold at once: the line is divided evenly among them
-    cfg.gridDim = dim3(sms / kCluster * kCluster);
-    if (e == cudaSuccess) {
-        static std::mutex mu;
-        static int known[64] = {0};  // per device
-        int device = 0;
-        e = cudaGetDevice(&device);
-        const std::lock_guard<std::mutex> lock(mu);
-        int n = device >= 0 && device < 64 ? known[device] : 0;
-        if (e == cudaSuccess && n == 0) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-        if (e == cudaSuccess && n < 1) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no room for a cluster");
-        if (device >= 0 && device < 64) known[device] = n;
-        cfg.gridDim = dim3(uint32_t(n) < sms / kCluster ? uint32_t(n) * kCluster : sms / kCluster * kCluster);
+    const uint32_t most = device.sms / kCluster;
+    cfg.gridDim = dim3(most * kCluster);
+    static std::atomic<int> known[64];  // per device
+    const bool keep = device.index >= 0 && device.index < 64;
+    int n = keep ? known[device.index].load(std::memory_order_relaxed) : 0;
+    if (e == cudaSuccess && n == 0) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e == cudaSuccess && (n < 1 || most < 1)) {
+        return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no room for a cluster");
     }
+    if (e == cudaSuccess && keep) known[device.index].store(n, std::memory_order_relaxed);
+    if (uint32_t(n) < most) cfg.gridDim = dim3(uint32_t(n) * kCluster);
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, maps, p, tokens);
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_attention_mass");
@@ -443,7 +441,7 @@ jfb_status launch(const MassMaps & maps, const MassParams & p, uint32_t tokens, 
 
 }  // namespace
 
-jfb_status launch_mass_tc(const jfb_paged_cache & cache, const CUtensorMap & k, MassParams p, uint32_t sms, cudaStream_t s) {
+jfb_status launch_mass_tc(const jfb_paged_cache & cache, const CUtensorMap & k, MassParams p, const Device & device, cudaStream_t s) {
     const uint32_t tokens = 128 / p.view.group;
     p.view.item_rows = tokens * p.view.group;
     MassMaps maps;
@@ -452,8 +450,8 @@ jfb_status launch_mass_tc(const jfb_paged_cache & cache, const CUtensorMap & k, 
         return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: could not encode a TMA tensor map");
     }
     const bool half = cache.dtype == JFB_DTYPE_F16;
-    if (cache.head_dim <= 64) return half ? launch<__half, 64>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 64>(maps, p, tokens, sms, s);
-    return half ? launch<__half, 128>(maps, p, tokens, sms, s) : launch<__nv_bfloat16, 128>(maps, p, tokens, sms, s);
+    if (cache.head_dim <= 64) return half ? launch<__half, 64>(maps, p, tokens, device, s) : launch<__nv_bfloat16, 64>(maps, p, tokens, device, s);
+    return half ? launch<__half, 128>(maps, p, tokens, device, s) : launch<__nv_bfloat16, 128>(maps, p, tokens, device, s);
 }
 
 }  // namespace paged

@@ -43,11 +43,16 @@ class RopeC(C.Structure):
 
 
 _bound = None
+torch = None
+_DTYPES: dict = {}  # torch dtype -> jfb_dtype
+_raw_stream = None
 
 
 def _bind():
-    global _bound
+    """The library with its signatures; binds torch on first use like the other modules."""
+    global _bound, torch, _raw_stream
     if _bound is None:
+        import torch as t
         L = lib()
         cache, batch = C.POINTER(CacheC), C.POINTER(BatchC)
         sig = {
@@ -67,23 +72,17 @@ def _bind():
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = res
+        torch = t
+        _DTYPES.update({t.float32: 0, t.float16: 1, t.bfloat16: 2})
+        # the current stream's address without building a Stream object, where torch offers it
+        _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (lambda i: t.cuda.current_stream(i).cuda_stream)
         _bound = L
     return _bound
-
-
-def _torch():
-    import torch
-    return torch
 
 
 def _require(ok: bool, message: str) -> None:
     if not ok:
         raise InvalidArgument(message)
-
-
-def _dtypes():
-    torch = _torch()
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 class PagedCache:
@@ -93,7 +92,7 @@ class PagedCache:
     head_dim] is passed as pool.transpose(1, 2)."""
 
     def __init__(self, k, v):
-        torch = _torch()
+        _bind()
         _require(k.dim() == 4 and k.shape == v.shape, "paged pools are [pages, page_size, kv_heads, head_dim]")
         _require(k.is_cuda and v.device == k.device, "paged pools must be on one CUDA device")
         _require(k.dtype in (torch.float16, torch.bfloat16) and v.dtype == k.dtype, "paged pools are float16 or bfloat16")
@@ -108,13 +107,15 @@ class PagedCache:
                 strides.append(k.stride(dim))
         self.k, self.v, self.device = k, v, k.device
         self.dtype = k.dtype
+        self.scale = k.shape[3] ** -0.5
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
-        self.desc = CacheC(k.data_ptr(), v.data_ptr(), *strides, _dtypes()[k.dtype], *k.shape, 0)
+        self.desc = CacheC(k.data_ptr(), v.data_ptr(), *strides, _DTYPES[k.dtype], *k.shape, 0)
         self.ref = C.byref(self.desc)
 
 
 def _int32(t, dim: int, device, what: str) -> None:
-    _require(t.dtype == _torch().int32 and t.dim() == dim and t.device == device, f"{what} must be int32 on the cache's device")
+    if t.dtype != torch.int32 or t.dim() != dim or t.device != device:
+        raise InvalidArgument(f"{what} must be int32 with {dim} dimensions on the cache's device")
 
 
 class PagedBatch:
@@ -124,6 +125,7 @@ class PagedBatch:
     change between calls."""
 
     def __init__(self, q_start, kv_len, page_table):
+        _bind()
         dev = q_start.device
         _require(q_start.is_cuda, "paged batch arrays must be on a CUDA device")
         _int32(q_start, 1, dev, "q_start")
@@ -166,7 +168,8 @@ class Rope:
     float64 CUDA tensor of radians per position, `factor` multiplies cos and sin."""
 
     def __init__(self, freq, interleaved: bool = False, factor: float = 1.0):
-        _require(freq.is_cuda and freq.dtype == _torch().float64 and freq.dim() == 1 and freq.is_contiguous() and freq.numel() > 0,
+        _bind()
+        _require(freq.is_cuda and freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous() and freq.numel() > 0,
                  "rope frequencies are a contiguous float64 CUDA vector")
         self.freq, self.device = freq, freq.device
         self.desc = RopeC(freq.data_ptr(), 2 * freq.numel(), int(interleaved), factor, 0)
@@ -175,52 +178,64 @@ class Rope:
     @classmethod
     def scaled(cls, rope_dims: int, base: float, scaling: str = "none", interleaved: bool = False, device="cuda", **kw):
         freq, factor = rope_frequencies(rope_dims, base, scaling, **kw)
-        return cls(_torch().from_numpy(freq).to(device), interleaved, factor)
+        return cls(torch.from_numpy(freq).to(device), interleaved, factor)
 
 
-def _rows(x, cache: PagedCache, what: str, dtype=None):
+def _rows(x, cache: PagedCache, what: str):
     """(address, row stride, rows, heads) of [rows, heads, head_dim] or [rows, heads * head_dim]."""
-    _require(x.device == cache.device, f"{what} must be on the cache's device")
-    _require(dtype is None or x.dtype == dtype, f"{what} must be {dtype}")
+    if x.device != cache.device:
+        raise InvalidArgument(f"{what} must be on the cache's device")
     hd = cache.head_dim
-    shape = x.shape
+    shape, strides = x.shape, x.stride()
+    rows = shape[0] if shape else 0
     if len(shape) == 3:
         heads = shape[1]
-        ok = shape[2] == hd and (hd == 1 or x.stride(2) == 1) and (heads == 1 or x.stride(1) == hd)
+        ok = shape[2] == hd and strides[2] == 1 and (strides[1] == hd or heads == 1)
     else:
-        ok = len(shape) == 2 and shape[1] % hd == 0 and (shape[1] == 1 or x.stride(1) == 1)
+        ok = len(shape) == 2 and shape[1] % hd == 0 and strides[1] == 1
         heads = shape[1] // hd if ok else 0
-    _require(ok and heads > 0, f"{what} must be rows of contiguous heads of {hd}")
-    stride = x.stride(0) if shape[0] > 1 else heads * hd
-    _require(stride >= heads * hd, f"{what} rows overlap")
-    return x.data_ptr(), stride, shape[0], heads
+    if not ok or heads == 0:
+        raise InvalidArgument(f"{what} must be rows of contiguous heads of {hd}")
+    stride = strides[0] if rows > 1 else heads * hd  # a single row is never stepped over
+    if stride < heads * hd:
+        raise InvalidArgument(f"{what} rows overlap")
+    return x.data_ptr(), stride, rows, heads
+
+
+def _cache_rows(x, cache: PagedCache, what: str):
+    if x.dtype != cache.dtype:
+        raise InvalidArgument(f"{what} must have the cache's dtype, {cache.dtype}")
+    return _rows(x, cache, what)
 
 
 def _flag(error_flag, device):
     if error_flag is None:
         return None
-    _require(error_flag.dtype == _torch().int32 and error_flag.device == device and error_flag.numel() == 1,
+    _require(error_flag.dtype == torch.int32 and error_flag.device == device and error_flag.numel() == 1,
              "error_flag must be one int32 on the cache's device")
     return error_flag.data_ptr()
 
 
-def _call(name: str, device, stream, *args) -> None:
+def _call(fn, device, stream, *args) -> None:
     """The C call on the device of its tensors, on `stream` or that device's current one."""
-    torch = _torch()
-    fn = getattr(_bind(), name)
+    index = device.index
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        address = _raw_stream(index)
     else:
         _require(stream.device == device, "the stream must be on the cache's device")
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, stream.cuda_stream))
+        address = stream.cuda_stream
+    if index == torch.cuda.current_device():
+        status = fn(*args, address)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, stream.cuda_stream))
+            status = fn(*args, address)
+    if status.code:
+        check(status)
 
 
 def _on(batch: PagedBatch, cache: PagedCache) -> None:
-    _require(batch.device == cache.device, "cache and batch must be on one device")
+    if batch.device != cache.device:
+        raise InvalidArgument("cache and batch must be on one device")
 
 
 def rope_append(q, k, v, pos, rope: Rope, cache: PagedCache, batch: PagedBatch, q_out, error_flag=None, stream=None) -> None:
@@ -229,27 +244,27 @@ def rope_append(q, k, v, pos, rope: Rope, cache: PagedCache, batch: PagedBatch, 
     (float32, float16 or bfloat16), q_out has the cache's; pos int32 [rows]."""
     _on(batch, cache)
     _require(rope.device == cache.device, "rope and cache must be on one device")
-    dtype = _dtypes().get(q.dtype)
+    dtype = _DTYPES.get(q.dtype)
     _require(dtype is not None and k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must share a float dtype")
     qp, qs, rows, heads = _rows(q, cache, "q")
     kp, ks, k_rows, k_heads = _rows(k, cache, "k")
     vp, vs, v_rows, v_heads = _rows(v, cache, "v")
-    op, os, o_rows, o_heads = _rows(q_out, cache, "q_out", cache.dtype)
+    op, os, o_rows, o_heads = _cache_rows(q_out, cache, "q_out")
     _require(k_rows == v_rows == o_rows == rows, "q, k, v and q_out must have the same rows")
     _require(k_heads == v_heads == cache.kv_heads and o_heads == heads, "the heads of q, k, v and q_out do not fit the cache")
     _int32(pos, 1, cache.device, "pos")
     _require(pos.shape[0] == rows and pos.is_contiguous(), "pos must hold one position per row")
-    _call("jfb_rope_paged_append", cache.device, stream, qp, kp, vp, dtype, qs, ks, vs, rows, heads, pos.data_ptr(), rope.ref,
+    _call(_bound.jfb_rope_paged_append, cache.device, stream, qp, kp, vp, dtype, qs, ks, vs, rows, heads, pos.data_ptr(), rope.ref,
           cache.ref, batch.ref, op, os, _flag(error_flag, cache.device))
 
 
 def attention_workspace(device=None):
     """A zero-filled workspace for attention() on `device`: one per stream that
     runs attention calls, or captured graph that may overlap others."""
-    torch = _torch()
+    L = _bind()
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):
-        return torch.zeros(int(_bind().jfb_paged_attention_workspace_bytes()), dtype=torch.uint8, device=dev)
+        return torch.zeros(int(L.jfb_paged_attention_workspace_bytes()), dtype=torch.uint8, device=dev)
 
 
 def attention(q, cache: PagedCache, batch: PagedBatch, out, workspace, scale: float | None = None, window: int = 0, lse=None,
@@ -258,13 +273,13 @@ def attention(q, cache: PagedCache, batch: PagedBatch, out, workspace, scale: fl
     with `window` > 0 only over the last `window` slots (jfb_paged_attention);
     lse, if given, float32 [rows, heads]. scale defaults to head_dim ** -0.5."""
     _on(batch, cache)
-    qp, qs, rows, heads = _rows(q, cache, "q", cache.dtype)
-    op, os, o_rows, o_heads = _rows(out, cache, "out", cache.dtype)
+    qp, qs, rows, heads = _cache_rows(q, cache, "q")
+    op, os, o_rows, o_heads = _cache_rows(out, cache, "out")
     _require(o_rows == rows and o_heads == heads, "q and out must have the same rows and heads")
     _lse(lse, rows, heads, cache, optional=True)
     _require(workspace.device == cache.device and workspace.is_contiguous(), "workspace must be on the cache's device")
     _window(window)
-    _call("jfb_paged_attention", cache.device, stream, qp, qs, rows, heads, cache.head_dim ** -0.5 if scale is None else scale,
+    _call(_bound.jfb_paged_attention, cache.device, stream, qp, qs, rows, heads, cache.scale if scale is None else scale,
           window, cache.ref, batch.ref, op, os, None if lse is None else lse.data_ptr(), workspace.data_ptr(),
           workspace.numel() * workspace.element_size(), _flag(error_flag, cache.device))
 
@@ -276,12 +291,12 @@ def _window(window: int) -> None:
 def _lse(lse, rows, heads, cache, optional=False) -> None:
     if lse is None and optional:
         return
-    _require(lse.dtype == _torch().float32 and lse.device == cache.device and lse.shape == (rows, heads) and lse.is_contiguous(),
+    _require(lse.dtype == torch.float32 and lse.device == cache.device and lse.shape == (rows, heads) and lse.is_contiguous(),
              "lse must be contiguous float32 [rows, heads]")
 
 
 def _masses(x, batch: PagedBatch, cache: PagedCache, what: str) -> int:
-    _require(x.dtype == _torch().float32 and x.device == cache.device and x.dim() == 3 and x.is_contiguous() and
+    _require(x.dtype == torch.float32 and x.device == cache.device and x.dim() == 3 and x.is_contiguous() and
              x.shape[0] == batch.sequences and x.shape[1] == cache.kv_heads and x.shape[2] > 0,
              f"{what} must be contiguous float32 [sequences, kv_heads, slots]")
     return x.shape[2]
@@ -293,14 +308,14 @@ def attention_mass(q, lse, cache: PagedCache, batch: PagedBatch, mass_out, mass_
     and everywhere without mass_in) plus the attention weight every key received
     from the rows of q (jfb_paged_attention_mass); mass_in may be mass_out."""
     _on(batch, cache)
-    qp, qs, rows, heads = _rows(q, cache, "q", cache.dtype)
+    qp, qs, rows, heads = _cache_rows(q, cache, "q")
     _lse(lse, rows, heads, cache)
     slots = _masses(mass_out, batch, cache, "mass_out")
     if mass_in is not None:
         _require(_masses(mass_in, batch, cache, "mass_in") == slots, "mass_in and mass_out must hold the same slots")
     _window(window)
-    _call("jfb_paged_attention_mass", cache.device, stream, qp, qs, rows, heads,
-          cache.head_dim ** -0.5 if scale is None else scale, window, lse.data_ptr(), cache.ref, batch.ref,
+    _call(_bound.jfb_paged_attention_mass, cache.device, stream, qp, qs, rows, heads,
+          cache.scale if scale is None else scale, window, lse.data_ptr(), cache.ref, batch.ref,
           None if mass_in is None else mass_in.data_ptr(), mass_out.data_ptr(), slots, _flag(error_flag, cache.device))
 
 
@@ -325,6 +340,6 @@ def evict(mass, cache: PagedCache, batch: PagedBatch, keep, kv_len_out, recent: 
              "keep must be contiguous [sequences, kv_heads, budget]")
     _require(kv_len_out.is_contiguous() and kv_len_out.shape[0] == batch.sequences, "kv_len_out must be [sequences]")
     _require(0 <= recent <= keep.shape[2], "recent must be from 0 to the budget")
-    _call("jfb_paged_evict", cache.device, stream, mass.data_ptr(), slots, cache.ref, batch.ref, keep.shape[2], recent,
+    _call(_bound.jfb_paged_evict, cache.device, stream, mass.data_ptr(), slots, cache.ref, batch.ref, keep.shape[2], recent,
           keep.data_ptr(), kv_len_out.data_ptr(), mass_out.data_ptr(), out_slots, table.data_ptr(), _row_stride(table),
           table.shape[1], _flag(error_flag, cache.device))
