@@ -4,13 +4,14 @@
 // 1. select: a CTA per (sequence, kv head) brings the masses into shared memory
 //    and orders them as unsigned numbers. The threshold (the need-th largest) is
 //    found two bits at a time by counting how many reach each of three
-//    candidates: sixteen passes without atomics on data, whose cost does not
-//    depend on how the masses are spread (counting digits in a histogram took
-//    three times as long on the usual few octaves). A last pass in slot order
+//    candidates: sixteen passes over registers (up to 16384 keys) with one
+//    barrier each, whose cost does not depend on how the masses are spread
+//    (a histogram of digits in shared memory was slower: the usual few octaves
+//    make its counters collide). A last pass in slot order
 //    keeps all above it and the first of those that equal it, so ties fall to
 //    the lowest slot and the result is exact.
 // 2. move: K and V rows to their new slots, 16 bytes a thread. Out of place,
-//    every 64 rows of a (sequence, head) are a CTA of their own. In place a CTA
+//    every 32 rows of a (sequence, head) are a CTA of their own (D = 128). In place a CTA
 //    owns a column slice of one (sequence, head) and walks the rows in order,
 //    reading a whole step before it writes it: a row only moves to lower
 //    slots, so a step overwrites no later step's source.
@@ -23,8 +24,9 @@ namespace {
 constexpr int kThreads = 1024;  // of the selection
 constexpr uint32_t kWarps = kThreads / 32;
 constexpr uint32_t kCached = 49152;  // masses that fit shared memory
+constexpr uint32_t kOwn = 16;        // keys a thread of the selection holds
 // threads of the move and 16-byte pieces in flight in each
-constexpr int kFarThreads = 256, kFarPieces = 4;
+constexpr int kFarThreads = 256, kFarPieces = 2;
 constexpr int kNearThreads = 512, kNearPieces = 8;
 
 struct EvictParams {
@@ -62,7 +64,7 @@ __device__ __forceinline__ uint32_t evict_length(const EvictParams & p, uint32_t
 
 __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
     extern __shared__ float cache[];
-    __shared__ uint32_t counts[2][4];
+    __shared__ uint32_t counts[2][3][kWarps];
     __shared__ uint32_t above_of[kWarps], equal_of[kWarps];
     pdl_trigger();
     pdl_wait();
@@ -82,41 +84,75 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
     }
     const bool cached = len <= p.cached;
     if (cached) {
+#pragma unroll 8
         for (uint32_t i = t; i < len; i += kThreads) cache[i] = mass[i];
     }
-    if (t < 8) counts[t >> 2][t & 3] = 0;
     __syncthreads();
     const auto mass_of = [&](uint32_t j) { return cached ? cache[j] : mass[j]; };
     const uint32_t tail = len - p.recent;  // from here on every slot is kept
     const uint32_t need = p.budget - p.recent;
     if (need > 0) {
         // the need-th largest of slots [0, tail): need < tail
-        uint32_t threshold = 0, above = 0;  // above: how many exceed it
+        const bool own = cached && tail <= kOwn * kThreads;
+        uint32_t keys[kOwn];  // 0 reaches no candidate
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            const uint32_t j = t + i * kThreads;
+            keys[i] = own && j < tail ? order_key(cache[j]) : 0u;
+        }
+        uint32_t threshold = 0, above = 0, reach = tail;  // how many exceed it, and how many reach it
         for (int shift = 30; shift >= 0; shift -= 2) {
             const uint32_t c1 = threshold | (1u << shift), c2 = threshold | (2u << shift), c3 = threshold | (3u << shift);
             uint32_t n1 = 0, n2 = 0, n3 = 0;
-            for (uint32_t j = t; j < tail; j += kThreads) {
-                const uint32_t k = order_key(mass_of(j));
-                n1 += k >= c1;
-                n2 += k >= c2;
-                n3 += k >= c3;
+            const uint32_t half = (shift >> 1) & 1;  // the other half is still read by who is a pass behind
+            if (own) {
+                // three counts of up to 512 a warp in one word, then two of up to 16384 in another
+                uint32_t n = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kOwn; ++i) {
+                    if (i * kThreads < tail) {
+                        n += keys[i] >= c1 ? 1u : 0u;
+                        n += keys[i] >= c2 ? 1u << 10 : 0u;
+                        n += keys[i] >= c3 ? 1u << 20 : 0u;
+                    }
+                }
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (lane == 0) counts[half][0][warp] = n;
+                __syncthreads();
+                n = counts[half][0][lane];
+                const uint32_t low = __reduce_add_sync(0xffffffffu, (n & 1023u) | ((n >> 10) & 1023u) << 16);
+                n1 = low & 0xffffu;
+                n2 = low >> 16;
+                n3 = __reduce_add_sync(0xffffffffu, n >> 20);
+            } else {
+                for (uint32_t j = t; j < tail; j += kThreads) {
+                    const uint32_t k = order_key(mass_of(j));
+                    n1 += k >= c1;
+                    n2 += k >= c2;
+                    n3 += k >= c3;
+                }
+                n1 = __reduce_add_sync(0xffffffffu, n1);
+                n2 = __reduce_add_sync(0xffffffffu, n2);
+                n3 = __reduce_add_sync(0xffffffffu, n3);
+                if (lane == 0) {
+                    counts[half][0][warp] = n1;
+                    counts[half][1][warp] = n2;
+                    counts[half][2][warp] = n3;
+                }
+                __syncthreads();
+                n1 = __reduce_add_sync(0xffffffffu, counts[half][0][lane]);
+                n2 = __reduce_add_sync(0xffffffffu, counts[half][1][lane]);
+                n3 = __reduce_add_sync(0xffffffffu, counts[half][2][lane]);
             }
-            n1 = __reduce_add_sync(0xffffffffu, n1);
-            n2 = __reduce_add_sync(0xffffffffu, n2);
-            n3 = __reduce_add_sync(0xffffffffu, n3);
-            uint32_t * sum = counts[(shift >> 1) & 1];
-            if (lane == 0) {
-                atomicAdd(sum + 1, n1);
-                atomicAdd(sum + 2, n2);
-                atomicAdd(sum + 3, n3);
-            }
-            if (t < 4) counts[((shift >> 1) & 1) ^ 1][t] = 0;  // read by all before the barrier of the pass before
-            __syncthreads();
-            n1 = sum[1], n2 = sum[2], n3 = sum[3];
             const uint32_t digit = n3 >= need ? 3u : n2 >= need ? 2u : n1 >= need ? 1u : 0u;
             if (digit < 3) above = digit == 2 ? n3 : digit == 1 ? n2 : n1;
+            if (digit > 0) reach = digit == 3 ? n3 : digit == 2 ? n2 : n1;
             threshold |= digit << shift;
-            __syncthreads();
+            if (reach == need) {  // those are the ones: nothing left to tell apart
+                --threshold;
+                above = need;
+                break;
+            }
         }
         // keep everything above the threshold and the first `ties` that equal it: a warp per run of slots
         const uint32_t ties = need - above;

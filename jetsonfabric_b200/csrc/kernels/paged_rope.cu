@@ -8,10 +8,12 @@
 // f32, each output rounded once.
 //
 // The kernel moves bytes: (q + k + v) in, the same out. A CTA takes 4 rows
-// (one when few rows would leave SMs idle), its threads 16 elements at a time
-// as 16-byte vectors: both partners of 8 pairs (half layout) or two 8-element
-// runs. Rows or rotations that are not made of 8-element runs take the
-// element-wise form of the same kernel.
+// (one when few rows would leave SMs idle), its threads 16-byte vectors: both
+// partners of 8 pairs (half layout) or a run of 8 elements. Sixteen small CTAs
+// an SM keep more loads in flight than several items per thread did (2, 4 and 8
+// of them: 63, 73 and 89 us against 55 for 16192 rows of 36 heads, bf16, 5.5
+// TB/s). Rows or rotations that are not made of 8-element runs take an
+// element-wise form.
 #include <cmath>
 
 #include "paged.cuh"
@@ -20,7 +22,7 @@ namespace jfb {
 namespace paged {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxPairs = 64;
 constexpr int kMaxRows = 4;
 constexpr uint64_t kNoSlot = ~0ull;
@@ -56,22 +58,31 @@ __device__ __forceinline__ __half to16<__half>(float x) { return __float2half_rn
 template <>
 __device__ __forceinline__ __nv_bfloat16 to16<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Eight elements as they lie in memory.
 template <typename S>
-__device__ __forceinline__ void load8(const S * p, float (&x)[8]) {
-    if constexpr (sizeof(S) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+    uint4 w[sizeof(S) / 2];
+    __device__ __forceinline__ void load(const S * p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = Num<S>::unpack(w[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
+        for (int i = 0; i < int(sizeof(S)) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < int(sizeof(S)) / 2; ++i) {
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(S) == 4) {
+                    x[4 * i + k] = __uint_as_float(u[k]);
+                } else {
+                    const float2 f = Num<S>::unpack(u[k]);
+                    x[2 * k] = f.x;
+                    x[2 * k + 1] = f.y;
+                }
+            }
         }
     }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void store8(T * p, const float (&x)[8]) {
@@ -79,54 +90,71 @@ __device__ __forceinline__ void store8(T * p, const float (&x)[8]) {
                                               Num<T>::pack(x[4], x[5]), Num<T>::pack(x[6], x[7]));
 }
 
-// One item of a head: the elements it covers, rotated or passed through.
-// Vector form, half layout: items [0, P/8) are the pairs 8c .. 8c + 7, items
-// behind them runs of 8 elements that pass through. Interleaved: runs of 8
-// elements. Element-wise form: pairs, then single elements.
-template <typename S, typename T, bool VEC, bool INTER>
-__device__ __forceinline__ void rotate_item(const S * src, T * dst, uint32_t c, uint32_t pairs, const float2 * cs) {
-    if constexpr (VEC && !INTER) {
-        if (c < pairs / 8) {
-            float a[8], b[8], y[8], z[8];
-            load8(src + c * 8, a);
-            load8(src + pairs + c * 8, b);
+// Item c of a head in vectors. Half layout: items [0, P/8) are the pairs 8c ..
+// 8c + 7, those behind them runs of 8 elements that pass through. Interleaved:
+// runs of 8 elements. `turned` is false for v.
+template <typename S, typename T, bool INTER>
+struct VectorItem {
+    T * dst;
+    const float2 * cs;
+    uint32_t pairs;  // distance of the partners; 0: one run
+    Raw8<S> a, b;
+    __device__ __forceinline__ void load(const S * src, T * to, uint32_t c, uint32_t half, bool turned, const float2 * turns) {
+        if constexpr (INTER) {
+            pairs = 0;
+            cs = turned && c < half / 4 ? turns + c * 4 : nullptr;
+            a.load(src + c * 8);
+            dst = to + c * 8;
+        } else {
+            const bool both = turned && c < half / 8;
+            const uint32_t at = both || !turned ? c * 8 : half + c * 8;
+            pairs = both ? half : 0u;
+            cs = turns + c * 8;
+            a.load(src + at);
+            if (both) b.load(src + half + c * 8);
+            dst = to + at;
+        }
+    }
+    __device__ __forceinline__ void store() const {
+        float x[8], y[8];
+        a.get(x);
+        if constexpr (INTER) {
+            if (cs != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 t = cs[i];
+                    const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                    x[2 * i] = x0 * t.x - x1 * t.y;
+                    x[2 * i + 1] = x0 * t.y + x1 * t.x;
+                }
+            }
+        } else if (pairs != 0) {
+            b.get(y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float2 t = cs[c * 8 + i];
-                y[i] = a[i] * t.x - b[i] * t.y;
-                z[i] = a[i] * t.y + b[i] * t.x;
+                const float2 t = cs[i];
+                const float x0 = x[i], x1 = y[i];
+                x[i] = x0 * t.x - x1 * t.y;
+                y[i] = x0 * t.y + x1 * t.x;
             }
-            store8(dst + c * 8, y);
-            store8(dst + pairs + c * 8, z);
-        } else {
-            float a[8];
-            const uint32_t at = 2 * pairs + (c - pairs / 8) * 8;
-            load8(src + at, a);
-            store8(dst + at, a);
+            store8(dst + pairs, y);
         }
-    } else if constexpr (VEC) {
-        float a[8], y[8];
-        load8(src + c * 8, a);
-        if (c < pairs / 4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 t = cs[c * 4 + i];
-                y[2 * i] = a[2 * i] * t.x - a[2 * i + 1] * t.y;
-                y[2 * i + 1] = a[2 * i] * t.y + a[2 * i + 1] * t.x;
-            }
-            store8(dst + c * 8, y);
-        } else {
-            store8(dst + c * 8, a);
-        }
+        store8(dst, x);
+    }
+};
+
+// The same in elements: pairs, then single elements that pass through.
+template <typename S, typename T, bool INTER>
+__device__ __forceinline__ void element_item(const S * src, T * dst, uint32_t c, uint32_t half, bool turned, const float2 * cs) {
+    if (!turned) {
+        dst[c] = to16<T>(load1(src + c));
+    } else if (c < half) {
+        const uint32_t i0 = INTER ? 2 * c : c, i1 = INTER ? 2 * c + 1 : c + half;
+        const float a = load1(src + i0), b = load1(src + i1);
+        dst[i0] = to16<T>(a * cs[c].x - b * cs[c].y);
+        dst[i1] = to16<T>(a * cs[c].y + b * cs[c].x);
     } else {
-        if (c < pairs) {
-            const uint32_t i0 = INTER ? 2 * c : c, i1 = INTER ? 2 * c + 1 : c + pairs;
-            const float a = load1(src + i0), b = load1(src + i1);
-            dst[i0] = to16<T>(a * cs[c].x - b * cs[c].y);
-            dst[i1] = to16<T>(a * cs[c].y + b * cs[c].x);
-        } else {
-            dst[c + pairs] = to16<T>(load1(src + c + pairs));
-        }
+        dst[c + half] = to16<T>(load1(src + c + half));
     }
 }
 
@@ -180,33 +208,52 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeParams 
     __syncthreads();
     const uint32_t per_head = VEC ? (INTER ? hd / 8 : hd / 8 - pairs / 8) : hd - pairs;
     const uint32_t v_head = VEC ? hd / 8 : hd;
-    const uint32_t n_q = p.heads * per_head, n_k = v.kv_heads * per_head, n_v = v.kv_heads * v_head;
-    for (uint32_t r = 0; r < rows; ++r) {
-        if (!live[r]) continue;
-        const uint64_t row = row0 + r, at = slot[r];
-        for (uint32_t i = threadIdx.x; i < n_q + n_k + n_v; i += kThreads) {
-            if (i < n_q) {
-                const uint32_t h = i / per_head, c = i - h * per_head;
-                rotate_item<S, T, VEC, INTER>(static_cast<const S *>(p.q) + row * p.q_stride + h * hd,
-                                              static_cast<T *>(p.q_out) + row * p.q_out_stride + h * hd, c, pairs, cs[r]);
-            } else if (at == kNoSlot) {
-                break;
-            } else if (i < n_q + n_k) {
-                const uint32_t h = (i - n_q) / per_head, c = (i - n_q) - h * per_head;
-                rotate_item<S, T, VEC, INTER>(static_cast<const S *>(p.k) + row * p.k_stride + h * hd,
-                                              static_cast<T *>(p.k_pool) + at + h * v.head_stride, c, pairs, cs[r]);
-            } else {
-                const uint32_t h = (i - n_q - n_k) / v_head, c = (i - n_q - n_k) - h * v_head;
-                const S * src = static_cast<const S *>(p.v) + row * p.v_stride + h * hd;
-                T * dst = static_cast<T *>(p.v_pool) + at + h * v.head_stride;
-                if constexpr (VEC) {
-                    float x[8];
-                    load8(src + c * 8, x);
-                    store8(dst + c * 8, x);
-                } else {
-                    dst[c] = to16<T>(load1(src + c));
-                }
-            }
+    const uint32_t n_q = p.heads * per_head, n_k = v.kv_heads * per_head, n_row = n_q + n_k + v.kv_heads * v_head;
+    // source, destination and place in its head of item i of the CTA's rows; no destination: nothing to do
+    struct Place {
+        const S * src;
+        T * dst;
+        uint32_t c, r;
+        bool turned;
+    };
+    const auto place = [&](uint32_t i) {
+        Place o;
+        o.r = i / n_row;
+        i -= o.r * n_row;
+        const uint64_t row = row0 + o.r, at = slot[o.r];
+        o.turned = i < n_q + n_k;
+        if (i < n_q) {
+            const uint32_t h = i / per_head;
+            o.c = i - h * per_head;
+            o.src = static_cast<const S *>(p.q) + row * p.q_stride + h * hd;
+            o.dst = static_cast<T *>(p.q_out) + row * p.q_out_stride + h * hd;
+        } else if (o.turned) {
+            const uint32_t h = (i - n_q) / per_head;
+            o.c = (i - n_q) - h * per_head;
+            o.src = static_cast<const S *>(p.k) + row * p.k_stride + h * hd;
+            o.dst = at == kNoSlot ? nullptr : static_cast<T *>(p.k_pool) + at + h * v.head_stride;
+        } else {
+            const uint32_t h = (i - n_q - n_k) / v_head;
+            o.c = (i - n_q - n_k) - h * v_head;
+            o.src = static_cast<const S *>(p.v) + row * p.v_stride + h * hd;
+            o.dst = at == kNoSlot ? nullptr : static_cast<T *>(p.v_pool) + at + h * v.head_stride;
+        }
+        if (!live[o.r]) o.dst = nullptr;
+        return o;
+    };
+    const uint32_t total = rows * n_row;
+    if constexpr (VEC) {
+        for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
+            const Place o = place(i);
+            if (o.dst == nullptr) continue;
+            VectorItem<S, T, INTER> item;
+            item.load(o.src, o.dst, o.c, pairs, o.turned, cs[o.r]);
+            item.store();
+        }
+    } else {
+        for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
+            const Place o = place(i);
+            if (o.dst != nullptr) element_item<S, T, INTER>(o.src, o.dst, o.c, pairs, o.turned, cs[o.r]);
         }
     }
 }
@@ -332,7 +379,7 @@ extern "C" jfb_status jfb_rope_paged_append(const void * q, const void * k, cons
     p.heads = heads;
     p.rope_dims = dims;
     p.factor = rope->factor;
-    // fewer than about eight CTAs per SM with 4 rows each: one row per CTA
+    // few rows: one per CTA, to fill the SMs; many: four share the work of finding their sequences and angles (110 us with one)
     p.rows_per_cta = rows >= 8u * 148u * kMaxRows ? kMaxRows : 1;
     const bool inter = rope->interleaved != 0;
     // 16-byte vectors: runs of 8 elements on both sides of every pair, aligned rows
