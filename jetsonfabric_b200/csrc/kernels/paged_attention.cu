@@ -21,30 +21,44 @@ namespace {
 // flops) and the products run on mma.sync m16n8k16, whose 16 rows waste the
 // least of them. Two producer warps bring K and V tiles of 128 keys page by
 // page through TMA into a ring of 3 (D = 128: 192 KB, 128 KB or more in flight
-// per SM); of the 8 consumer warps each takes 16 keys of every tile with its
-// own running maximum and sums, so warps meet only at the end of an item's
-// segment, in shared memory.
+// per SM). Each of the 8 consumer warps forms the scores of 16 keys of a tile;
+// the probabilities meet in shared memory, and each warp forms all keys' sums
+// of its D / 8 output columns. The warps share one running maximum, so the end
+// of an item costs one exchange of the softmax sums. (Warps that kept their own
+// maximum and sums over their own keys had 64 KB to add up at every end: 2
+// more us each, of which a batch of short sequences has several per CTA.)
 
 constexpr int kRowsM = 16;
 constexpr int kItemRows = 0;  // units of an item's start and end
 constexpr int kConsumers = 8;
 constexpr int kThreadsRows = (kConsumers + 2) * 32;
+constexpr float kSlack = 8.0f;  // growth of the maximum (log 2) before the sums are rescaled
 
 template <int D>
 struct RowsSmem {
     static constexpr int kStages = D == 128 ? 3 : 6;
     static constexpr uint32_t kStage = 2 * kTileBytes<D>;
-    static constexpr uint32_t kMerge = kStages * kStage;                       // [8 warps][16 rows][64] f32
-    static constexpr uint32_t kMl = kMerge + kConsumers * kRowsM * 64 * 4;     // [8][16] (m, l)
-    static constexpr uint32_t kBars = kMl + kConsumers * kRowsM * 8;           // full K, full V, empty
+    static constexpr uint32_t kP = kStages * kStage;                            // [2][16 rows][128 keys] probabilities
+    static constexpr uint32_t kTops = kP + 2 * kRowsM * kTileKeys * 2;          // [8 warps][16]
+    static constexpr uint32_t kSums = kTops + kConsumers * kRowsM * 4;          // [8 warps][16]
+    static constexpr uint32_t kBars = kSums + kConsumers * kRowsM * 4;          // full K, full V, empty
     static constexpr uint32_t kWalk = kBars + 3 * kStages * 8;
-    static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(Walk);  // abort, last
-    static constexpr uint32_t kBytes = kFlags + 16 + 1024;                     // + alignment
+    static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(Walk);  // abort, join
+    static constexpr uint32_t kBytes = kFlags + 16 + 1024;                        // + alignment
 };
 static_assert(RowsSmem<128>::kBytes <= 232448 && RowsSmem<64>::kBytes <= 232448);
-static_assert(RowsSmem<64>::kMerge >= JFB_PAGED_MAX_SEQUENCES * 8);
+static_assert(RowsSmem<64>::kP >= JFB_PAGED_MAX_SEQUENCES * 8);
 
 __device__ __forceinline__ void bar_consumers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The same, and whether any of the threads brings true.
+__device__ __forceinline__ bool bar_consumers_or(bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any)
+                 : "r"(uint32_t(mine))
+                 : "memory");
+    return any != 0;
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -121,31 +135,34 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     }
 
     // consumers
+    constexpr int kCols = D / 8;      // output columns of a warp
+    constexpr int kTilesN = kCols / 8;
     const uint32_t grp = lane >> 2, tig = lane & 3;
     const uint32_t G = v.group, hd = v.head_dim;
     const float scale2 = p.scale * kLog2e;
-    float * merge = reinterpret_cast<float *>(smem + L::kMerge);
-    float2 * ml = reinterpret_cast<float2 *>(smem + L::kMl);
+    float * tops = reinterpret_cast<float *>(smem + L::kTops);
+    float * sums = reinterpret_cast<float *>(smem + L::kSums);
+    const uint32_t p_base = smem_u32(smem) + L::kP;
     uint32_t n = 0;
     do {
         uint32_t t0, t1;
         walk_segment<kItemRows>(w, t0, t1);
-        const uint32_t packed = w.s.count * G;  // rows of an item: below 2^32 (checked on the host)
+        const uint32_t packed = w.s.count * G;  // rows of an item: below 2^31 (checked on the host)
         const uint32_t row0 = w.tile * kRowsM;
-        const int64_t first = int64_t(w.s.kv) - w.s.count;
+        const int32_t first = int32_t(w.s.kv) - int32_t(w.s.count);
         // Q fragments of rows grp and grp + 8
         uint32_t qa[D / 16][4];
         int32_t pos[2];
-        uint32_t token_row[2], head[2];
+        uint32_t out_row[2], out_head[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const uint32_t r = row0 + grp + 8 * e;
             const bool valid = r < packed;
             const uint32_t i = valid ? r / G : 0u, g = valid ? r % G : 0u;
-            token_row[e] = w.s.q0 + i;
-            head[e] = w.kv_head * G + g;
-            pos[e] = int32_t(first + i);
-            const T * src = static_cast<const T *>(p.q) + uint64_t(token_row[e]) * p.q_stride + uint64_t(head[e]) * hd;
+            out_row[e] = w.s.q0 + i;
+            out_head[e] = w.kv_head * G + g;
+            pos[e] = first + int32_t(i);
+            const T * src = static_cast<const T *>(p.q) + uint64_t(out_row[e]) * p.q_stride + uint64_t(out_head[e]) * hd;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
@@ -155,11 +172,11 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 }
             }
         }
-        const int32_t pos_first = int32_t(first + row0 / G);
-        const int32_t pos_last = int32_t(first + (min(row0 + uint32_t(kRowsM), packed) - 1) / G);
-        float o[D / 8][4];
+        const int32_t pos_first = first + int32_t(row0 / G);
+        const int32_t pos_last = first + int32_t((min(row0 + uint32_t(kRowsM), packed) - 1) / G);
+        float o[kTilesN][4];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
+        for (int j = 0; j < kTilesN; ++j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
         }
@@ -167,185 +184,221 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
         for (uint32_t t = t0; t < t1; ++t, ++n) {
             const uint32_t st = n % L::kStages, parity = (n / L::kStages) & 1;
             const uint32_t kbase = smem_u32(smem) + st * L::kStage, vbase = kbase + kTileBytes<D>;
+            const uint32_t pbase = p_base + (n & 1) * (kRowsM * kTileKeys * 2);
             const int32_t key = int32_t(w.k.begin + t * kTileKeys + warp * 16);  // this warp's first key
-            // after a wait that gave up the tiles are skipped, but every warp
-            // still meets the others at the segments' barriers
-            if (__any_sync(0xffffffffu, flags[0]) || !__all_sync(0xffffffffu, mbar_wait(full_k + st, parity, flags, v.error))) continue;
+            // after a wait that gave up no work is done, but every warp still meets the others at the barriers
+            bool live = !__any_sync(0xffffffffu, flags[0]) && __all_sync(0xffffffffu, mbar_wait(full_k + st, parity, flags, v.error));
             float s[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
-            }
-            const uint32_t krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                uint32_t b[4];
-                const uint32_t chunk = kk * 2 + ((lane >> 3) & 1);
-                ldsm4(b, kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4));
-                mma_16816<T>(s[0], qa[kk], b[0], b[1]);
-                mma_16816<T>(s[1], qa[kk], b[2], b[3]);
-            }
-            if (key + 15 > pos_first || (v.window > 0 && key <= pos_last - int32_t(v.window))) {
+            float mx[2] = {-INFINITY, -INFINITY};
+            if (live) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int32_t k = key + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
-                        if (k > q || (v.window > 0 && k <= q - int32_t(v.window))) s[j][e] = -INFINITY;
+                    for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+                }
+                const uint32_t krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    uint32_t b[4];
+                    const uint32_t chunk = kk * 2 + ((lane >> 3) & 1);
+                    ldsm4(b, kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4));
+                    mma_16816<T>(s[0], qa[kk], b[0], b[1]);
+                    mma_16816<T>(s[1], qa[kk], b[2], b[3]);
+                }
+                if (key + 15 > pos_first || (v.window > 0 && key <= pos_last - int32_t(v.window))) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int32_t k = key + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
+                            if (k > q || (v.window > 0 && k <= q - int32_t(v.window))) s[j][e] = -INFINITY;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    mx[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * scale2;
+                }
+            }
+            // The sums refer to a maximum that all warps share; it moves only
+            // when some row's has grown by more than 2^8.
+            if (bar_consumers_or(mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (tig == 0) tops[warp * kRowsM + grp + 8 * e] = mx[e];
+                }
+                bar_consumers();
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < kConsumers; ++x) top = fmaxf(top, tops[x * kRowsM + grp + 8 * e]);
+                    if (top > m[e] + kSlack) {
+                        const float f = exp2_approx(m[e] - top);
+                        m[e] = top;
+                        l[e] *= f;
+#pragma unroll
+                        for (int j = 0; j < kTilesN; ++j) {
+                            o[j][2 * e] *= f;
+                            o[j][2 * e + 1] *= f;
+                        }
                     }
                 }
             }
-            float alpha[2];
-            uint32_t pa[4];
+            bool clean = false;
+            if (live) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float mx = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                mx = fmaxf(m[e], mx * scale2);
-                const float base = mx == -INFINITY ? 0.0f : mx;  // nothing seen yet: every term is 0
-                alpha[e] = exp2_approx(m[e] - base);
-                m[e] = mx;
-                float q[4];
+                for (int e = 0; e < 2; ++e) {
+                    const float base = m[e] == -INFINITY ? 0.0f : m[e];  // nothing seen yet: every term is 0
+                    float q[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) q[c] = exp2_approx(fmaf(s[c >> 1][2 * e + (c & 1)], scale2, -base));
-                l[e] = l[e] * alpha[e] + ((q[0] + q[1]) + (q[2] + q[3]));
-                pa[e] = Num<T>::pack(q[0], q[1]);
-                pa[e + 2] = Num<T>::pack(q[2], q[3]);
-            }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    o[j][0] *= alpha[0];
-                    o[j][1] *= alpha[0];
-                    o[j][2] *= alpha[1];
-                    o[j][3] *= alpha[1];
+                    for (int c = 0; c < 4; ++c) q[c] = exp2_approx(fmaf(s[c >> 1][2 * e + (c & 1)], scale2, -base));
+                    l[e] += (q[0] + q[1]) + (q[2] + q[3]);
+                    // 16-byte chunks 2 warp and 2 warp + 1 of the row's 128 keys, chunk c at c ^ (row % 8)
+                    const uint32_t row = grp + 8 * e, at = pbase + row * (kTileKeys * 2) + tig * 4;
+                    const uint32_t c0 = (2 * warp) ^ (row & 7), c1 = (2 * warp + 1) ^ (row & 7);
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c0 * 16), "r"(Num<T>::pack(q[0], q[1])) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c1 * 16), "r"(Num<T>::pack(q[2], q[3])) : "memory");
                 }
-            }
-            if (!__all_sync(0xffffffffu, mbar_wait(full_v + st, parity, flags, v.error))) continue;
-            // what no row sees may hold anything: its probability is 0, but 0 x NaN is not
-            const bool clean = key < int32_t(w.k.lo) || key + 16 > int32_t(w.k.hi);
-            if (clean) {
-                for (int r = 0; r < 16; ++r) {
-                    if (key + r >= int32_t(w.k.lo) && key + r < int32_t(w.k.hi)) continue;
-                    for (uint32_t c = lane; c < D / 8; c += 32) {
-                        const uint32_t at = vbase + (c >> 3) * (kTileKeys * 128) + (warp * 16 + r) * 128 + ((c & 7) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                live = __all_sync(0xffffffffu, mbar_wait(full_v + st, parity, flags, v.error));
+                // what no row sees may hold anything: its probability is 0, but 0 x NaN is not
+                clean = live && (key < int32_t(w.k.lo) || key + 16 > int32_t(w.k.hi));
+                if (clean) {
+                    for (int r = 0; r < 16; ++r) {
+                        if (key + r >= int32_t(w.k.lo) && key + r < int32_t(w.k.hi)) continue;
+                        for (uint32_t c = lane; c < D / 8; c += 32) {
+                            const uint32_t at = vbase + (c >> 3) * (kTileKeys * 128) + (warp * 16 + r) * 128 + ((c & 7) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                        }
                     }
+                    fence_proxy_async();  // before the copy that reuses the stage
                 }
-                __syncwarp();
             }
-            const uint32_t vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+            bar_consumers();
+            if (!live) continue;
 #pragma unroll
-            for (int j = 0; j < D / 8; j += 2) {
-                uint32_t b[4];
-                const uint32_t chunk = j + (lane >> 4);
+            for (int kk = 0; kk < kTileKeys / 16; ++kk) {
+                uint32_t a[4], b[4];
+                const uint32_t arow = lane & 15;
+                ldsm4(a, pbase + arow * (kTileKeys * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4));
+                const uint32_t vrow = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+                const uint32_t chunk = warp * kTilesN + (kTilesN == 2 ? lane >> 4 : 0u);
                 ldsm4_trans(b, vbase + (chunk >> 3) * (kTileKeys * 128) + vrow * 128 + (((chunk & 7) ^ (vrow & 7)) << 4));
-                mma_16816<T>(o[j], pa, b[0], b[1]);
-                mma_16816<T>(o[j + 1], pa, b[2], b[3]);
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j) mma_16816<T>(o[j], a, b[2 * j], b[2 * j + 1]);
             }
-            if (clean) fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + st);
         }
 
-        // the warps' parts of the segment
+        // the softmax sums of all keys
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-            if (tig == 0) ml[warp * kRowsM + grp + 8 * e] = make_float2(m[e], l[e]);
+            if (tig == 0) sums[warp * kRowsM + grp + 8 * e] = l[e];
         }
         bar_consumers();
-        float part[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float top = -INFINITY;
+            l[e] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < kConsumers; ++x) top = fmaxf(top, ml[x * kRowsM + grp + 8 * e].x);
-            part[e] = m[e] == -INFINITY ? 0.0f : exp2_approx(m[e] - top);
+            for (int x = 0; x < kConsumers; ++x) l[e] += sums[x * kRowsM + grp + 8 * e];
         }
-        const uint32_t orow = threadIdx.x >> 4, oc = (threadIdx.x & 15) * 4;  // output row and columns of this thread
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int x = 0; x < kConsumers; ++x) top = fmaxf(top, ml[x * kRowsM + orow].x);
-#pragma unroll
-        for (int x = 0; x < kConsumers; ++x) {
-            const float2 a = ml[x * kRowsM + orow];
-            sum += a.x == -INFINITY ? 0.0f : a.y * exp2_approx(a.x - top);
-        }
-        const uint32_t r = row0 + orow;
-        const RowsOut<T> out(p, r < packed, w.s.q0 + r / G, w.kv_head * G + r % G);
-        const bool whole = t0 == 0 && t1 == w.k.tiles;
-        float * slot = p.partial + uint64_t(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * kSlotFloats;
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t c = j * 8 + tig * 2;
-                float * a = merge + (warp * kRowsM + grp) * 64 + (c ^ ((grp & 3) << 3));
-                *reinterpret_cast<float2 *>(a) = make_float2(o[h * 8 + j][0] * part[0], o[h * 8 + j][1] * part[0]);
-                *reinterpret_cast<float2 *>(a + 8 * 64) = make_float2(o[h * 8 + j][2] * part[1], o[h * 8 + j][3] * part[1]);
-            }
-            bar_consumers();
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int x = 0; x < kConsumers; ++x) {
-                const float4 a = *reinterpret_cast<const float4 *>(merge + (x * kRowsM + orow) * 64 + (oc ^ ((orow & 3) << 3)));
-                acc.x += a.x;
-                acc.y += a.y;
-                acc.z += a.z;
-                acc.w += a.w;
-            }
-            if (whole) out.store4(h * 64 + oc, acc, sum, hd);
-            else __stcg(reinterpret_cast<float4 *>(slot + orow * D + h * 64 + oc), acc);
-            bar_consumers();
-        }
-        if (whole) {
-            if ((threadIdx.x & 15) == 0) out.store_lse(p, top, sum);
-        } else {
-            if ((threadIdx.x & 15) == 0) __stcg(reinterpret_cast<float2 *>(slot + kRowsM * D + 2 * orow), make_float2(top, sum));
-            // the last CTA of the item to arrive joins the parts, in CTA order
+        bool write = t0 == 0 && t1 == w.k.tiles;
+        if (!write) {
+            // One part of an item that spans CTAs: the last of them to get here
+            // joins all, in CTA order. Mostly that is the CTA that began the item,
+            // at its end, and finds the others' parts already there.
             uint32_t c0, c1;
             walk_owners<kItemRows>(w, c0, c1);
-            __threadfence();
-            bar_consumers();
+            const uint32_t others = c1 - c0;
             if (threadIdx.x == 0) {
-                const bool last = atomicAdd(p.counters + c0, 1u) == c1 - c0;
-                if (last) p.counters[c0] = 0;
-                flags[1] = last;
+                uint32_t there;
+                asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.counters + c0) : "memory");
+                flags[1] = there == others;
             }
             bar_consumers();
-            if (flags[1]) {
-                __threadfence();
-                auto part_of = [&](uint32_t c) { return p.partial + uint64_t(2 * c + (c == c0 ? 1 : 0)) * kSlotFloats; };
-                float jtop = -INFINITY;
-                for (uint32_t c = c0; c <= c1; ++c) jtop = fmaxf(jtop, __ldcg(part_of(c) + kRowsM * D + 2 * orow));
-                float jsum = 0.0f;
-                float4 acc[D / 64];
+            write = flags[1] != 0;
+            auto part_of = [&](uint32_t c) { return p.partial + uint64_t(2 * c + (c == c0 ? 1 : 0)) * kSlotFloats; };
+            if (!write) {
+                float * to = part_of(blockIdx.x);
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) acc[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t row = grp + 8 * e;
+#pragma unroll
+                    for (int j = 0; j < kTilesN; ++j) {
+                        __stcg(reinterpret_cast<float2 *>(to + row * D + warp * kCols + j * 8 + tig * 2), make_float2(o[j][2 * e], o[j][2 * e + 1]));
+                    }
+                    if (warp == 0 && tig == 0) __stcg(reinterpret_cast<float2 *>(to + kRowsM * D + 2 * row), make_float2(m[e], l[e]));
+                }
+                bar_consumers();
+                if (threadIdx.x == 0) {
+                    __threadfence();
+                    flags[1] = atomicAdd(p.counters + c0, 1u) == others;
+                    __threadfence();
+                }
+                bar_consumers();
+                write = flags[1] != 0;
+            }
+            if (write) {
+                if (threadIdx.x == 0) p.counters[c0] = 0;  // nobody else is left to arrive
+                float jm[2] = {-INFINITY, -INFINITY}, jl[2] = {0.0f, 0.0f}, jo[kTilesN][4];
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) jo[j][e] = 0.0f;
+                }
                 for (uint32_t c = c0; c <= c1; ++c) {
                     const float * from = part_of(c);
-                    const float2 a = __ldcg(reinterpret_cast<const float2 *>(from + kRowsM * D + 2 * orow));
-                    const float f = a.x == -INFINITY ? 0.0f : exp2_approx(a.x - jtop);
-                    jsum = fmaf(a.y, f, jsum);
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + orow * D + h * 64 + oc));
-                        acc[h].x = fmaf(x.x, f, acc[h].x);
-                        acc[h].y = fmaf(x.y, f, acc[h].y);
-                        acc[h].z = fmaf(x.z, f, acc[h].z);
-                        acc[h].w = fmaf(x.w, f, acc[h].w);
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t row = grp + 8 * e;
+                        float2 ml = make_float2(m[e], l[e]), x[kTilesN];
+#pragma unroll
+                        for (int j = 0; j < kTilesN; ++j) x[j] = make_float2(o[j][2 * e], o[j][2 * e + 1]);
+                        if (c != blockIdx.x) {
+                            ml = __ldcg(reinterpret_cast<const float2 *>(from + kRowsM * D + 2 * row));
+#pragma unroll
+                            for (int j = 0; j < kTilesN; ++j) {
+                                x[j] = __ldcg(reinterpret_cast<const float2 *>(from + row * D + warp * kCols + j * 8 + tig * 2));
+                            }
+                        }
+                        const float top = fmaxf(jm[e], ml.x);
+                        const float f = jm[e] == -INFINITY ? 0.0f : exp2_approx(jm[e] - top);
+                        const float g = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - top);
+                        jm[e] = top;
+                        jl[e] = jl[e] * f + ml.y * g;
+#pragma unroll
+                        for (int j = 0; j < kTilesN; ++j) {
+                            jo[j][2 * e] = jo[j][2 * e] * f + x[j].x * g;
+                            jo[j][2 * e + 1] = jo[j][2 * e + 1] * f + x[j].y * g;
+                        }
                     }
                 }
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) out.store4(h * 64 + oc, acc[h], jsum, hd);
-                if ((threadIdx.x & 15) == 0) out.store_lse(p, jtop, jsum);
+                for (int e = 0; e < 2; ++e) {
+                    m[e] = jm[e];
+                    l[e] = jl[e];
+                }
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] = jo[j][e];
+                }
             }
-            bar_consumers();
+            bar_consumers();  // flags may be written again
+        }
+        if (write) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const RowsOut<T> out(p, row0 + grp + 8 * e < packed, out_row[e], out_head[e]);
+#pragma unroll
+                for (int j = 0; j < kTilesN; ++j) out.store2(warp * kCols + j * 8 + tig * 2, o[j][2 * e], o[j][2 * e + 1], l[e], hd);
+                if (warp == 0 && tig == 0) out.store_lse(p, m[e], l[e]);
+            }
         }
     } while (walk_warp_next<kItemRows>(v, &w));
 }

@@ -35,11 +35,11 @@ struct RowsOut {
         out = valid ? static_cast<T *>(p.out) + uint64_t(row) * p.out_stride + uint64_t(head) * p.view.head_dim : nullptr;
         at = uint64_t(row) * p.heads + head;
     }
-    // four columns of sums over the softmax sum; a row that saw nothing is zero
-    __device__ __forceinline__ void store4(uint32_t d, float4 a, float sum, uint32_t head_dim) const {
+    // two columns of sums over the softmax sum; a row that saw nothing is zero
+    __device__ __forceinline__ void store2(uint32_t d, float a, float b, float sum, uint32_t head_dim) const {
         if (out == nullptr || d >= head_dim) return;
         const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
-        *reinterpret_cast<uint2 *>(out + d) = make_uint2(Num<T>::pack(a.x * f, a.y * f), Num<T>::pack(a.z * f, a.w * f));
+        *reinterpret_cast<uint32_t *>(out + d) = Num<T>::pack(a * f, b * f);
     }
     // sixteen columns, as one 32-byte sector where rows are aligned to it
     __device__ __forceinline__ void store16(uint32_t d, const float * a, float sum, uint32_t head_dim, bool sectors) const {
