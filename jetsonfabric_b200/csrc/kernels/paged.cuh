@@ -384,8 +384,14 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
         __syncthreads();
         for (uint32_t b = lane; b < v.sequences; b += 32) per_head += cost[b];
     }
+    // sums of 32 bits where they fit: wide ones take several times the shuffles
+    const bool narrow = __all_sync(0xffffffffu, per_head < (1u << 26));
+    if (narrow) {
+        per_head = __reduce_add_sync(0xffffffffu, uint32_t(per_head));
+    } else {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
+        for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
+    }
     WalkOf<Items> x = {};
     x.total = uint64_t(per_head) * v.kv_heads;
     x.ctas = uint64_t(workers) < x.total ? workers : uint32_t(x.total);
@@ -397,10 +403,20 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
         unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;
         const auto find32 = [&](unsigned long long mine, int & src) {
             unsigned long long upto = mine;
+            if (narrow) {
+                uint32_t sum = uint32_t(mine);
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
-                if (int(lane) >= d) upto += o;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t o = __shfl_up_sync(0xffffffffu, sum, d);
+                    if (int(lane) >= d) sum += o;
+                }
+                upto = sum;
+            } else {
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (int(lane) >= d) upto += o;
+                }
             }
             const uint32_t over = __ballot_sync(0xffffffffu, upto > left);
             src = __ffs(over) - 1;

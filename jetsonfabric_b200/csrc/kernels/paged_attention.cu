@@ -26,12 +26,15 @@ namespace {
 // of its D / 8 output columns. The warps share one running maximum, so the end
 // of an item costs one exchange of the softmax sums. (Warps that kept their own
 // maximum and sums over their own keys had 64 KB to add up at every end: 2
-// more us each, of which a batch of short sequences has several per CTA.)
+// more us each, of which a batch of short sequences has several per CTA.) The
+// scores of the next tile are formed beside the second product of this one.
+// A part of an item that began in another CTA is published by a warp of its
+// own, so that the consumers go on to their next item at once.
 
 constexpr int kRowsM = 16;
 constexpr int kItemRows = 0;  // units of an item's start and end
 constexpr int kConsumers = 8;
-constexpr int kThreadsRows = (kConsumers + 2) * 32;
+constexpr int kThreadsRows = (kConsumers + 3) * 32;  // and K's and V's producers, the publisher
 constexpr float kSlack = 8.0f;  // growth of the maximum (log 2) before the sums are rescaled
 
 template <int D>
@@ -43,7 +46,7 @@ struct RowsSmem {
     static constexpr uint32_t kSums = kTops + kConsumers * kRowsM * 4;          // [8 warps][16]
     static constexpr uint32_t kBars = kSums + kConsumers * kRowsM * 4;          // full K, full V, empty
     static constexpr uint32_t kWalk = kBars + 3 * kStages * 8;
-    static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(Walk);  // abort, join
+    static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(Walk);  // abort, joined at once
     static constexpr uint32_t kBytes = kFlags + 16 + 1024;                        // + alignment
 };
 static_assert(RowsSmem<128>::kBytes <= 232448 && RowsSmem<64>::kBytes <= 232448);
@@ -71,6 +74,93 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr)
                  : "memory");
+}
+
+// Consumers hand the part of an item that began elsewhere to the publisher,
+// and learn at the CTA's end whether it was the item's last.
+__device__ __forceinline__ void part_arrive() { asm volatile("bar.arrive 2, 288;" ::: "memory"); }
+__device__ __forceinline__ void part_wait() { asm volatile("bar.sync 2, 288;" ::: "memory"); }
+__device__ __forceinline__ void verdict_arrive() { asm volatile("bar.arrive 3, 288;" ::: "memory"); }
+__device__ __forceinline__ void verdict_wait() { asm volatile("bar.sync 3, 288;" ::: "memory"); }
+
+// Counts a part in; true when all the item's parts are.
+__device__ __forceinline__ bool count_part(uint32_t * counter, uint32_t others) {
+    __threadfence();
+    const bool last = atomicAdd(counter, 1u) == others;
+    __threadfence();
+    if (last) *counter = 0;
+    return last;
+}
+
+// Where CTA c keeps its part of the item that begins in CTA c0: [16][D] sums, then [16] (maximum, sum).
+__device__ __forceinline__ float * part_of(const AttentionParams & p, uint32_t c, uint32_t c0) {
+    return p.partial + uint64_t(2 * c + (c == c0 ? 1 : 0)) * kSlotFloats;
+}
+
+// Adds a part (maximum, sum and N columns) to another. The operations are
+// spelled out, so that every place that joins gets the same bits.
+template <int N>
+__device__ __forceinline__ void join_part(float & m, float & l, float (&o)[N], float pm, float pl, const float (&po)[N]) {
+    const float top = fmaxf(m, pm);
+    const float f = m == -INFINITY ? 0.0f : exp2_approx(m - top), g = pm == -INFINITY ? 0.0f : exp2_approx(pm - top);
+    m = top;
+    l = fmaf(pl, g, __fmul_rn(l, f));
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = fmaf(po[i], g, __fmul_rn(o[i], f));
+}
+
+// The consumers join all parts of the walk's item: 16 threads per row and
+// slice of the parts, the slices merged in order. Where rows are few their
+// parts are many (a long context of one sequence), and more slices keep more
+// loads in flight. Two parts are joined in plain CTA order whatever the slices.
+template <typename T, int D>
+__device__ __forceinline__ void join_item(const AttentionParams & p, const Walk & w, float * scratch) {
+    constexpr int kN = D / 16;  // columns per thread
+    uint32_t c0, c1;
+    walk_owners<kItemRows>(w, c0, c1);
+    const uint32_t row0 = w.tile * kRowsM, rows = min(uint32_t(kRowsM), w.s.count * p.view.group - row0);
+    const uint32_t slices = kRowsM / rows, unit = threadIdx.x >> 4, slice = unit / rows, row = unit - slice * rows;
+    const uint32_t col = (threadIdx.x & 15) * kN;
+    float m = -INFINITY, l = 0.0f, o[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) o[i] = 0.0f;
+    if (slice < slices) {
+#pragma unroll 8
+        for (uint32_t c = c0 + slice; c <= c1; c += slices) {
+            const float * from = part_of(p, c, c0);
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + kRowsM * D + 2 * row));
+            float x[kN];
+#pragma unroll
+            for (int i = 0; i < kN; i += 4) {
+                const float4 y = __ldcg(reinterpret_cast<const float4 *>(from + row * D + col + i));
+                x[i] = y.x, x[i + 1] = y.y, x[i + 2] = y.z, x[i + 3] = y.w;
+            }
+            join_part(m, l, o, ml.x, ml.y, x);
+        }
+    }
+    float * mine = scratch + threadIdx.x * (kN + 2);
+    if (slice > 0) {
+        mine[0] = m;
+        mine[1] = l;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) mine[2 + i] = o[i];
+    }
+    bar_consumers();
+    if (slice == 0) {
+        for (uint32_t s = 1; s < slices; ++s) {
+            const float * other = mine + s * rows * 16 * (kN + 2);
+            float x[kN];
+#pragma unroll
+            for (int i = 0; i < kN; ++i) x[i] = other[2 + i];
+            join_part(m, l, o, other[0], other[1], x);
+        }
+        const uint32_t r = row0 + row;
+        const RowsOut<T> out(p, true, w.s.q0 + r / p.view.group, w.kv_head * p.view.group + r % p.view.group);
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) out.store2(col + i, o[i], o[i + 1], l, p.view.head_dim);
+        if (col == 0) out.store_lse(p, m, l);
+    }
+    bar_consumers();  // scratch may be written again
 }
 
 template <typename T, int D>
@@ -101,6 +191,20 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     if (!walk_begin<kItemRows>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
     Walk & w = walks[warp];
 
+    uint32_t s0, s1;
+    walk_segment<kItemRows>(w, s0, s1);
+    // the CTA's first segment is a part of an item that began elsewhere, and others follow it
+    const bool handed = s0 > 0 && w.item0 + w.k.tiles + 2 * kItemRows < w.end;
+    if (warp == kConsumers + 2) {
+        if (!handed) return;
+        uint32_t c0, c1;
+        walk_owners<kItemRows>(w, c0, c1);
+        part_wait();
+        if (lane == 0) flags[2] = count_part(p.counters + c0, c1 - c0);
+        __syncwarp();
+        verdict_arrive();
+        return;
+    }
     if (warp >= kConsumers) {
         const bool is_v = warp > kConsumers;
         const CUtensorMap * map = is_v ? &map_v : &map_k;
@@ -112,6 +216,16 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             walk_segment<kItemRows>(w, t0, t1);
             const int32_t * row = v.table + uint64_t(w.b) * v.table_stride;
             const uint32_t begin = w.k.begin, hi = w.k.hi, head = w.kv_head;
+            if (!is_v) {
+                // the item's queries on their way to L1 before the consumers get to it: half a row per lane
+                const uint32_t r = w.tile * kRowsM + lane / 2;
+                if (r < w.s.count * v.group && (lane & 1) * 64 < v.head_dim) {
+                    const T * src = static_cast<const T *>(p.q) + uint64_t(w.s.q0 + r / v.group) * p.q_stride +
+                                    uint64_t(head * v.group + r % v.group) * v.head_dim + (lane & 1) * 64;
+                    uint32_t unused;
+                    asm volatile("ld.global.b32 %0, [%1];" : "=r"(unused) : "l"(src));
+                }
+            }
             auto pages_of = [&](uint32_t t) {
                 const uint32_t key0 = begin + t * kTileKeys;
                 return tile_pages(v, row, key0, hi <= key0 ? key0 : min(hi, key0 + uint32_t(kTileKeys)));
@@ -181,46 +295,53 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
         }
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-        for (uint32_t t = t0; t < t1; ++t, ++n) {
-            const uint32_t st = n % L::kStages, parity = (n / L::kStages) & 1;
-            const uint32_t kbase = smem_u32(smem) + st * L::kStage, vbase = kbase + kTileBytes<D>;
-            const uint32_t pbase = p_base + (n & 1) * (kRowsM * kTileKeys * 2);
-            const int32_t key = int32_t(w.k.begin + t * kTileKeys + warp * 16);  // this warp's first key
-            // after a wait that gave up no work is done, but every warp still meets the others at the barriers
-            bool live = !__any_sync(0xffffffffu, flags[0]) && __all_sync(0xffffffffu, mbar_wait(full_k + st, parity, flags, v.error));
-            float s[2][4];
-            float mx[2] = {-INFINITY, -INFINITY};
-            if (live) {
+        const int32_t begin = int32_t(w.k.begin + warp * 16), lo = int32_t(w.k.lo), hi = int32_t(w.k.hi);
+        // scores of this warp's 16 keys of tile t, the a-th of the CTA; after a wait that gave up
+        // no work is done, but every warp still meets the others at the barriers
+        float s[2][4];
+        bool live;
+        const auto scores = [&](uint32_t a, uint32_t t) {
+            live = !__any_sync(0xffffffffu, flags[0]) &&
+                   __all_sync(0xffffffffu, mbar_wait(full_k + a % L::kStages, (a / L::kStages) & 1, flags, v.error));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+            }
+            if (!live) return;
+            const uint32_t kbase = smem_u32(smem) + (a % L::kStages) * L::kStage;
+            const uint32_t krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                uint32_t b[4];
+                const uint32_t chunk = kk * 2 + ((lane >> 3) & 1);
+                ldsm4(b, kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4));
+                mma_16816<T>(s[0], qa[kk], b[0], b[1]);
+                mma_16816<T>(s[1], qa[kk], b[2], b[3]);
+            }
+            const int32_t key = begin + int32_t(t * kTileKeys);
+            if (key + 15 > pos_first || (v.window > 0 && key <= pos_last - int32_t(v.window))) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
-                }
-                const uint32_t krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    uint32_t b[4];
-                    const uint32_t chunk = kk * 2 + ((lane >> 3) & 1);
-                    ldsm4(b, kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4));
-                    mma_16816<T>(s[0], qa[kk], b[0], b[1]);
-                    mma_16816<T>(s[1], qa[kk], b[2], b[3]);
-                }
-                if (key + 15 > pos_first || (v.window > 0 && key <= pos_last - int32_t(v.window))) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int32_t k = key + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
-                            if (k > q || (v.window > 0 && k <= q - int32_t(v.window))) s[j][e] = -INFINITY;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const int32_t k = key + j * 8 + int32_t(tig) * 2 + (e & 1), q = pos[e >> 1];
+                        if (k > q || (v.window > 0 && k <= q - int32_t(v.window))) s[j][e] = -INFINITY;
                     }
                 }
+            }
+        };
+        scores(n, t0);
+        for (uint32_t t = t0; t < t1; ++t, ++n) {
+            const uint32_t st = n % L::kStages, parity = (n / L::kStages) & 1;
+            const uint32_t vbase = smem_u32(smem) + st * L::kStage + kTileBytes<D>;
+            const uint32_t pbase = p_base + (n & 1) * (kRowsM * kTileKeys * 2);
+            float mx[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    mx[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * scale2;
-                }
+            for (int e = 0; e < 2; ++e) {
+                mx[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * scale2;
             }
             // The sums refer to a maximum that all warps share; it moves only
             // when some row's has grown by more than 2^8.
@@ -247,37 +368,36 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                     }
                 }
             }
-            bool clean = false;
-            if (live) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float base = m[e] == -INFINITY ? 0.0f : m[e];  // nothing seen yet: every term is 0
-                    float q[4];
+            for (int e = 0; e < 2; ++e) {
+                const float base = m[e] == -INFINITY ? 0.0f : m[e];  // nothing seen yet: every term is 0
+                float q[4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) q[c] = exp2_approx(fmaf(s[c >> 1][2 * e + (c & 1)], scale2, -base));
-                    l[e] += (q[0] + q[1]) + (q[2] + q[3]);
-                    // 16-byte chunks 2 warp and 2 warp + 1 of the row's 128 keys, chunk c at c ^ (row % 8)
-                    const uint32_t row = grp + 8 * e, at = pbase + row * (kTileKeys * 2) + tig * 4;
-                    const uint32_t c0 = (2 * warp) ^ (row & 7), c1 = (2 * warp + 1) ^ (row & 7);
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c0 * 16), "r"(Num<T>::pack(q[0], q[1])) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c1 * 16), "r"(Num<T>::pack(q[2], q[3])) : "memory");
-                }
-                live = __all_sync(0xffffffffu, mbar_wait(full_v + st, parity, flags, v.error));
-                // what no row sees may hold anything: its probability is 0, but 0 x NaN is not
-                clean = live && (key < int32_t(w.k.lo) || key + 16 > int32_t(w.k.hi));
-                if (clean) {
-                    for (int r = 0; r < 16; ++r) {
-                        if (key + r >= int32_t(w.k.lo) && key + r < int32_t(w.k.hi)) continue;
-                        for (uint32_t c = lane; c < D / 8; c += 32) {
-                            const uint32_t at = vbase + (c >> 3) * (kTileKeys * 128) + (warp * 16 + r) * 128 + ((c & 7) << 4);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                        }
+                for (int c = 0; c < 4; ++c) q[c] = exp2_approx(fmaf(s[c >> 1][2 * e + (c & 1)], scale2, -base));
+                l[e] += (q[0] + q[1]) + (q[2] + q[3]);
+                // 16-byte chunks 2 warp and 2 warp + 1 of the row's 128 keys, chunk c at c ^ (row % 8)
+                const uint32_t row = grp + 8 * e, at = pbase + row * (kTileKeys * 2) + tig * 4;
+                const uint32_t c0 = (2 * warp) ^ (row & 7), c1 = (2 * warp + 1) ^ (row & 7);
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c0 * 16), "r"(Num<T>::pack(q[0], q[1])) : "memory");
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + c1 * 16), "r"(Num<T>::pack(q[2], q[3])) : "memory");
+            }
+            const bool ready = live && __all_sync(0xffffffffu, mbar_wait(full_v + st, parity, flags, v.error));
+            // what no row sees may hold anything: its probability is 0, but 0 x NaN is not
+            const int32_t key = begin + int32_t(t * kTileKeys);
+            if (ready && (key < lo || key + 16 > hi)) {
+                const int32_t from = max(0, min(16, lo - key)), to = max(0, min(16, hi - key));  // rows [from, to) stay
+                for (int32_t i = int32_t(lane); i < 16 * (D / 8); i += 32) {
+                    const int32_t r = i / (D / 8), c = i % (D / 8);
+                    if (r < from || r >= to) {
+                        const uint32_t at = vbase + (c >> 3) * (kTileKeys * 128) + (warp * 16 + r) * 128 + ((c & 7) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
                     }
-                    fence_proxy_async();  // before the copy that reuses the stage
                 }
+                fence_proxy_async();  // before the copy that reuses the stage
             }
             bar_consumers();
-            if (!live) continue;
+            if (t + 1 < t1) scores(n + 1, t + 1);
+            if (!ready) continue;
 #pragma unroll
             for (int kk = 0; kk < kTileKeys / 16; ++kk) {
                 uint32_t a[4], b[4];
@@ -308,23 +428,47 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             for (int x = 0; x < kConsumers; ++x) l[e] += sums[x * kRowsM + grp + 8 * e];
         }
         bool write = t0 == 0 && t1 == w.k.tiles;
+        bool join = false;
         if (!write) {
-            // One part of an item that spans CTAs: the last of them to get here
-            // joins all, in CTA order. Mostly that is the CTA that began the item,
-            // at its end, and finds the others' parts already there.
+            // One part of an item that spans CTAs: the last CTA to get here joins
+            // all. With two parts that is mostly the CTA that began the item, at
+            // its end: it finds the other's there and keeps its own in registers.
             uint32_t c0, c1;
             walk_owners<kItemRows>(w, c0, c1);
-            const uint32_t others = c1 - c0;
-            if (threadIdx.x == 0) {
-                uint32_t there;
-                asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.counters + c0) : "memory");
-                flags[1] = there == others;
+            if (t0 == 0 && c1 == c0 + 1) {
+                if (threadIdx.x == 0) {
+                    uint32_t there;
+                    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(p.counters + c0) : "memory");
+                    flags[1] = there;
+                    if (there) p.counters[c0] = 0;  // nobody else is left to arrive
+                }
+                bar_consumers();
+                write = flags[1] != 0;
             }
-            bar_consumers();
-            write = flags[1] != 0;
-            auto part_of = [&](uint32_t c) { return p.partial + uint64_t(2 * c + (c == c0 ? 1 : 0)) * kSlotFloats; };
-            if (!write) {
-                float * to = part_of(blockIdx.x);
+            if (write) {
+                const float * from = part_of(p, c1, c0);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t row = grp + 8 * e;
+                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + kRowsM * D + 2 * row));
+                    float mine[2 * kTilesN], x[2 * kTilesN];
+#pragma unroll
+                    for (int j = 0; j < kTilesN; ++j) {
+                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(from + row * D + warp * kCols + j * 8 + tig * 2));
+                        x[2 * j] = y.x;
+                        x[2 * j + 1] = y.y;
+                        mine[2 * j] = o[j][2 * e];
+                        mine[2 * j + 1] = o[j][2 * e + 1];
+                    }
+                    join_part(m[e], l[e], mine, ml.x, ml.y, x);
+#pragma unroll
+                    for (int j = 0; j < kTilesN; ++j) {
+                        o[j][2 * e] = mine[2 * j];
+                        o[j][2 * e + 1] = mine[2 * j + 1];
+                    }
+                }
+            } else {
+                float * to = part_of(p, blockIdx.x, c0);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t row = grp + 8 * e;
@@ -334,63 +478,17 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                     }
                     if (warp == 0 && tig == 0) __stcg(reinterpret_cast<float2 *>(to + kRowsM * D + 2 * row), make_float2(m[e], l[e]));
                 }
-                bar_consumers();
-                if (threadIdx.x == 0) {
-                    __threadfence();
-                    flags[1] = atomicAdd(p.counters + c0, 1u) == others;
-                    __threadfence();
-                }
-                bar_consumers();
-                write = flags[1] != 0;
-            }
-            if (write) {
-                if (threadIdx.x == 0) p.counters[c0] = 0;  // nobody else is left to arrive
-                float jm[2] = {-INFINITY, -INFINITY}, jl[2] = {0.0f, 0.0f}, jo[kTilesN][4];
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) jo[j][e] = 0.0f;
-                }
-                for (uint32_t c = c0; c <= c1; ++c) {
-                    const float * from = part_of(c);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t row = grp + 8 * e;
-                        float2 ml = make_float2(m[e], l[e]), x[kTilesN];
-#pragma unroll
-                        for (int j = 0; j < kTilesN; ++j) x[j] = make_float2(o[j][2 * e], o[j][2 * e + 1]);
-                        if (c != blockIdx.x) {
-                            ml = __ldcg(reinterpret_cast<const float2 *>(from + kRowsM * D + 2 * row));
-#pragma unroll
-                            for (int j = 0; j < kTilesN; ++j) {
-                                x[j] = __ldcg(reinterpret_cast<const float2 *>(from + row * D + warp * kCols + j * 8 + tig * 2));
-                            }
-                        }
-                        const float top = fmaxf(jm[e], ml.x);
-                        const float f = jm[e] == -INFINITY ? 0.0f : exp2_approx(jm[e] - top);
-                        const float g = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - top);
-                        jm[e] = top;
-                        jl[e] = jl[e] * f + ml.y * g;
-#pragma unroll
-                        for (int j = 0; j < kTilesN; ++j) {
-                            jo[j][2 * e] = jo[j][2 * e] * f + x[j].x * g;
-                            jo[j][2 * e + 1] = jo[j][2 * e + 1] * f + x[j].y * g;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    m[e] = jm[e];
-                    l[e] = jl[e];
-                }
-#pragma unroll
-                for (int j = 0; j < kTilesN; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] = jo[j][e];
+                if (handed && t0 > 0) {
+                    part_arrive();
+                } else {  // the CTA's last segment
+                    bar_consumers();
+                    if (threadIdx.x == 0) flags[1] = count_part(p.counters + c0, c1 - c0);
+                    bar_consumers();
+                    join = flags[1] != 0;
                 }
             }
-            bar_consumers();  // flags may be written again
         }
+        if (join) join_item<T, D>(p, w, reinterpret_cast<float *>(smem));  // the ring is idle: no segment follows
         if (write) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -401,6 +499,10 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             }
         }
     } while (walk_warp_next<kItemRows>(v, &w));
+    if (handed) {
+        verdict_wait();
+        if (flags[2]) join_item<T, D>(p, walks[kConsumers + 2], reinterpret_cast<float *>(smem));
+    }
 }
 
 template <typename T, int D>
