@@ -227,15 +227,23 @@ struct KeyRange {
     uint32_t tiles;    // max(1, tiles of [begin, hi))
 };
 
-// Packed rows of a sequence: the host refuses calls with 2^31 or more.
+// Packed rows of a sequence: the host refuses calls with 2^31 or more. A
+// division is a long chain of instructions before the first copy: a single
+// item, as in decode, takes none.
 __device__ __forceinline__ uint32_t row_tiles(const View & v, const Sequence & s) {
-    return (s.count * v.group + v.item_rows - 1) / v.item_rows;
+    const uint32_t packed = s.count * v.group;
+    return packed <= v.item_rows ? (packed > 0 ? 1u : 0u) : (packed + v.item_rows - 1) / v.item_rows;
 }
 
 __device__ __forceinline__ KeyRange key_range(const View & v, const Sequence & s, uint32_t tile) {
-    const uint32_t r0 = tile * v.item_rows, r1 = min(r0 + v.item_rows, s.count * v.group) - 1;
+    const uint32_t packed = s.count * v.group;
     const int32_t first = int32_t(s.kv) - int32_t(s.count);
-    const int32_t p0 = first + int32_t(r0 / v.group), p1 = first + int32_t(r1 / v.group);
+    int32_t p0 = first, p1 = first + int32_t(s.count) - 1;
+    if (packed > v.item_rows) {
+        const uint32_t r0 = tile * v.item_rows;
+        p0 = first + int32_t(r0 / v.group);
+        if (r0 + v.item_rows < packed) p1 = first + int32_t((r0 + v.item_rows - 1) / v.group);
+    }
     KeyRange k;
     k.hi = p1 < 0 ? 0u : uint32_t(p1 + 1);
     k.lo = v.window > 0 && p0 >= int32_t(v.window) ? uint32_t(p0) - v.window + 1 : 0u;
@@ -256,24 +264,23 @@ template <class Items>
 struct WalkOf {
     uint64_t unit, end;    // this CTA's line segment still to do
     uint64_t item0;        // first unit of the current item
-    uint64_t total;        // units in all
-    uint32_t ctas;         // CTAs that have work
+    uint64_t share;        // units of a CTA; the first `extra` have one more
+    uint32_t extra;
     uint32_t kv_head, b, tile;
     Sequence s;
     typename Items::Part k;
 };
 using Walk = WalkOf<RowItems>;
 
-// a * b / c, in 32 bits where that holds it (a 64-bit division takes hundreds of cycles).
-__device__ __forceinline__ uint64_t mul_div(uint64_t a, uint64_t b, uint64_t c) {
-    const uint64_t n = a * b;
-    return (n | c) >> 32 ? n / c : uint32_t(n) / uint32_t(c);
+__device__ __forceinline__ uint64_t divide(uint64_t a, uint64_t b) {
+    // 64-bit divisions take hundreds of cycles
+    return (a | b) >> 32 ? a / b : uint32_t(a) / uint32_t(b);
 }
 
-// The CTA that holds `unit`: the last c with c * total / ctas <= unit.
-__device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t total, uint64_t ctas) {
-    const uint64_t n = (unit + 1) * ctas - 1;
-    return (n | total) >> 32 ? uint32_t(n / total) : uint32_t(n) / uint32_t(total);
+// The CTA that holds `unit`.
+__device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t share, uint32_t extra) {
+    const uint64_t larger = extra * (share + 1);
+    return unit < larger ? uint32_t(divide(unit, share + 1)) : extra + uint32_t(divide(unit - larger, share));
 }
 
 // Key tiles [t0, t1) of the current item that this CTA does.
@@ -322,8 +329,8 @@ __device__ __forceinline__ bool walk_warp_next(const View & v, WalkOf<Items> * w
 // The CTAs that hold the first and the last tile of the current item.
 template <int E, class Items>
 __device__ __forceinline__ void walk_owners(const WalkOf<Items> & w, uint32_t & c0, uint32_t & c1) {
-    c0 = cta_of(w.item0 + E, w.total, w.ctas);
-    c1 = cta_of(w.item0 + E + w.k.tiles - 1, w.total, w.ctas);
+    c0 = cta_of(w.item0 + E, w.share, w.extra);
+    c1 = cta_of(w.item0 + E + w.k.tiles - 1, w.share, w.extra);
 }
 
 // Positions `walks`, one WalkOf per warp of the CTA in shared memory, at the
@@ -393,14 +400,18 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
         for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
     }
     WalkOf<Items> x = {};
-    x.total = uint64_t(per_head) * v.kv_heads;
-    x.ctas = uint64_t(workers) < x.total ? workers : uint32_t(x.total);
-    if (index < x.ctas) {
-        x.unit = mul_div(index, x.total, x.ctas);
-        x.end = mul_div(index + 1, x.total, x.ctas);
-        x.kv_head = uint32_t(mul_div(x.unit, 1, per_head));
+    const uint64_t total = uint64_t(per_head) * v.kv_heads;
+    x.share = divide(total, workers);
+    x.extra = uint32_t(total - x.share * workers);
+    x.unit = index * x.share + min(index, x.extra);
+    x.end = x.unit + x.share + (index < x.extra ? 1 : 0);
+    if (x.unit < x.end) {
+        unsigned long long left = x.unit;
+        while (left >= per_head) {
+            left -= per_head;
+            ++x.kv_head;
+        }
         // the first entry of a list whose running sum exceeds what is left: 32 at a time
-        unsigned long long left = x.unit - uint64_t(x.kv_head) * per_head;
         const auto find32 = [&](unsigned long long mine, int & src) {
             unsigned long long upto = mine;
             if (narrow) {
