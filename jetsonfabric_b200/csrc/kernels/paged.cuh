@@ -164,46 +164,47 @@ template <int D>
 constexpr uint32_t kTileBytes = kTileKeys * D * 2;
 
 // A tile's load by one warp, a box (a page, or 128 keys of a larger one) per
-// lane, in two steps: the page ids are fetched while the tile's place in the
-// ring is still in use, their latency being most of the way to issuing.
+// lane, in two steps: the page ids are asked for while the tile's place in the
+// ring is still in use and looked at only when it is free.
 struct TileLoad {
-    int32_t page;      // of this lane's box
+    int32_t page;      // of this lane's box, as the table has it
     uint32_t token;    // its first token within the page
     uint32_t boxes, step;
 };
 
 // Boxes of keys [key0, key1) (at most 128, key0 a multiple of the box) of the
-// sequence whose table row is `row`. A page id outside the pool becomes one
-// that reads as zeros: the tensor map fills coordinates outside the pool.
+// sequence whose table row is `row`.
 __device__ __forceinline__ TileLoad tile_pages(const View & v, const int32_t * row, uint32_t key0, uint32_t key1) {
     const uint32_t lane = threadIdx.x & 31;
     TileLoad l;
     l.step = v.page_size < uint32_t(kTileKeys) ? v.page_size : uint32_t(kTileKeys);
-    l.boxes = (key1 - key0 + l.step - 1) / l.step;
+    l.boxes = (key1 - key0 + l.step - 1) >> (v.page_shift < 7 ? v.page_shift : 7);
     const uint32_t key = key0 + lane * l.step;
     l.token = key & (v.page_size - 1);
     l.page = 0;
-    if (lane < l.boxes) {
-        l.page = row[key >> v.page_shift];
-        if (l.page < 0 || uint32_t(l.page) >= v.pages) {
-            flag_error(v.error, JFB_PAGED_ERROR_RANGE);
-            l.page = int32_t(v.pages);
-        }
-    }
+    if (lane < l.boxes) l.page = row[key >> v.page_shift];
     return l;
 }
 
-// Lane 0 announces the bytes, then every lane issues its boxes.
+// Lane 0 announces the bytes, then every lane issues its boxes. A page id
+// outside the pool becomes one that reads as zeros: the tensor map fills
+// coordinates outside the pool.
 template <int D>
-__device__ __forceinline__ void tile_issue(const TileLoad & l, const CUtensorMap * map, uint32_t head, uint32_t dst, uint64_t * bar) {
+__device__ __forceinline__ void tile_issue(const View & v, const TileLoad & l, const CUtensorMap * map, uint32_t head, uint32_t dst,
+                                           uint64_t * bar) {
     const uint32_t lane = threadIdx.x & 31;
     if (lane == 0) mbar_arrive_expect_tx(bar, l.boxes * l.step * D * 2);
     __syncwarp();
     if (lane < l.boxes) {
+        int32_t page = l.page;
+        if (page < 0 || uint32_t(page) >= v.pages) {
+            flag_error(v.error, JFB_PAGED_ERROR_RANGE);
+            page = int32_t(v.pages);
+        }
         const uint32_t to = dst + lane * l.step * 128;
 #pragma unroll
         for (int h = 0; h < D / 64; ++h) {
-            tma_load_page(to + h * (kTileKeys * 128), map, h * 64, int32_t(l.token), int32_t(head), l.page, bar);
+            tma_load_page(to + h * (kTileKeys * 128), map, h * 64, int32_t(l.token), int32_t(head), page, bar);
         }
     }
     __syncwarp();

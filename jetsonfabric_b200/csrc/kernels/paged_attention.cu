@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 const uint32_t st = n % L::kStages, turn = n / L::kStages;
                 if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
                 if (!ok) break;
-                tile_issue<D>(load, map, head, smem_u32(smem) + st * L::kStage + (is_v ? kTileBytes<D> : 0u), full + st);
+                tile_issue<D>(v, load, map, head, smem_u32(smem) + st * L::kStage + (is_v ? kTileBytes<D> : 0u), full + st);
             }
         } while (ok && walk_warp_next<kItemRows>(v, &w));
         if (flags[0]) {

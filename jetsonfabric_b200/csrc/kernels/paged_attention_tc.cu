@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                     for (uint32_t is_v = 0; is_v < 2; ++is_v, ++n) {
                         const uint32_t st = n % L::kStages, turn = n / L::kStages;
                         if (turn > 0 && !wait(empty + st, (turn - 1) & 1)) break;
-                        tile_issue<D>(load, is_v ? &maps.v : &maps.k, head, ring + st * kTileBytes<D>, full + st);
+                        tile_issue<D>(v, load, is_v ? &maps.v : &maps.k, head, ring + st * kTileBytes<D>, full + st);
                     }
                 }
             } while (ok && walk_warp_next<kItemTc>(v, &w));

@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             const uint32_t key1 = min(limit, key0 + uint32_t(kTileKeys));
             const TileLoad k1 = tile_pages(v, row, key1, min(limit, key0 + kItemKeys));
             if (item > 0 && !wait(k_free, (item - 1) & 1)) break;
-            tile_issue<D>(k0, &maps.k, w.kv_head, smem_u32(smem), k_full);
-            tile_issue<D>(k1, &maps.k, w.kv_head, smem_u32(smem) + kTileBytes<D>, k_full);
+            tile_issue<D>(v, k0, &maps.k, w.kv_head, smem_u32(smem), k_full);
+            tile_issue<D>(v, k1, &maps.k, w.kv_head, smem_u32(smem) + kTileBytes<D>, k_full);
             for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
                 const uint32_t st = s % L::kQStages;
                 if (s >= L::kQStages && !wait(q_free + st, (s / L::kQStages - 1) & 1)) break;
