@@ -19,7 +19,7 @@ namespace {
 // head of the group) 16 at a time through mma.sync m16n8k16.
 
 constexpr int kConsumers = 8;
-constexpr int kThreadsRows = (kConsumers + 1) * 32;
+constexpr int kThreadsRows = (kConsumers + 2) * 32;  // and the producers of K and of the masses
 
 // A sequence and kv head is one item, its key tiles the units.
 struct SequenceItems {
@@ -41,7 +41,8 @@ using SequenceWalk = WalkOf<SequenceItems>;
 template <int D>
 struct MassSmem {
     static constexpr int kStages = D == 128 ? 6 : 12;
-    static constexpr uint32_t kBars = kStages * kTileBytes<D>;  // full, empty
+    static constexpr uint32_t kBefore = kStages * kTileBytes<D>;             // [stages][128] masses
+    static constexpr uint32_t kBars = kBefore + kStages * kTileKeys * 4;     // full, empty
     static constexpr uint32_t kWalk = kBars + 2 * kStages * 8;
     static constexpr uint32_t kFlags = kWalk + kThreadsRows / 32 * sizeof(SequenceWalk);
     static constexpr uint32_t kBytes = kFlags + 16 + 1024;
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) {
-            mbar_init(full + i, 1);
+            mbar_init(full + i, 33);  // the K copy's announcement, and every producer lane's masses
             mbar_init(empty + i, kConsumers);
         }
         flags[0] = 0;
@@ -85,7 +86,8 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
     if (!walk_begin<0>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
     SequenceWalk & w = walks[warp];
 
-    if (warp == kConsumers) {
+    if (warp >= kConsumers) {
+        const bool keys = warp == kConsumers;
         uint32_t n = 0;
         bool ok = true;
         do {
@@ -93,20 +95,36 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             walk_segment<0>(w, t0, t1);
             const int32_t * row = v.table + uint64_t(w.b) * v.table_stride;
             const uint32_t limit = SequenceItems::limit(v, w.s), head = w.kv_head;
+            const int64_t first = int64_t(w.s.kv) - w.s.count;
+            const uint64_t line = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots;
             auto pages_of = [&](uint32_t t) {
                 return tile_pages(v, row, t * kTileKeys, min(limit, (t + 1) * uint32_t(kTileKeys)));
             };
-            TileLoad next = pages_of(t0);
+            TileLoad next = {};
+            if (keys) next = pages_of(t0);
             for (uint32_t t = t0; t < t1; ++t, ++n) {
                 const TileLoad load = next;
-                if (t + 1 < t1) next = pages_of(t + 1);
+                if (keys && t + 1 < t1) next = pages_of(t + 1);
                 const uint32_t st = n % L::kStages, turn = n / L::kStages;
                 if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty + st, (turn - 1) & 1, flags, v.error));
                 if (!ok) break;
-                tile_issue<D>(v, load, &map_k, head, smem_u32(smem) + st * kTileBytes<D>, full + st);
+                if (keys) {
+                    tile_issue<D>(v, load, &map_k, head, smem_u32(smem) + st * kTileBytes<D>, full + st);
+                    continue;
+                }
+                const uint32_t to = smem_u32(smem) + L::kBefore + st * (kTileKeys * 4);
+#pragma unroll
+                for (uint32_t j = 0; j < uint32_t(kTileKeys) / 32; ++j) {  // zeros for new slots and behind the keys
+                    const uint32_t i = j * 32 + lane, k = t * kTileKeys + i;
+                    const bool held = p.mass_in != nullptr && k < limit && int64_t(k) < first;
+                    const float * src = held ? p.mass_in + line + k : p.lse;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + i * 4), "l"(src), "r"(held ? 4u : 0u) : "memory");
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full + st)) : "memory");
             }
         } while (ok && walk_warp_next<0>(v, &w));
-        if (flags[0]) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (keys && flags[0]) {
             for (uint32_t i = n > uint32_t(L::kStages) ? n - L::kStages : 0u; i < n; ++i) {
                 mbar_drain(full + i % L::kStages, (i / L::kStages) & 1);
             }
@@ -165,16 +183,11 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                              : "r"(kbase + (chunk >> 3) * (kTileKeys * 128) + krow * 128 + (((chunk & 7) ^ (krow & 7)) << 4))
                              : "memory");
             }
+            const float before = reinterpret_cast<const float *>(smem + L::kBefore)[st * kTileKeys + warp * 16 + (lane & 15)];
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + st);
             const uint32_t key = t * kTileKeys + warp * 16;
             if (key >= limit) continue;
-            float before[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of this lane's four keys, fetched while the products run
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t k = key + (x >> 1) * 8 + tig * 2 + (x & 1);
-                if (grp == 0 && p.mass_in != nullptr && k < limit && int64_t(k) < first) before[x] = p.mass_in[line + k];
-            }
             uint32_t r0, r1;
             seeing_rows(w.s, G, v.window, key, min(limit, key + 16), r0, r1);
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -206,13 +219,14 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor_sync(0xffffffffu, acc[x], d);
             }
-            if (grp == 0) {
+            // key i's sum lies in lane i % 8 / 2, register i / 8 * 2 + i % 2
+            float sum = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t k = key + (x >> 1) * 8 + tig * 2 + (x & 1);
-                    if (k < limit) p.mass_out[line + k] = before[x] + acc[x];
-                }
+            for (int x = 0; x < 4; ++x) {
+                const float y = __shfl_sync(0xffffffffu, acc[x], (lane & 7) >> 1);
+                if ((lane >> 3) * 2 + (lane & 1) == uint32_t(x)) sum = y;
             }
+            if (lane < 16 && key + lane < limit) p.mass_out[line + key + lane] = before + sum;
         }
     } while (walk_warp_next<0>(v, &w));
 }
