@@ -656,3 +656,94 @@ def test_a_conversation_through_all_of_them(P, dtype):
         values[b] = torch.stack([values[b][at[:, h], h] for h in range(kvh)], 1)
     step([1, 1, 1])
     step([17, 1, 40])
+
+
+# ---- the whole range, at random ---------------------------------------------------------------
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_batches(P, seed):
+    """Random shapes through attention and accumulated weight, twice with one workspace: right and bit for bit the same."""
+    import random
+    rng = random.Random(seed)
+    kv_heads = rng.choice([1, 2, 3, 8])
+    group = rng.choice([1, 2, 3, 5, 6, 7, 8, 16, 24])
+    hd = rng.choice([8, 64, 72, 128, 128])
+    ps = rng.choice([8, 16, 64, 256])
+    window = rng.choice([0, 0, 1, 7, 130, 1000])
+    n = rng.choice([1, 2, 5, 40, 150])
+    most = max(2, 6000 // n)
+    kv = [rng.choice([0, 1, rng.randrange(1, most), rng.randrange(1, most)]) for _ in range(n)]
+    longest = rng.choice([1, 1, 4, 40, 300])
+    new = [min(k + rng.choice([0, 0, 0, 2]), rng.choice([0, 1, rng.randrange(1, longest + 1)])) for k in kv]
+    if sum(new) == 0:
+        new[0], kv[0] = 1, max(1, kv[0])
+    dtype = rng.choice([torch.float16, torch.bfloat16])
+    case = Case(P, new, kv, kv_heads, hd, ps, dtype, seed=seed, pad=rng.randrange(3), heads_first=rng.random() < 0.5)
+    q = case.queries(kv_heads * group)
+    workspace = P.attention_workspace()
+    out, lse = run_attention(P, case, q, window, workspace=workspace)
+    check_attention(case, q, out, lse, hd ** -0.5, window)
+    again, lse2 = run_attention(P, case, q, window, workspace=workspace)
+    assert torch.equal(out.nan_to_num(), again.nan_to_num()) and torch.equal(lse, lse2)
+    mass = torch.full((n, kv_heads, max(max(kv), 1)), math.nan, device="cuda")
+    P.attention_mass(q, lse, case.cache, case.batch, mass, window=window, error_flag=case.error)
+    torch.cuda.synchronize()
+    check_mass(case, q, lse, None, mass, hd ** -0.5, window)
+    assert int(case.error) == 0
+
+
+@pytest.mark.parametrize("n", [129, 700, 4096])
+@pytest.mark.parametrize("new", [1, 7])
+def test_many_sequences(P, n, new):
+    """More sequences than a warp's registers hold, up to the most a call takes."""
+    kv = [new + (b * 37) % 90 for b in range(n)]
+    case = Case(P, [new] * n, kv, 1, 64, 16, torch.bfloat16, seed=n)
+    q = case.queries(8)
+    out, lse = run_attention(P, case, q)
+    mass = torch.full((n, 1, max(kv)), math.nan, device="cuda")
+    P.attention_mass(q, lse, case.cache, case.batch, mass)
+    torch.cuda.synchronize()
+    for b in range(0, n, max(1, n // 60)):  # each sequence like a case of its own
+        one = Case.__new__(Case)
+        one.new, one.kv, one.kvh, one.hd = [new], [kv[b]], 1, 64
+        one.starts, one.keys, one.values = [0, new], [case.keys[b]], [case.values[b]]
+        r = slice(case.starts[b], case.starts[b + 1])
+        check_attention(one, q[r], out[r], lse[r], 0.125, 0)
+        check_mass(one, q[r], lse[r], None, mass[b:b + 1], 0.125, 0)
+
+
+def test_one_long_context_over_all_ctas(P):
+    """One sequence of 60000 keys, split over every CTA and joined, for a single token and for a chunk."""
+    for new in (1, 20, 300):
+        case = Case(P, [new], [60000], 2, 128, 64, torch.float16, seed=new)
+        q = case.queries(4)
+        workspace = P.attention_workspace()
+        out, lse = run_attention(P, case, q, workspace=workspace)
+        check_attention(case, q, out, lse, 128 ** -0.5, 0)
+        for _ in range(5):
+            again, lse2 = run_attention(P, case, q, workspace=workspace)
+            assert torch.equal(out, again) and torch.equal(lse, lse2)
+        mass = torch.empty(1, 2, 60000, device="cuda")
+        P.attention_mass(q, lse, case.cache, case.batch, mass)
+        torch.cuda.synchronize()
+        check_mass(case, q, lse, None, mass, 128 ** -0.5, 0)
+
+
+def test_evict_beyond_the_selections_cache(P):
+    """More keys than the selection holds in registers and in shared memory, in place, with many ties."""
+    for kv in ([16385, 70000], [49153, 40000]):
+        case = Case(P, [0, 0], kv, 1, 8, 128, torch.float16, seed=kv[0])
+        mass = torch.randint(0, 50, (2, 1, max(kv)), device="cuda", generator=case.g).float()
+        weights = mass.cpu().tolist()
+        keep = torch.empty(2, 1, 20000, dtype=torch.int32, device="cuda")
+        P.evict(mass, case.cache, case.batch, keep, case.kv_len, recent=100, error_flag=case.error)
+        torch.cuda.synchronize()
+        assert int(case.error) == 0
+        for b, k in enumerate(kv):
+            m = min(k, 20000)
+            want = kept_slots(weights[b][0], k, 20000, 100)
+            assert keep[b, 0, :m].tolist() == want and torch.all(keep[b, 0, m:] == -1)
+            at = torch.tensor(want).cuda()
+            page, place = case.where(b, torch.arange(m))
+            assert torch.equal(case.k_pool[page, place], case.keys[b][at])
+            assert torch.equal(mass[b, 0, :m], torch.tensor(weights[b][0], device="cuda")[at])
