@@ -29,7 +29,7 @@ namespace jfb {
 namespace paged {
 namespace {
 
-constexpr int kItemTc = 2;  // units of an item's start and end
+constexpr int kItemTc = 3;  // units of an item's start and end (a prompt of 8192, 28/4 heads: 449, 409, 388, 389 us with 1 to 4)
 constexpr int kThreadsTc = 384;
 constexpr int kWarpS = 8, kWarpKV = 9, kWarpQ = 10;  // warp 11 issues P V
 constexpr uint32_t kColO = 0, kColP = 256, kColS = 384;  // O_1 is 128 and P_1 64 columns further
