@@ -5,13 +5,16 @@
 //    and orders them as unsigned numbers. The threshold (the need-th largest) is
 //    found two bits at a time by counting how many reach each of three
 //    candidates: sixteen passes over registers (up to 16384 keys) with one
-//    barrier each, whose cost does not depend on how the masses are spread
+//    barrier each (fewer once the kept set is settled), whose cost does not
+//    depend on how the masses are spread
 //    (a histogram of digits in shared memory was slower: the usual few octaves
 //    make its counters collide). A last pass in slot order
 //    keeps all above it and the first of those that equal it, so ties fall to
 //    the lowest slot and the result is exact.
-// 2. move: K and V rows to their new slots, 16 bytes a thread. Out of place,
-//    every 32 rows of a (sequence, head) are a CTA of their own (D = 128). In place a CTA
+// 2. move: K and V rows to their new slots. Out of place, every 32 rows of a
+//    (sequence, head) are a CTA of their own (D = 128), a thread moving 32-byte
+//    sectors (66 us for a batch of 32 sequences of 1500 to 8192 keys cut to 2048,
+//    4 kv heads, both steps; 75 with 16 bytes a thread). In place a CTA
 //    owns a column slice of one (sequence, head) and walks the rows in order,
 //    reading a whole step before it writes it: a row only moves to lower
 //    slots, so a step overwrites no later step's source.
@@ -21,12 +24,10 @@ namespace jfb {
 namespace paged {
 namespace {
 
-constexpr int kThreads = 1024;  // of the selection
-constexpr uint32_t kWarps = kThreads / 32;
 constexpr uint32_t kCached = 49152;  // masses that fit shared memory
 constexpr uint32_t kOwn = 16;        // keys a thread of the selection holds
-// threads of the move and 16-byte pieces in flight in each
-constexpr int kFarThreads = 256, kFarPieces = 2;
+// threads of the move and the pieces in flight in each
+constexpr int kFarThreads = 128, kFarPieces = 2;
 constexpr int kNearThreads = 512, kNearPieces = 8;
 
 struct EvictParams {
@@ -62,7 +63,9 @@ __device__ __forceinline__ uint32_t evict_length(const EvictParams & p, uint32_t
     return len;
 }
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
+    constexpr uint32_t kWarps = kThreads / 32;
     extern __shared__ float cache[];
     __shared__ uint32_t counts[2][3][kWarps];
     __shared__ uint32_t above_of[kWarps], equal_of[kWarps];
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
                 n = __reduce_add_sync(0xffffffffu, n);
                 if (lane == 0) counts[half][0][warp] = n;
                 __syncthreads();
-                n = counts[half][0][lane];
+                n = lane < kWarps ? counts[half][0][lane] : 0u;
                 const uint32_t low = __reduce_add_sync(0xffffffffu, (n & 1023u) | ((n >> 10) & 1023u) << 16);
                 n1 = low & 0xffffu;
                 n2 = low >> 16;
@@ -140,9 +143,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
                     counts[half][2][warp] = n3;
                 }
                 __syncthreads();
-                n1 = __reduce_add_sync(0xffffffffu, counts[half][0][lane]);
-                n2 = __reduce_add_sync(0xffffffffu, counts[half][1][lane]);
-                n3 = __reduce_add_sync(0xffffffffu, counts[half][2][lane]);
+                n1 = __reduce_add_sync(0xffffffffu, lane < kWarps ? counts[half][0][lane] : 0u);
+                n2 = __reduce_add_sync(0xffffffffu, lane < kWarps ? counts[half][1][lane] : 0u);
+                n3 = __reduce_add_sync(0xffffffffu, lane < kWarps ? counts[half][2][lane] : 0u);
             }
             const uint32_t digit = n3 >= need ? 3u : n2 >= need ? 2u : n1 >= need ? 1u : 0u;
             if (digit < 3) above = digit == 2 ? n3 : digit == 1 ? n2 : n1;
@@ -205,7 +208,30 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const EvictParams p) {
     }
 }
 
-template <int THREADS, int PIECES, bool IN_PLACE>
+// What a thread moves at once: 16 bytes, or a 32-byte sector.
+struct Piece16 {
+    static constexpr uint32_t kElements = 8;
+    uint4 x;
+    __device__ __forceinline__ void load(const uint16_t * p) { x = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void store(uint16_t * p) const { *reinterpret_cast<uint4 *>(p) = x; }
+};
+struct Piece32 {
+    static constexpr uint32_t kElements = 16;
+    uint32_t x[8];
+    __device__ __forceinline__ void load(const uint16_t * p) {
+        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
+                     : "l"(p)
+                     : "memory");
+    }
+    __device__ __forceinline__ void store(uint16_t * p) const {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]),
+                     "r"(x[5]), "r"(x[6]), "r"(x[7])
+                     : "memory");
+    }
+};
+
+template <class Piece, int THREADS, int PIECES, bool IN_PLACE>
 __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
     pdl_trigger();
     pdl_wait();
@@ -215,7 +241,7 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
     const int32_t * keep = p.keep + uint64_t(line) * p.budget;
     const int32_t * from = v.table + uint64_t(b) * v.table_stride;
     const int32_t * to = p.table_out + uint64_t(b) * p.table_out_stride;
-    const uint32_t width = v.head_dim / 8 / p.slices, first = blockIdx.z * width;  // pieces of a row
+    const uint32_t width = v.head_dim / Piece::kElements / p.slices, first = blockIdx.z * width;  // pieces of a row
     const uint32_t step = THREADS * PIECES / width;                                  // rows read before they are written
     const uint32_t kept = min(evict_length(p, b), p.budget);
     // The new length may replace the old one that other CTAs still read: they
@@ -223,13 +249,12 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
     if (head == 0 && (blockIdx.x & 1) == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.kv_len_out[b] = int32_t(kept);
     const uint32_t begin = IN_PLACE ? 0u : blockIdx.y * step, end = IN_PLACE ? kept : min(kept, begin + step);
     for (uint32_t row0 = begin; row0 < end; row0 += step) {
-        uint4 x[PIECES];
+        Piece x[PIECES];
         uint64_t dst[PIECES];
 #pragma unroll
         for (int u = 0; u < PIECES; ++u) {
-            const uint32_t i = threadIdx.x + u * THREADS, r = i / width, c = (first + i - r * width) * 8;
+            const uint32_t i = threadIdx.x + u * THREADS, r = i / width, c = (first + i - r * width) * Piece::kElements;
             dst[u] = ~0ull;
-            x[u] = make_uint4(0, 0, 0, 0);
             if (r < step && row0 + r < end) {
                 const uint32_t at = row0 + r;
                 const uint32_t j = uint32_t(keep[at]);
@@ -239,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
                     dst[u] = uint64_t(dst_page) * v.page_stride + (at & (v.page_size - 1)) * v.token_stride + in;
                     const uint64_t src = uint64_t(src_page) * v.page_stride + (j & (v.page_size - 1)) * v.token_stride + in;
                     if (src == dst[u]) dst[u] = ~0ull;  // stays where it is
-                    else x[u] = *reinterpret_cast<const uint4 *>(pool + src);
+                    else x[u].load(pool + src);
                 } else {
                     flag_error(v.error, JFB_PAGED_ERROR_RANGE);
                 }
@@ -248,7 +273,7 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
         if (IN_PLACE) __syncthreads();
 #pragma unroll
         for (int u = 0; u < PIECES; ++u) {
-            if (dst[u] != ~0ull) *reinterpret_cast<uint4 *>(pool + dst[u]) = x[u];
+            if (dst[u] != ~0ull) x[u].store(pool + dst[u]);
         }
         if (IN_PLACE) __syncthreads();
     }
@@ -313,15 +338,26 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     while (in_place && p.slices < 4 && pieces % (p.slices * 2) == 0 && pieces / (p.slices * 2) >= 4 && lines * 2 * p.slices < 4 * device.sms) {
         p.slices *= 2;
     }
-    const uint32_t step = kFarThreads * kFarPieces / pieces;
+    // out of place in 32-byte sectors where rows are made of them
+    const bool sectors = !in_place && cache->head_dim % 16 == 0 && (cache->page_stride | cache->token_stride | cache->head_stride) % 16 == 0 &&
+                         ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) & 31u) == 0;
+    const uint32_t step = kFarThreads * kFarPieces / (sectors ? pieces / 2 : pieces);
     const uint32_t steps = in_place ? 1u : (budget + step - 1) / step;
     if (steps > 65535u) return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: a budget of %u is too large", budget);
     cudaStream_t s = as_stream(stream);
-    cudaError_t e = allow_smem<select_kernel>(device, kCached * sizeof(float));
-    if (e == cudaSuccess) e = launch_k(select_kernel, dim3(lines), dim3(kThreads), p.cached * sizeof(float), s, p);
+    // Short lines: a small CTA, whose barriers are cheaper (one sequence of 2000
+    // keys, 2 kv heads: 9.3 us with both steps, 12 with 1024 threads).
+    cudaError_t e;
+    if (p.cached <= kOwn * 256) {
+        e = launch_k(select_kernel<256>, dim3(lines), dim3(256), p.cached * sizeof(float), s, p);
+    } else {
+        e = allow_smem<select_kernel<1024>>(device, kCached * sizeof(float));
+        if (e == cudaSuccess) e = launch_k(select_kernel<1024>, dim3(lines), dim3(1024), p.cached * sizeof(float), s, p);
+    }
     if (e == cudaSuccess) {
-        e = in_place ? launch_k(move_kernel<kNearThreads, kNearPieces, true>, dim3(lines * 2, 1, p.slices), dim3(kNearThreads), 0, s, p)
-                     : launch_k(move_kernel<kFarThreads, kFarPieces, false>, dim3(lines * 2, steps), dim3(kFarThreads), 0, s, p);
+        e = in_place  ? launch_k(move_kernel<Piece16, kNearThreads, kNearPieces, true>, dim3(lines * 2, 1, p.slices), dim3(kNearThreads), 0, s, p)
+            : sectors ? launch_k(move_kernel<Piece32, kFarThreads, kFarPieces, false>, dim3(lines * 2, steps), dim3(kFarThreads), 0, s, p)
+                      : launch_k(move_kernel<Piece16, kFarThreads, kFarPieces, false>, dim3(lines * 2, steps), dim3(kFarThreads), 0, s, p);
     }
     if (e != cudaSuccess) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_evict: %s", cudaGetErrorString(e));
     return launch_status("jfb_paged_evict");
