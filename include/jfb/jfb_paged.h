@@ -122,8 +122,8 @@ typedef struct jfb_rope {
  * f32; each value is rounded once. q_out may be q itself (same dtype and
  * stride). pos[r] is row r's rotary position, any int32: after an eviction a
  * token's position is no longer its slot. A row whose slot is negative or
- * whose page id is outside the pool keeps its q_out and appends nothing
- * (error bit 0). Two rows of one call must not share a slot. */
+ * beyond the table, or whose page id is outside the pool, gets its q_out but
+ * appends nothing (error bit 0). Two rows of one call must not share a slot. */
 jfb_status jfb_rope_paged_append(const void * q, const void * k, const void * v, uint32_t in_dtype, uint64_t q_stride,
                                  uint64_t k_stride, uint64_t v_stride, uint32_t rows, uint32_t heads,
                                  const int32_t * pos, const jfb_rope * rope, const jfb_paged_cache * cache,

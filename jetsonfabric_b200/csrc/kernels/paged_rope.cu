@@ -193,8 +193,10 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeParams 
             const Sequence s = load_sequence(v, lo);
             in = r >= s.q0 && r - s.q0 < s.count;
             if (in) {
-                const int64_t j = int64_t(s.kv) - s.count + (r - s.q0);
-                const int32_t page = j < 0 ? -1 : v.table[uint64_t(lo) * v.table_stride + (uint64_t(j) >> v.page_shift)];
+                // from the length as it is, not as the table cuts it: that slot holds another key
+                const int64_t j = int64_t(v.kv_len[lo]) - s.count + (r - s.q0);
+                const bool there = j >= 0 && uint64_t(j) >> v.page_shift < v.table_width;
+                const int32_t page = there ? v.table[uint64_t(lo) * v.table_stride + (uint64_t(j) >> v.page_shift)] : -1;
                 if (page >= 0 && uint32_t(page) < v.pages) {
                     at = uint64_t(page) * v.page_stride + (uint64_t(j) & (v.page_size - 1)) * v.token_stride;
                 } else {

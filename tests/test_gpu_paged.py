@@ -451,6 +451,24 @@ def test_rope_skips_bad_slots(P):
     assert torch.equal(case.k_pool.view(torch.int16), before.view(torch.int16))
 
 
+def test_rope_appends_nothing_beyond_the_table(P):
+    """A length beyond the table: the row that has no slot must not take the last one's."""
+    case = Case(P, [2, 1], [64, 64])
+    case.kv_len[0] = 65  # new tokens at slots 63 and 64, the table holds 64
+    case.kv_len[1] = 2 ** 31 - 1
+    before = case.k_pool.clone()
+    q, k = rand(case.g, 3, 4, 128), rand(case.g, 3, 2, 128)
+    out = torch.zeros(3, 4, 128, dtype=torch.float16, device="cuda")
+    rope = P.Rope(torch.zeros(64, dtype=torch.float64, device="cuda"))
+    P.rope_append(q, k, k, torch.zeros(3, dtype=torch.int32, device="cuda"), rope, case.cache, case.batch, out, error_flag=case.error)
+    torch.cuda.synchronize()
+    assert torch.equal(out, q.half()) and int(case.error) == P.ERROR_RANGE
+    page, place = case.where(0, torch.arange(63, 64))
+    assert torch.equal(case.k_pool[page, place], k[:1].half())
+    case.k_pool[page, place] = before[page, place]
+    assert torch.equal(case.k_pool.view(torch.int16), before.view(torch.int16))
+
+
 # ---- accumulated weight ----------------------------------------------------------------
 
 def check_mass(case, q, lse, before, got, scale, window):
