@@ -19,6 +19,10 @@
  * stated per call), bit 1 when a bounded wait inside a kernel gave up and the
  * outputs are incomplete.
  *
+ * Calls without rows or without sequences are allowed, with NULL for the
+ * arrays that are then empty. Without rows the accumulated weight still carries
+ * mass_in over to mass_out; the others do nothing.
+ *
  * The reference keeps one contiguous cache per session
  * (qwen2_architecture.cpp:1072-1079) and has no counterpart of these calls.
  */

@@ -555,7 +555,8 @@ inline jfb_status check_cache(const jfb_paged_cache * c) {
 }
 
 inline jfb_status check_batch(const jfb_paged_batch * b, bool rows) {
-    if (b == nullptr || (rows && b->q_start == nullptr) || b->kv_len == nullptr || b->page_table == nullptr) {
+    // the arrays of no sequences need not exist
+    if (b == nullptr || (b->sequences > 0 && ((rows && b->q_start == nullptr) || b->kv_len == nullptr || b->page_table == nullptr))) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "paged batch arrays are required");
     }
     if (b->sequences > JFB_PAGED_MAX_SEQUENCES) {

@@ -537,6 +537,7 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     if (!(scale > 0.0f) || scale > 3.0e38f || window > 0x7fffffffu) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a positive finite scale and a window below 2^31");
     }
+    if (rows == 0 || batch->sequences == 0) return status_ok();
     const Device device = current_device();
     const uint32_t sms = device.sms;
     if (sms == 0 || sms * 2 * sizeof(uint32_t) > kCounterBytes) {
@@ -547,7 +548,6 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a 16-byte aligned workspace of %llu bytes",
                             static_cast<unsigned long long>(need));
     }
-    if (rows == 0 || batch->sequences == 0) return status_ok();
     AttentionParams p;
     p.view = make_view(*cache, *batch, rows, heads / cache->kv_heads, window, error_flag);
     p.view.item_rows = kRowsM;

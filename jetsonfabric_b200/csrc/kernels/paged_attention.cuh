@@ -87,7 +87,7 @@ jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap 
 // Query-shaped rows [rows][heads x head_dim] of 16-bit numbers.
 inline jfb_status check_rows(const char * what, const void * x, uint64_t stride, uint32_t rows, uint32_t heads,
                              const jfb_paged_cache & c) {
-    if (x == nullptr || (reinterpret_cast<uintptr_t>(x) & 15u) != 0) {
+    if ((x == nullptr && rows > 0) || (reinterpret_cast<uintptr_t>(x) & 15u) != 0) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "%s rows must be given, 16-byte aligned", what);
     }
     if (heads == 0 || heads % c.kv_heads != 0) {

@@ -294,7 +294,8 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     jfb_status st = check_cache(cache);
     if (st.code == JFB_STATUS_OK) st = check_batch(batch, false);
     if (st.code != JFB_STATUS_OK) return st;
-    if (mass == nullptr || keep == nullptr || kv_len_out == nullptr || mass_out == nullptr || page_table_out == nullptr) {
+    if (batch->sequences > 0 &&
+        (mass == nullptr || keep == nullptr || kv_len_out == nullptr || mass_out == nullptr || page_table_out == nullptr)) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict operands are required");
     }
     if (budget == 0 || recent > budget || budget > 0x7fffffffu) {
@@ -304,6 +305,7 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
         uint64_t(table_out_width) * cache->page_size < budget) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: mass_out or page_table_out does not hold %u keys", budget);
     }
+    if (batch->sequences == 0) return status_ok();
     if (mass_out == mass && mass_out_stride != mass_stride) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: mass in place needs one stride");
     }
@@ -313,7 +315,6 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     if (uint64_t(batch->sequences) * cache->kv_heads > 0x3fffffffull) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: too many sequences and heads");
     }
-    if (batch->sequences == 0) return status_ok();
     EvictParams p;
     p.view = make_view(*cache, *batch, 0, 1, 0, error_flag);
     p.mass = mass;

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                 for (uint32_t j = 0; j < uint32_t(kTileKeys) / 32; ++j) {  // zeros for new slots and behind the keys
                     const uint32_t i = j * 32 + lane, k = t * kTileKeys + i;
                     const bool held = p.mass_in != nullptr && k < limit && int64_t(k) < first;
-                    const float * src = held ? p.mass_in + line + k : p.lse;
+                    const float * src = held ? p.mass_in + line + k : p.mass_out;
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + i * 4), "l"(src), "r"(held ? 4u : 0u) : "memory");
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full + st)) : "memory");
@@ -254,16 +254,16 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     if (st.code == JFB_STATUS_OK) st = check_batch(batch, true);
     if (st.code == JFB_STATUS_OK) st = check_rows("jfb_paged_attention_mass", q, q_stride, rows, heads, *cache);
     if (st.code != JFB_STATUS_OK) return st;
-    if (lse == nullptr || mass_out == nullptr || mass_stride == 0) {
+    if ((lse == nullptr && rows > 0) || (mass_out == nullptr && batch->sequences > 0) || mass_stride == 0) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention_mass needs lse and mass_out");
     }
     if (!(scale > 0.0f) || scale > 3.0e38f || window > 0x7fffffffu) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT,
                             "jfb_paged_attention_mass needs a positive finite scale and a window below 2^31");
     }
+    if (batch->sequences == 0) return status_ok();
     const Device device = current_device();
     if (device.sms == 0) return status_error(JFB_STATUS_CUDA_ERROR, "jfb_paged_attention_mass: no usable device");
-    if (batch->sequences == 0) return status_ok();
     MassParams p;
     p.view = make_view(*cache, *batch, rows, heads / cache->kv_heads, window, error_flag);
     p.view.slots = mass_stride;

@@ -340,8 +340,8 @@ extern "C" jfb_status jfb_rope_paged_append(const void * q, const void * k, cons
     jfb_status st = check_cache(cache);
     if (st.code == JFB_STATUS_OK) st = check_batch(batch, true);
     if (st.code != JFB_STATUS_OK) return st;
-    if (q == nullptr || k == nullptr || v == nullptr || pos == nullptr || q_out == nullptr || rope == nullptr ||
-        rope->freq == nullptr) {
+    if (rope == nullptr || rope->freq == nullptr ||
+        (rows > 0 && (q == nullptr || k == nullptr || v == nullptr || pos == nullptr || q_out == nullptr))) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_rope_paged_append operands are required");
     }
     if (in_dtype > JFB_DTYPE_BF16) return status_error(JFB_STATUS_INVALID_ARGUMENT, "unknown input dtype %u", in_dtype);
@@ -354,7 +354,7 @@ extern "C" jfb_status jfb_rope_paged_append(const void * q, const void * k, cons
         q_out_stride >= most || k_stride >= most || v_stride >= most) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_rope_paged_append row strides do not fit the heads");
     }
-    if (q == q_out && (in_dtype != cache->dtype || q_stride != q_out_stride)) {
+    if (q == q_out && rows > 0 && (in_dtype != cache->dtype || q_stride != q_out_stride)) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "q in place needs the cache's dtype and one stride");
     }
     const uint32_t in_bytes = in_dtype == JFB_DTYPE_F32 ? 4 : 2;

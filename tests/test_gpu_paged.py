@@ -537,6 +537,28 @@ def kept_slots(weights, n, budget, recent):
     return sorted(early[:budget - recent] + list(range(n - recent, n)))
 
 
+def test_empty_batches(P):
+    """No new rows: only the masses go over. No sequences: nothing happens."""
+    case = Case(P, [0, 0], [50, 200])
+    flag, ws = case.error, P.attention_workspace()
+    empty = torch.empty(0, 4, 128, dtype=torch.float16, device="cuda")
+    kv = torch.empty(0, 2, 128, dtype=torch.float16, device="cuda")
+    lse, pos = torch.empty(0, 4, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
+    rope = P.Rope(torch.ones(64, dtype=torch.float64, device="cuda"))
+    before = torch.rand(2, 2, 210, device="cuda", generator=case.g)
+    got = torch.full_like(before, 9.0)
+    nobody = P.PagedBatch(case.q_start[:1], case.kv_len[:0], case.table[:0])
+    for batch, x, y in ((case.batch, before, got), (nobody, before[:0], got[:0])):
+        P.rope_append(empty, kv, kv, pos, rope, case.cache, batch, empty, error_flag=flag)
+        P.attention(empty, case.cache, batch, empty, ws, lse=lse, error_flag=flag)
+        P.attention_mass(empty, lse, case.cache, batch, y, mass_in=x, error_flag=flag)
+    P.evict(before[:0], case.cache, nobody, torch.empty(0, 2, 16, dtype=torch.int32, device="cuda"), case.kv_len[:0], recent=0)
+    torch.cuda.synchronize()
+    for b, k in enumerate(case.kv):
+        assert torch.equal(got[b, :, :k], before[b, :, :k]) and torch.all(got[b, :, k:] == 9.0)
+    assert int(flag) == 0
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("kv,budget,recent,kv_heads,hd,ps", [
     ([1], 1, 0, 2, 128, 16), ([700], 512, 64, 2, 128, 16), ([5, 300, 64, 65, 0], 64, 10, 4, 128, 8), ([200, 90], 33, 33, 1, 96, 32),

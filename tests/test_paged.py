@@ -187,6 +187,18 @@ def test_empty_calls_need_no_device(P):
     assert rope_call(P, cache(P), batch(P), rows=0).code == 0
 
 
+def test_empty_arrays_may_be_absent(P):
+    """Tensors without elements have no address: no sequences, or no rows."""
+    none = batch(P, q_start=None, kv_len=None, page_table=None, sequences=0)
+    assert rope_call(P, cache(P), none).code == 0
+    assert attention_call(P, cache(P), none).code == 0
+    assert mass_call(P, cache(P), none, out=None).code == 0
+    assert evict_call(P, cache(P), none, mass=None, mass_out=None, keep=None, kv_out=None, table=None).code == 0
+    assert rope_call(P, cache(P), batch(P), rows=0, q=None, k=None, v=None, pos=None, q_out=None).code == 0
+    assert attention_call(P, cache(P), batch(P), rows=0, q=None, out=None).code == 0
+    refused(attention_call(P, cache(P), batch(P), rows=0, heads=3))
+
+
 def test_python_refuses_host_tensors(P):
     pool = torch.zeros(4, 16, 2, 128, dtype=torch.float16)
     with pytest.raises(P.InvalidArgument):
