@@ -75,10 +75,12 @@ typedef struct jfb_paged_cache {
  * call's row arrays are sequence b's new tokens (possibly none), in order; its
  * keys are slots 0 .. kv_len[b] - 1, slot j lying in page
  * page_table[b * table_stride + j / page_size]. kv_len counts the new tokens:
- * they hold the last slots, so new token i of n has slot kv_len - n + i. Page
- * ids beyond the last used one are not read. Rows at and behind
- * q_start[sequences] belong to no sequence: nothing of theirs is read or
- * written. */
+ * they hold the last slots, so new token i of n has slot kv_len - n + i. A
+ * length beyond the table, or beyond 2^31 - 1024, is cut to it. Page ids beyond
+ * the last used one are not read. Sequences may share pages that no call writes
+ * (a common prefix). Rows at and behind q_start[sequences] belong to no
+ * sequence: nothing of theirs is used or written. The arrays must not change
+ * while a call that was given them runs. */
 typedef struct jfb_paged_batch {
     const int32_t * q_start;     /* [sequences + 1] */
     const int32_t * kv_len;      /* [sequences] */
@@ -143,7 +145,8 @@ uint64_t jfb_paged_attention_workspace_bytes(void);
  * b at slot p sees the slots j <= p, with window > 0 only j > p - window:
  *     x_j = scale * q . k_j,   out = sum_j exp(x_j - lse) v_j,
  *     lse = log sum_j exp(x_j).
- * Query head h reads kv head h / (heads / kv_heads). q and out have the
+ * scale is positive, up to 1e38. Query head h reads kv head
+ * h / (heads / kv_heads). q and out do not overlap; they have the
  * cache's dtype, rows of heads x head_dim at their strides (elements,
  * multiples of 8, 16-byte aligned pointers); lse (may be NULL) is f32
  * [rows][heads]. Scores, the softmax's maximum and sum and the output sums are
@@ -184,7 +187,8 @@ jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride, uint32_t 
  * [sequences][kv_heads][budget] receives the kept slots in order, -1 behind
  * them, and kv_len_out [sequences] the new lengths, min(kv_len, budget).
  * page_table_out is either the batch's own page_table (the compaction is in
- * place; mass_out may be mass, kv_len_out kv_len) or shares no page with it.
+ * place; mass_out may be mass, kv_len_out kv_len) or shares no page with it;
+ * either way no page stands in it twice.
  * A length beyond the table or mass_stride is cut to it; a kept row with a
  * page id outside the pool on either side is not moved (error bit 0). The
  * batch's q_start is not read. */

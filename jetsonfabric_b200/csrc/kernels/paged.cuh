@@ -47,12 +47,19 @@ struct Sequence {
     uint32_t q0, count, kv;
 };
 
-__device__ __forceinline__ uint32_t cut_length(const View & v, int32_t len, bool & bad) {
+// Keys that a sequence can hold: what the table covers, and slots whose tile
+// ends below 2^31 (slot arithmetic is signed).
+__device__ __forceinline__ uint32_t capacity(const View & v) {
     const uint64_t cap = uint64_t(v.table_width) * v.page_size;
+    return cap < 0x7ffffc00u ? uint32_t(cap) : 0x7ffffc00u;
+}
+
+__device__ __forceinline__ uint32_t cut_length(const View & v, int32_t len, bool & bad) {
+    const uint32_t cap = capacity(v);
     if (len < 0) bad = true;
     const uint32_t n = len < 0 ? 0u : uint32_t(len);
     if (n > cap) bad = true;
-    return n > cap ? uint32_t(cap) : n;
+    return n > cap ? cap : n;
 }
 
 __device__ __forceinline__ Sequence load_sequence(const View & v, uint32_t b) {

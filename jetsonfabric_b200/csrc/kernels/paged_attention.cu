@@ -534,8 +534,8 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     if (st.code == JFB_STATUS_OK) st = check_rows("jfb_paged_attention", q, q_stride, rows, heads, *cache);
     if (st.code == JFB_STATUS_OK) st = check_rows("jfb_paged_attention", out, out_stride, rows, heads, *cache);
     if (st.code != JFB_STATUS_OK) return st;
-    if (!(scale > 0.0f) || scale > 3.0e38f || window > 0x7fffffffu) {
-        return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a positive finite scale and a window below 2^31");
+    if (!(scale > 0.0f) || scale > 1.0e38f || window > 0x7fffffffu) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a positive scale up to 1e38 and a window below 2^31");
     }
     if (rows == 0 || batch->sequences == 0) return status_ok();
     const Device device = current_device();

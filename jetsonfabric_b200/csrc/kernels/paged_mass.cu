@@ -257,9 +257,9 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     if ((lse == nullptr && rows > 0) || (mass_out == nullptr && batch->sequences > 0) || mass_stride == 0) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention_mass needs lse and mass_out");
     }
-    if (!(scale > 0.0f) || scale > 3.0e38f || window > 0x7fffffffu) {
+    if (!(scale > 0.0f) || scale > 1.0e38f || window > 0x7fffffffu) {
         return status_error(JFB_STATUS_INVALID_ARGUMENT,
-                            "jfb_paged_attention_mass needs a positive finite scale and a window below 2^31");
+                            "jfb_paged_attention_mass needs a positive scale up to 1e38 and a window below 2^31");
     }
     if (batch->sequences == 0) return status_ok();
     const Device device = current_device();

@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const RopeParams 
             if (in) {
                 // from the length as it is, not as the table cuts it: that slot holds another key
                 const int64_t j = int64_t(v.kv_len[lo]) - s.count + (r - s.q0);
-                const bool there = j >= 0 && uint64_t(j) >> v.page_shift < v.table_width;
+                const bool there = j >= 0 && j < int64_t(capacity(v));
                 const int32_t page = there ? v.table[uint64_t(lo) * v.table_stride + (uint64_t(j) >> v.page_shift)] : -1;
                 if (page >= 0 && uint32_t(page) < v.pages) {
                     at = uint64_t(page) * v.page_stride + (uint64_t(j) & (v.page_size - 1)) * v.token_stride;

@@ -325,7 +325,8 @@ def evict(mass, cache: PagedCache, batch: PagedBatch, keep, kv_len_out, recent: 
     and the heaviest others, ties to the lowest slot (jfb_paged_evict). keep int32
     [sequences, kv_heads, budget] receives the kept slots, kv_len_out [sequences]
     the new lengths. Without mass_out the masses move in place, without
-    page_table_out (which must share no page with the batch's) the cache does."""
+    page_table_out (which must share no page with the batch's) the cache does; no
+    page may then belong to two sequences."""
     _on(batch, cache)
     slots = _masses(mass, batch, cache, "mass")
     mass_out = mass if mass_out is None else mass_out

@@ -262,6 +262,80 @@ def test_bad_lengths_are_cut_and_flagged(P):
     assert torch.all(out[1] == 0) and torch.all(lse[1] == -math.inf)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_slots_near_the_largest(P, new):
+    """A context of 2^31 - 1024 keys whose table repeats one page, seen through a window; more is cut."""
+    case = Case(P, [new], [1024], kv_heads=1, page_size=1024)
+    table = case.table.expand(1, 1 << 21).contiguous()
+    kv_len = torch.tensor([2 ** 31 - 1], dtype=torch.int32).cuda()
+    case.batch = P.PagedBatch(case.q_start, kv_len, table)
+    q = case.queries(4)
+    out, lse = run_attention(P, case, q, 300)
+    assert int(case.error) == P.ERROR_RANGE
+    check_attention(case, q, out, lse, 128 ** -0.5, 300)  # the last slots are the page's last
+    kv_len.fill_(2 ** 31 - 1024)
+    again, lse2 = run_attention(P, case, q, 300)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    k = rand(case.g, new, 1, 128)
+    pos = torch.arange(new, dtype=torch.int32, device="cuda")
+    P.rope_append(q, k.half(), k.half(), pos, P.Rope(torch.zeros(64, dtype=torch.float64, device="cuda")), case.cache, case.batch,
+                  torch.empty_like(q))
+    torch.cuda.synchronize()
+    page, place = case.where(0, torch.arange(1024 - new, 1024))
+    assert torch.equal(case.k_pool[page, place], k.half())
+
+
+@pytest.mark.parametrize("new,kv,heads,kvh,hd", [([9], [200], 132, 1, 64), ([40, 1], [90, 300], 300, 2, 128), ([64], [64], 128, 1, 128)])
+def test_large_groups(P, new, kv, heads, kvh, hd):
+    """More query heads per kv head than a tile has rows, and exactly as many."""
+    case = Case(P, new, kv, kvh, hd)
+    q = case.queries(heads)
+    out, lse = run_attention(P, case, q)
+    check_attention(case, q, out, lse, hd ** -0.5, 0)
+    before = torch.rand(len(kv), kvh, max(kv), device="cuda", generator=case.g)
+    got = torch.empty_like(before)
+    P.attention_mass(q, lse, case.cache, case.batch, got, mass_in=before, error_flag=case.error)
+    torch.cuda.synchronize()
+    check_mass(case, q, lse, before, got, hd ** -0.5, 0)
+    assert int(case.error) == 0
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_a_pool_of_one_page_shared_by_sequences(P, new):
+    case = Case(P, [new, 0, new], [60, 64, 64], kv_heads=1, hd=64, page_size=64)
+    pool = case.k_pool[:1].clone()
+    pool[0] = rand(case.g, 64, 1, 64, dtype=case.dtype)
+    case.cache = P.PagedCache(pool, pool)
+    case.batch = P.PagedBatch(case.q_start, case.kv_len, torch.zeros(3, 1, dtype=torch.int32, device="cuda"))
+    case.keys = case.values = [pool[0, :k] for k in case.kv]
+    q = case.queries(8)
+    out, lse = run_attention(P, case, q)
+    check_attention(case, q, out, lse, 0.125, 0)
+    assert int(case.error) == 0
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_masses_shorter_than_the_keys(P, new):
+    """Only the slots that have a mass get one, and the cut is flagged."""
+    case = Case(P, [new, new], [400, 150])
+    q = case.queries(8)
+    out, lse = run_attention(P, case, q)
+    before = torch.rand(2, 2, 170, device="cuda", generator=case.g)
+    got = torch.full_like(before, 9.0)
+    P.attention_mass(q, lse, case.cache, case.batch, got, mass_in=before, error_flag=case.error)
+    wide = torch.full((2, 2, 400), 9.0, device="cuda")
+    wide[:, :, :170] = before
+    full = torch.full_like(wide, 9.0)
+    P.attention_mass(q, lse, case.cache, case.batch, full, mass_in=wide)
+    torch.cuda.synchronize()
+    assert int(case.error) == P.ERROR_RANGE
+    check_mass(case, q, lse, wide, full, 128 ** -0.5, 0)
+    # the same positive terms, new x 4 heads and `before`, in an order that the items' cut may
+    # change: each sum of n of them is off by at most n U of itself
+    assert torch.allclose(got, full[:, :, :170], rtol=2 * (4 * new + 8) * U, atol=0)
+    assert torch.all(got[1, :, 150:] == 9.0)
+
+
 @pytest.mark.parametrize("new,kv,heads", [([1] * 3, [900, 20, 400], 16), ([200, 90], [700, 90], 16)])
 def test_captured_calls_follow_new_lengths(P, new, kv, heads):
     """One captured attention replayed after the lengths and the pages changed, next to a second

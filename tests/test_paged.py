@@ -162,7 +162,7 @@ def test_rope_refusals(P, bad):
 
 @pytest.mark.parametrize("call", [attention_call, mass_call])
 @pytest.mark.parametrize("bad", [dict(q=None), dict(q=A + 2), dict(qs=511), dict(qs=256), dict(heads=3), dict(heads=0), dict(scale=0.0),
-                                 dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(window=1 << 31), dict(out=None),
+                                 dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=2e38), dict(window=1 << 31), dict(out=None),
                                  dict(rows=1 << 31)])
 def test_attention_refusals(P, call, bad):
     refused(call(P, cache(P), batch(P), **bad))
