@@ -347,7 +347,13 @@ __device__ __forceinline__ void walk_owners(const WalkOf<Items> & w, uint32_t & 
 // sequence. Up to 128 sequences every warp works it out by itself from
 // registers, one load's latency long: it precedes the first copy of a call
 // that may be all latency. More go through `cost` and two CTA barriers.
-template <int E, class Items>
+//
+// A part of an item costs its joining CTA time as well: with JOIN > 0, the cost
+// of joining one in sixteenths of a unit, only so many workers get work that a
+// share has sqrt(JOIN / 16 x the mean item's units), which makes an item's
+// longest part and the joining take the least time in sum. (Many sequences
+// have many items, and short parts do not arise.)
+template <int E, class Items, uint32_t JOIN = 0>
 __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uint32_t index, uint32_t workers, WalkOf<Items> * walks) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     constexpr uint32_t kOwn = 4;  // sequences per lane
@@ -409,10 +415,21 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
     }
     WalkOf<Items> x = {};
     const uint64_t total = uint64_t(per_head) * v.kv_heads;
+    if (JOIN > 0 && few) {
+        uint32_t items = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < kOwn; ++r) items += Items::count(v, own[r]);
+        items = __reduce_add_sync(0xffffffffu, items);
+        if (items > 0) {
+            const uint32_t least = uint32_t(ceilf(sqrtf(JOIN / 16.0f * float(per_head) / float(items))));
+            if (total < uint64_t(least) * workers) workers = uint32_t(total) < least ? 1u : uint32_t(total) / least;
+        }
+    }
     x.share = divide(total, workers);
     x.extra = uint32_t(total - x.share * workers);
     x.unit = index * x.share + min(index, x.extra);
     x.end = x.unit + x.share + (index < x.extra ? 1 : 0);
+    if (JOIN > 0 && index >= workers) x.unit = x.end;
     if (x.unit < x.end) {
         unsigned long long left = x.unit;
         while (left >= per_head) {
@@ -486,9 +503,9 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
 
 // The same for CTAs that share items: at the first segment that has tiles.
 // False when the CTA has no work.
-template <int E, class Items>
+template <int E, uint32_t JOIN = 0, class Items>
 __device__ __forceinline__ bool walk_begin(const View & v, uint64_t * cost, WalkOf<Items> * walks) {
-    walk_locate<E>(v, cost, blockIdx.x, gridDim.x, walks);
+    walk_locate<E, Items, JOIN>(v, cost, blockIdx.x, gridDim.x, walks);
     WalkOf<Items> * w = walks + (threadIdx.x >> 5);
     if (w->unit >= w->end) return false;
     uint32_t t0, t1;

@@ -30,6 +30,12 @@ namespace paged {
 namespace {
 
 constexpr int kItemTc = 3;  // units of an item's start and end (a prompt of 8192, 28/4 heads: 449, 409, 388, 389 us with 1 to 4)
+// A part's joining in sixteenths of a unit, which bounds the parts of an item.
+// One chunk of 16 tokens over 8000 keys, 28/4 heads: 60 us when every SM took
+// a part, and 45, 37, 34, 33 us with 64, 32, 16, 8; 41 with 2 (over 30000 keys
+// 67, and 75, 62, 56, 54, 62). Unrolling the join's loop over the parts did not
+// help: its code runs once, and costs more to fetch than the loads' latency.
+constexpr uint32_t kJoinTc = 8;
 constexpr int kThreadsTc = 384;
 constexpr int kWarpS = 8, kWarpKV = 9, kWarpQ = 10;  // warp 11 issues P V
 constexpr uint32_t kColO = 0, kColP = 256, kColS = 384;  // O_1 is 128 and P_1 64 columns further
@@ -114,7 +120,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
         return;
     }
     Walk * walks = reinterpret_cast<Walk *>(smem + L::kWalk);
-    if (!walk_begin<kItemTc>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
+    if (!walk_begin<kItemTc, kJoinTc>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
     Walk & w = walks[warp];
     __syncthreads();
     // rows that no query fills stay zero (and this may have held the walk's scratch)

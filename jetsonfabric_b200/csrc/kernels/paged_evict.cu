@@ -346,7 +346,7 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     const uint32_t steps = in_place ? 1u : (budget + step - 1) / step;
     if (steps > 65535u) return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: a budget of %u is too large", budget);
     cudaStream_t s = as_stream(stream);
-    // Short lines: a small CTA, whose barriers are cheaper (one sequence of 2000
+    // Short lines: a small CTA, whose barriers are cheaper (one sequence of 700
     // keys, 2 kv heads: 9.3 us with both steps, 12 with 1024 threads).
     cudaError_t e;
     if (p.cached <= kOwn * 256) {
