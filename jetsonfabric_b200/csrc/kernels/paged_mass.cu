@@ -3,6 +3,8 @@
 // The sum runs along the rows, so the keys are the stationary side: an item is
 // one tile of 128 keys of one sequence and kv head, no two CTAs add to the
 // same key, and the order of every sum is fixed.
+#include <algorithm>
+
 #include "paged.cuh"
 #include "paged_attention.cuh"
 #include "paged_mass.cuh"
@@ -281,7 +283,16 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
     const uint32_t group = p.view.group;
-    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences) return launch_mass_tc(*cache, mk, p, device, s);
+    // The tcgen05 kernel from 2 row tiles of 16 a sequence on, if there is work
+    // for it, counted in (16 rows, 128 keys) tiles of the keys that the table can hold. This kernel /
+    // the tcgen05 kernel at 28/4 heads, in us: 64 sequences of 1150 keys with 4, 8, 16 new tokens 58/86,
+    // 99/86, 185/87; 4 of them with 8, 16, 40: 11/16, 16/16 (1008 tiles), 31/19; one of 8000 with 4, 8, 16:
+    // 11/15 (441), 16/15 (882), 26/15.
+    const uint64_t keys = std::min(uint64_t(batch->table_width) * cache->page_size, mass_stride);
+    const double tiles = double((uint64_t(rows) * group + 15) / 16) * cache->kv_heads * double((keys + kTileKeys - 1) / kTileKeys);
+    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences && tiles > 700) {
+        return launch_mass_tc(*cache, mk, p, device, s);
+    }
     if (cache->head_dim <= 64) {
         return half ? launch_rows<__half, 64>(mk, p, device, s) : launch_rows<__nv_bfloat16, 64>(mk, p, device, s);
     }

@@ -138,6 +138,33 @@ __device__ __forceinline__ bool next_item(const View & v, KeyTileWalk * w) {
     if ((threadIdx.x & 31) == 0) more = step_item(v, *w);
     return __shfl_sync(0xffffffffu, more, 0) != 0;
 }
+// Whether the CTAs of a cluster take items of their own: where that makes the
+// busiest one's time, counted in steps and 4 for an item's start and end (the
+// longest item and as many mean ones as come before it), smaller than sharing
+// each item's steps. Many sequences have many items.
+__device__ __forceinline__ bool items_apart(const View & v, uint32_t ctas) {
+    if (v.sequences > 128) return true;
+    const uint32_t lane = threadIdx.x & 31, tokens = v.item_rows / v.group;
+    float items = 0.0f, steps = 0.0f, most = 0.0f;
+    for (uint32_t b = lane; b < v.sequences; b += 32) {
+        const Sequence s = load_sequence(v, b);
+        const float n = float(KeyItems::count(v, s)), of = float((s.count + tokens - 1) / tokens);
+        items += n;
+        steps += n * of;
+        most = fmaxf(most, of);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        items += __shfl_xor_sync(0xffffffffu, items, d);
+        steps += __shfl_xor_sync(0xffffffffu, steps, d);
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    }
+    const float mean = steps / fmaxf(items, 1.0f), all = items * float(v.kv_heads);
+    const auto time = [&](float workers, float sharing) {
+        return fmaxf(ceilf(all / workers) - 1.0f, 0.0f) * (4.0f + ceilf(mean / sharing)) + 4.0f + ceilf(most / sharing);
+    };
+    return time(float(ctas), 1.0f) < time(float(ctas / kCluster), float(kCluster));
+}
 // Whether the item has keys in its second tile.
 __device__ __forceinline__ bool two_key_tiles(const View & v, const KeyTileWalk & w) {
     return KeyItems::limit(v, w.s) > w.tile * kItemKeys + kTileKeys;
@@ -185,7 +212,8 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
     pdl_wait();
     const View & v = p.view;
     KeyTileWalk * walks = reinterpret_cast<KeyTileWalk *>(smem + L::kWalk);
-    walk_locate<kItemMass>(v, reinterpret_cast<uint64_t *>(smem), blockIdx.x / kCluster, gridDim.x / kCluster, walks);
+    const uint32_t share = items_apart(v, gridDim.x) ? 1u : kCluster, part = share == 1 ? 0u : rank;  // CTAs of an item
+    walk_locate<kItemMass>(v, reinterpret_cast<uint64_t *>(smem), blockIdx.x / share, gridDim.x / share, walks);
     if (lane == 0) {
         KeyTileWalk & start = walks[warp];
         if (start.unit < start.end) {
@@ -211,7 +239,7 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
         ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, flags, v.error));
         return ok;
     };
-    // this CTA's steps of an item are row tiles k.first + rank, + kCluster, ...; s counts its steps over all items
+    // this CTA's steps of an item are row tiles k.first + part, + share, ...; s counts its steps over all items
     uint32_t s = 0;
 
     if (warp == kWarpLoad) {
@@ -225,7 +253,7 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             if (item > 0 && !wait(k_free, (item - 1) & 1)) break;
             tile_issue<D>(v, k0, &maps.k, w.kv_head, smem_u32(smem), k_full);
             tile_issue<D>(v, k1, &maps.k, w.kv_head, smem_u32(smem) + kTileBytes<D>, k_full);
-            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+            for (uint32_t i = part; i < w.k.tiles; i += share, ++s) {
                 const uint32_t st = s % L::kQStages;
                 if (s >= L::kQStages && !wait(q_free + st, (s / L::kQStages - 1) & 1)) break;
                 if (lane == 0) {
@@ -250,7 +278,7 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
         for (bool more = work; ok && more; ++item) {
             const bool two = two_key_tiles(v, w);
             if (!wait(k_full, item & 1)) break;
-            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+            for (uint32_t i = part; i < w.k.tiles; i += share, ++s) {
                 const uint32_t st = s % L::kQStages, q_addr = smem_u32(smem) + L::kQ + st * kTileBytes<D>;
                 if (!wait(q_full + st, (s / L::kQStages) & 1)) break;
                 for (uint32_t x = 0; x <= (two ? 1u : 0u); ++x) {
@@ -279,7 +307,7 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
         }
         for (bool more = work; ok && more;) {
             const int64_t first = int64_t(w.s.kv) - w.s.count;
-            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+            for (uint32_t i = part; i < w.k.tiles; i += share, ++s) {
                 const uint32_t st = s % kLseRing, token0 = (w.k.first + i) * tokens;
                 float2 x[4];
 #pragma unroll
@@ -310,21 +338,27 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
             const int64_t first = int64_t(w.s.kv) - w.s.count;
             const uint32_t key0 = w.tile * kItemKeys + x * kTileKeys, at = key0 + key;
             const bool mine = x == 0 || two_key_tiles(v, w);
+            const uint32_t first_tile = w.k.first, tiles = w.k.tiles, rows = w.s.count;
+            // this thread's result, and what was there before: asked for now, like the next item, for their latency
+            const bool writes = part == 0 && half == 0 && mine && at < KeyItems::limit(v, w.s);
+            const uint64_t to = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots + at;
+            const float before = writes && p.mass_in != nullptr && int64_t(at) < first ? p.mass_in[to] : 0.0f;
+            more = next_item(v, &w);
             float total = 0.0f;
-            for (uint32_t i = rank; i < w.k.tiles; i += kCluster, ++s) {
+            for (uint32_t i = part; i < tiles; i += share, ++s) {
                 const uint32_t st = s % kLseRing;
                 // after a wait that gave up the steps are skipped; the warps still meet at the barriers below
                 if (!wait(r_full + st, (s / kLseRing) & 1)) continue;
                 if (mine) {
                     const uint32_t buf = 2 * x + (n & 1);
-                    const uint32_t token0 = (w.k.first + i) * tokens;
+                    const uint32_t token0 = (first_tile + i) * tokens;
                     const int64_t pos0 = first + token0, pos1 = pos0 + tokens - 1;
-                    const bool edge = token0 + tokens > w.s.count || pos0 < int64_t(key0) + kTileKeys - 1 ||
+                    const bool edge = token0 + tokens > rows || pos0 < int64_t(key0) + kTileKeys - 1 ||
                                       (v.window > 0 && int64_t(key0) <= pos1 - int64_t(v.window));
                     if (!wait(s_full + buf, (n / 2) & 1)) continue;
                     ++n;
                     tc_fence_after();
-                    const float4 * rows = reinterpret_cast<const float4 *>(ring + st * 128 + half * 64);
+                    const float4 * data = reinterpret_cast<const float4 *>(ring + st * 128 + half * 64);
                     float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -339,7 +373,7 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                         if (edge) {
 #pragma unroll
                             for (int j = 0; j < 32; j += 2) {
-                                const float4 r = rows[c * 16 + j / 2];
+                                const float4 r = data[c * 16 + j / 2];
                                 float e0, e1;
                                 fma2(e0, e1, y[j], y[j + 1], scale2, r.x, r.z);
                                 e0 = exp2_approx(e0);
@@ -352,7 +386,7 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; j += 2) {
-                                const float4 r = rows[c * 16 + j / 2];
+                                const float4 r = data[c * 16 + j / 2];
                                 float e0, e1;
                                 fma2(e0, e1, y[j], y[j + 1], scale2, r.x, r.z);
                                 add2(a0, a1, exp2_approx(e0), exp2_approx(e1));
@@ -370,11 +404,12 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                 if (half) halves[q * 128] = total;
                 if (x == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
                 else asm volatile("bar.sync 2, 256;" ::: "memory");
-                if (half) {
-                    more = next_item(v, &w);
+                if (half) continue;
+                total += halves[q * 128];
+                if (share == 1) {
+                    if (ok && writes) p.mass_out[to] = before + total;
                     continue;
                 }
-                total += halves[q * 128];
                 if (turn > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(sum_free + q, (turn - 1) & 1, flags, v.error));
                 if (ok) {
                     remote_store(sums + (q * kCluster + rank) * 128 + key, 0, total);
@@ -384,12 +419,10 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                 }
                 if (rank == 0) {
                     ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(sum_full + q, turn & 1, flags, v.error));
-                    if (ok && at < KeyItems::limit(v, w.s)) {
+                    if (ok && writes) {
                         float sum = 0.0f;
 #pragma unroll
                         for (uint32_t r = 0; r < kCluster; ++r) sum += sums[(q * kCluster + r) * 128 + key];
-                        const uint64_t to = (uint64_t(w.b) * v.kv_heads + w.kv_head) * v.slots + at;
-                        const float before = p.mass_in != nullptr && int64_t(at) < first ? p.mass_in[to] : 0.0f;
                         p.mass_out[to] = before + sum;
                     }
                     if (x == 0) asm volatile("bar.sync 3, 128;" ::: "memory");
@@ -397,7 +430,6 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
                     if ((warp & 3) == 0 && lane < kCluster) remote_arrive(sum_free + q, lane);
                 }
             }
-            more = next_item(v, &w);
         }
     }
     tc_fence_before();
