@@ -9,9 +9,14 @@
 //                   as the 16-bit A operand, results out;
 //   warps 8, 11     the MMAs, S_x = Q_x K^T from one and O_x += P_x V from the
 //                   other, each waiting only for what its own chain needs;
-//   warp 9          K and V tiles, page by page through TMA, into one ring;
-//   warp 10         the queries of the next item, as soon as the last scores of
-//                   this one are formed.
+//   warps 9, 10     K and V tiles, page by page through TMA (one warp for both
+//                   was slower where pages are small, a copy per page and 64
+//                   columns: 104 us against 93 for chunks of 65 to 519 tokens at
+//                   16 tokens a page, 90 against 90 at 64); 10 also the queries of
+//                   the next item, as soon as the last scores of this one are formed.
+// K and V have a ring each. In one ring of five tiles a slot would hold them by
+// turns, and the warp that waits for K alone, by parity, could take the end of
+// an earlier phase than the V tile's, still on its way, for its own.
 // Tensor memory (512 columns): O_0 and O_1 of 128 f32 columns, P_0 and P_1 of
 // 64 columns of 16-bit pairs, and one S of 128. The row tiles take turns with
 // S: a softmax thread moves its row into registers at once, which frees S for
@@ -37,13 +42,15 @@ constexpr int kItemTc = 3;  // units of an item's start and end (a prompt of 819
 // help: its code runs once, and costs more to fetch than the loads' latency.
 constexpr uint32_t kJoinTc = 8;
 constexpr int kThreadsTc = 384;
-constexpr int kWarpS = 8, kWarpKV = 9, kWarpQ = 10;  // warp 11 issues P V
+constexpr int kWarpS = 8, kWarpK = 9, kWarpV = 10;  // warp 11 issues P V
 constexpr uint32_t kColO = 0, kColP = 256, kColS = 384;  // O_1 is 128 and P_1 64 columns further
 constexpr float kSlack = 8.0f;                           // growth of the maximum (log 2) that a rescale waits for
 
 template <int D>
 struct TcSmem {
-    static constexpr int kStages = D == 128 ? 5 : 10;
+    // the rings, one after the other (3 and 2: a prompt of 8192 at 28/4 heads 416 us, 411 with 2 and 3)
+    static constexpr int kStagesK = D == 128 ? 2 : 5, kStagesV = D == 128 ? 3 : 5;
+    static constexpr int kStages = kStagesK + kStagesV;
     static constexpr uint32_t kQ = 2 * kTileBytes<D>;
     static constexpr uint32_t kBars = kQ + kStages * kTileBytes<D>;
     static constexpr uint32_t kNumBars = 2 * kStages + 11;  // full, empty; s, p, o, q full and q free of both row tiles; S free
@@ -140,8 +147,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, flags, v.error));
             return ok;
         };
-        if (warp == kWarpKV) {
-            uint32_t n = 0;  // ring slots alternate K, V
+        if (warp == kWarpK || warp == kWarpV) {
+            const uint32_t is_v = warp == kWarpV ? 1 : 0;
+            const CUtensorMap * map = is_v ? &maps.v : &maps.k;
+            const uint32_t stages = is_v ? L::kStagesV : L::kStagesK, slot0 = is_v ? L::kStagesK : 0;
+            uint32_t n = 0, items[2] = {0, 0};
             do {
                 uint32_t t0, t1;
                 walk_segment<kItemTc>(w, t0, t1);
@@ -152,26 +162,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                     return tile_pages(v, row, key0, kv <= key0 ? key0 : min(kv, key0 + uint32_t(kTileKeys)));
                 };
                 TileLoad next = pages_of(t0);
-                for (uint32_t t = t0; ok && t < t1; ++t) {
-                    const TileLoad load = next;
-                    if (t + 1 < t1) next = pages_of(t + 1);
-                    for (uint32_t is_v = 0; is_v < 2; ++is_v, ++n) {
-                        const uint32_t st = n % L::kStages, turn = n / L::kStages;
-                        if (turn > 0 && !wait(empty + st, (turn - 1) & 1)) break;
-                        tile_issue<D>(v, load, is_v ? &maps.v : &maps.k, head, ring + st * kTileBytes<D>, full + st);
-                    }
-                }
-            } while (ok && walk_warp_next<kItemTc>(v, &w));
-            if (flags[0]) {
-                for (uint32_t i = n > uint32_t(L::kStages) ? n - L::kStages : 0u; i < n; ++i) {
-                    mbar_drain(full + i % L::kStages, (i / L::kStages) & 1);
-                }
-            }
-        } else if (warp == kWarpQ) {
-            uint32_t items[2] = {0, 0};
-            do {
-                const uint32_t two = two_tiles(w, tokens) ? 1 : 0;
-                for (uint32_t x = 0; ok && x <= two; ++x) {
+                const uint32_t queries = is_v ? (two_tiles(w, tokens) ? 2 : 1) : 0;
+                for (uint32_t x = 0; x < queries; ++x) {
                     if (items[x] > 0 && !wait(q_free + x, (items[x] - 1) & 1)) break;
                     ++items[x];
                     if (lane == 0) {
@@ -183,8 +175,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                     }
                     __syncwarp();
                 }
+                for (uint32_t t = t0; ok && t < t1; ++t, ++n) {
+                    const TileLoad load = next;
+                    if (t + 1 < t1) next = pages_of(t + 1);
+                    const uint32_t turn = n / stages, st = slot0 + n - turn * stages;
+                    if (turn > 0 && !wait(empty + st, (turn - 1) & 1)) break;
+                    tile_issue<D>(v, load, map, head, ring + st * kTileBytes<D>, full + st);
+                }
             } while (ok && walk_warp_next<kItemTc>(v, &w));
             if (flags[0]) {
+                for (uint32_t i = n > stages ? n - stages : 0u; i < n; ++i) mbar_drain(full + slot0 + i % stages, (i / stages) & 1);
                 for (uint32_t x = 0; x < 2; ++x) {
                     if (items[x] > 0) mbar_drain(q_full + x, (items[x] - 1) & 1);
                 }
@@ -196,7 +196,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
             uint32_t tiles[2] = {0, 0}, items[2] = {0, 0};
             uint32_t g = 0;      // key tiles before this segment
             uint32_t moved = 0;  // times S was used
-            auto full_of = [&](uint32_t n) { return wait(full + n % L::kStages, (n / L::kStages) & 1); };
+            const uint32_t stages = scores ? L::kStagesK : L::kStagesV, slot0 = scores ? 0 : L::kStagesK;
+            auto full_of = [&](uint32_t n) { return wait(full + slot0 + n % stages, (n / stages) & 1); };
             do {
                 uint32_t t0, t1;
                 walk_segment<kItemTc>(w, t0, t1);
@@ -206,8 +207,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                 // first slot that the sequence's first new row sees
                 const uint32_t seen_from = v.window > 0 && kv > w.s.count + (v.window - 1) ? kv - w.s.count - (v.window - 1) : 0u;
                 for (uint32_t j = 0; j < steps; ++j) {
-                    const uint32_t x = j & two, n = 2 * (g + (j >> two)) + (scores ? 0 : 1);
-                    const uint32_t addr = ring + (n % L::kStages) * kTileBytes<D>;
+                    const uint32_t x = j & two, n = g + (j >> two), st = slot0 + n % stages;
+                    const uint32_t addr = ring + st * kTileBytes<D>;
                     if (scores) {
                         if (x == 0 && !full_of(n)) break;
                         if (j <= two && !wait(q_full + x, items[x]++ & 1)) break;
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                         }
                         mma_commit(o_full + x);
                     }
-                    if (x == two) mma_commit(empty + n % L::kStages);
+                    if (x == two) mma_commit(empty + st);
                 }
                 g += t1 - t0;
             } while (ok && walk_warp_next<kItemTc>(v, &w));
