@@ -275,6 +275,7 @@ struct WalkOf {
     uint64_t share;        // units of a CTA; the first `extra` have one more
     uint32_t extra;
     uint32_t kv_head, b, tile;
+    uint32_t whole;        // the CTA does the items whose middle lies in its segment, none in parts
     Sequence s;
     typename Items::Part k;
 };
@@ -294,6 +295,11 @@ __device__ __forceinline__ uint32_t cta_of(uint64_t unit, uint64_t share, uint32
 // Key tiles [t0, t1) of the current item that this CTA does.
 template <int E, class Items>
 __device__ __forceinline__ void walk_segment(const WalkOf<Items> & w, uint32_t & t0, uint32_t & t1) {
+    if (E > 0 && w.whole) {
+        t0 = 0;
+        t1 = w.k.tiles;
+        return;
+    }
     const uint64_t a = w.unit - w.item0, b = w.end - w.item0;
     t0 = a > E ? uint32_t(a - E) : 0u;
     t1 = b <= E ? 0u : b - E < w.k.tiles ? uint32_t(b - E) : w.k.tiles;
@@ -318,6 +324,11 @@ __device__ __forceinline__ void walk_item(const View & v, WalkOf<Items> & w) {
 // Moves to the CTA's next segment with tiles; false at the end of its line.
 template <int E, class Items>
 __device__ __forceinline__ bool walk_next(const View & v, WalkOf<Items> & w) {
+    if (E > 0 && w.whole) {
+        if (w.item0 + w.k.tiles + E >= w.end) return false;
+        walk_item<E>(v, w);
+        return w.item0 + (w.k.tiles + E) / 2 < w.end;
+    }
     // what is left of the line, if not tiles of another item, is the start of one
     if (w.item0 + w.k.tiles + 2 * E >= w.end) return false;
     walk_item<E>(v, w);
@@ -351,19 +362,26 @@ __device__ __forceinline__ void walk_owners(const WalkOf<Items> & w, uint32_t & 
 // A part of an item costs its joining CTA time as well: with JOIN > 0, the cost
 // of joining one in sixteenths of a unit, only so many workers get work that a
 // share has sqrt(JOIN / 16 x the mean item's units), which makes an item's
-// longest part and the joining take the least time in sum. (Many sequences
-// have many items, and short parts do not arise.)
-template <int E, class Items, uint32_t JOIN = 0>
+// longest part and the joining take the least time in sum. And where items of
+// much the same length leave the busiest CTA at most `PARTS` units above an
+// even share, none is cut. (Many sequences have many items: neither matters.)
+template <int E, class Items, uint32_t JOIN = 0, uint32_t PARTS = 0>
 __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uint32_t index, uint32_t workers, WalkOf<Items> * walks) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     constexpr uint32_t kOwn = 4;  // sequences per lane
     const bool few = v.sequences <= 32 * kOwn;
+    uint32_t longest = 0;
+    const auto cost_of = [&](const Sequence & s, uint32_t i) {
+        const uint32_t units = Items::part(v, s, i).tiles + E;
+        if (PARTS > 0) longest = max(longest, units);
+        return units;
+    };
     // units of a sequence per lane; the lanes share the items of one that has many
     const auto units_of = [&](const Sequence & s) {
         const uint32_t items = Items::count(v, s);
         unsigned long long units = 0;
         if (items <= 4) {
-            for (uint32_t i = 0; i < items; ++i) units += Items::part(v, s, i).tiles + E;
+            for (uint32_t i = 0; i < items; ++i) units += cost_of(s, i);
         }
         uint32_t many = __ballot_sync(0xffffffffu, items > 4);
         while (many != 0) {
@@ -375,7 +393,7 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
             o.kv = __shfl_sync(0xffffffffu, s.kv, src);
             const uint32_t n = __shfl_sync(0xffffffffu, items, src);
             unsigned long long sum = 0;
-            for (uint32_t i = lane; i < n; i += 32) sum += Items::part(v, o, i).tiles + E;
+            for (uint32_t i = lane; i < n; i += 32) sum += cost_of(o, i);
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (int(lane) == src) units = sum;
@@ -420,7 +438,12 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
 #pragma unroll
         for (uint32_t r = 0; r < kOwn; ++r) items += Items::count(v, own[r]);
         items = __reduce_add_sync(0xffffffffu, items);
-        if (items > 0) {
+        if (PARTS > 0 && items > 0) {
+            longest = __reduce_max_sync(0xffffffffu, longest);
+            const float even = float(total) / float(workers), mean = float(per_head) / float(items);
+            x.whole = ceilf(even / mean) * float(longest) <= even + float(PARTS);
+        }
+        if (items > 0 && !x.whole) {
             const uint32_t least = uint32_t(ceilf(sqrtf(JOIN / 16.0f * float(per_head) / float(items))));
             if (total < uint64_t(least) * workers) workers = uint32_t(total) < least ? 1u : uint32_t(total) / least;
         }
@@ -493,6 +516,14 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
         x.item0 = x.unit - left;
         x.k = Items::part(v, x.s, x.tile);
     }
+    if (PARTS > 0 && x.whole && x.unit < x.end) {
+        // an item whose middle lies before or behind the segment is another CTA's
+        if (x.item0 + (x.k.tiles + E) / 2 < x.unit) {
+            if (x.item0 + x.k.tiles + E >= x.end) x.end = x.unit;
+            else walk_item<E>(v, x);
+        }
+        if (x.item0 + (x.k.tiles + E) / 2 >= x.end) x.end = x.unit;
+    }
     if (lane == 0) walks[warp] = x;
     __syncwarp();
     if (!few) {  // cost may be written again, by copies too
@@ -503,9 +534,9 @@ __device__ __forceinline__ void walk_locate(const View & v, uint64_t * cost, uin
 
 // The same for CTAs that share items: at the first segment that has tiles.
 // False when the CTA has no work.
-template <int E, uint32_t JOIN = 0, class Items>
+template <int E, uint32_t JOIN = 0, uint32_t PARTS = 0, class Items>
 __device__ __forceinline__ bool walk_begin(const View & v, uint64_t * cost, WalkOf<Items> * walks) {
-    walk_locate<E, Items, JOIN>(v, cost, blockIdx.x, gridDim.x, walks);
+    walk_locate<E, Items, JOIN, PARTS>(v, cost, blockIdx.x, gridDim.x, walks);
     WalkOf<Items> * w = walks + (threadIdx.x >> 5);
     if (w->unit >= w->end) return false;
     uint32_t t0, t1;

@@ -41,6 +41,9 @@ constexpr int kItemTc = 3;  // units of an item's start and end (a prompt of 819
 // 67, and 75, 62, 56, 54, 62). Unrolling the join's loop over the parts did not
 // help: its code runs once, and costs more to fetch than the loads' latency.
 constexpr uint32_t kJoinTc = 8;
+// What the parts at a CTA's start and end cost it, in units: up to that much
+// imbalance, items are not cut.
+constexpr uint32_t kPartsTc = 12;
 constexpr int kThreadsTc = 384;
 constexpr int kWarpS = 8, kWarpK = 9, kWarpV = 10;  // warp 11 issues P V
 constexpr uint32_t kColO = 0, kColP = 256, kColS = 384;  // O_1 is 128 and P_1 64 columns further
@@ -127,7 +130,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
         return;
     }
     Walk * walks = reinterpret_cast<Walk *>(smem + L::kWalk);
-    if (!walk_begin<kItemTc, kJoinTc>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
+    if (!walk_begin<kItemTc, kJoinTc, kPartsTc>(v, reinterpret_cast<uint64_t *>(smem), walks)) return;
     Walk & w = walks[warp];
     __syncthreads();
     // rows that no query fills stay zero (and this may have held the walk's scratch)
