@@ -262,19 +262,19 @@ def test_bad_lengths_are_cut_and_flagged(P):
     assert torch.all(out[1] == 0) and torch.all(lse[1] == -math.inf)
 
 
-@pytest.mark.parametrize("new", [1, 40])
-def test_slots_near_the_largest(P, new):
+@pytest.mark.parametrize("new,heads,window", [(1, 4, 300), (40, 4, 300), (1000, 8, 24)])
+def test_slots_near_the_largest(P, new, heads, window):
     """A context of 2^31 - 1024 keys whose table repeats one page, seen through a window; more is cut."""
     case = Case(P, [new], [1024], kv_heads=1, page_size=1024)
     table = case.table.expand(1, 1 << 21).contiguous()
     kv_len = torch.tensor([2 ** 31 - 1], dtype=torch.int32).cuda()
     case.batch = P.PagedBatch(case.q_start, kv_len, table)
-    q = case.queries(4)
-    out, lse = run_attention(P, case, q, 300)
+    q = case.queries(heads)
+    out, lse = run_attention(P, case, q, window)
     assert int(case.error) == P.ERROR_RANGE
-    check_attention(case, q, out, lse, 128 ** -0.5, 300)  # the last slots are the page's last
+    check_attention(case, q, out, lse, 128 ** -0.5, window)  # the last slots are the page's last
     kv_len.fill_(2 ** 31 - 1024)
-    again, lse2 = run_attention(P, case, q, 300)
+    again, lse2 = run_attention(P, case, q, window)
     assert torch.equal(out, again) and torch.equal(lse, lse2)
     k = rand(case.g, new, 1, 128)
     pos = torch.arange(new, dtype=torch.int32, device="cuda")
@@ -861,3 +861,27 @@ def test_evict_beyond_the_selections_cache(P):
             page, place = case.where(b, torch.arange(m))
             assert torch.equal(case.k_pool[page, place], case.keys[b][at])
             assert torch.equal(mass[b, 0, :m], torch.tensor(weights[b][0], device="cuda")[at])
+
+
+@pytest.mark.parametrize("seqs,new,lo,hi,heads,kvh,window", [
+    (150, 20, 100, 400, 8, 2, 0), (150, 30, 40, 300, 6, 1, 50),  # more sequences than a warp's registers hold
+    (64, 12, 200, 700, 28, 4, 0), (30, 40, 300, 310, 16, 2, 0),   # many short items
+    (4, 200, 1000, 1000, 28, 4, 0), (5, 260, 2000, 2001, 10, 2, 128)])  # few of one length
+def test_batches_of_short_chunks(P, seqs, new, lo, hi, heads, kvh, window):
+    """Items that are divided whole, in attention and in the accumulated weights."""
+    host = torch.Generator().manual_seed(seqs + new)
+    kv = torch.randint(lo, hi + 1, (seqs,), generator=host).tolist()
+    case = Case(P, [new - b % 3 for b in range(seqs)], kv, kvh, 128, 32, torch.bfloat16, seed=seqs)
+    q = case.queries(heads)
+    out, lse = run_attention(P, case, q, window)
+    check_attention(case, q, out, lse, 128 ** -0.5, window)
+    before = torch.rand(seqs, kvh, max(kv), device="cuda", generator=case.g)
+    got = torch.full_like(before, 9.0)
+    P.attention_mass(q, lse, case.cache, case.batch, got, mass_in=before, window=window, error_flag=case.error)
+    again = before.clone()
+    P.attention_mass(q, lse, case.cache, case.batch, again, mass_in=again, window=window)
+    torch.cuda.synchronize()
+    check_mass(case, q, lse, before, got, 128 ** -0.5, window)
+    for b, k in enumerate(kv):
+        assert torch.equal(again[b, :, :k], got[b, :, :k]) and torch.all(got[b, :, k:] == 9.0)
+    assert int(case.error) == 0
