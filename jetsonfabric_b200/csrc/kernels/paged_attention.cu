@@ -30,6 +30,10 @@ namespace {
 // scores of the next tile are formed beside the second product of this one.
 // A part of an item that began in another CTA is published by a warp of its
 // own, so that the consumers go on to their next item at once.
+//
+// 6 sequences of 9001 to 65001 keys, 28/4 heads: 79 us (88 % of the measured
+// copy bandwidth); 64 of 1025 to 1280: 37 us (63 %), of which the way to the
+// first tile and the ends are a third.
 
 constexpr int kRowsM = 16;
 constexpr int kItemRows = 0;  // units of an item's start and end

@@ -8,10 +8,13 @@
 // the unit against 1024 of the tensor pipe and 32 KB of queries, so the
 // exponentials bound the time (with 128 keys an item the queries' way from L2
 // did: 250 us for chunks of 700 to 2048 tokens over 2048 to 8000 keys, 16/2 heads;
-// 157 now). A cluster of 4 CTAs takes an item, every fourth
+// 152 to 157 now). A cluster of 4 CTAs takes an item, every fourth
 // step each, and adds the four sums over distributed shared memory: few long
 // items still fill the SMs, and no workspace or order of arrival is involved.
-// Clusters take whole items off the evenly divided line of units
+// Where items are many or their steps few, the CTAs of a cluster take items of
+// their own instead (items_apart; 64 sequences of 1150 keys with 8 new tokens,
+// 28/4 heads: 83 us, 223 shared).
+// Workers take whole items off the evenly divided line of units
 // (walk_locate), each the items whose middle lies in its part.
 //   warps 0-7, 8-15  sums of key tile 0 and 1, two threads per key, each half
 //                    of a step's rows (one thread per key, 8 warps, left the
