@@ -150,14 +150,15 @@ uint64_t jfb_paged_attention_workspace_bytes(void);
  * cache's dtype, rows of heads x head_dim at their strides (elements,
  * multiples of 8, 16-byte aligned pointers); lse (may be NULL) is f32
  * [rows][heads]. Scores, the softmax's maximum and sum and the output sums are
- * f32; the probabilities are rounded to the cache's dtype for the second
- * product. A row that sees no key gets zeros and lse = -inf. Slots behind
- * kv_len and before every row's window are never used, whatever they hold; a
- * key that one row of a sequence's chunk sees must hold finite values of v (a
- * non-finite one may reach rows of the chunk that do not see it). A page
- * id outside the pool reads as zeros, a length beyond the table is cut to it
- * (error bit 0). Results do not depend on timing: partial sums are joined in
- * a fixed order. */
+ * f32; the exponentials are rounded to the cache's dtype for the second
+ * product, where F16 leaves out those below 2^-32 of the row's largest. |x_j|
+ * is meant to stay below 2^26: from there the steps of f32 are 8 and more. A
+ * row that sees no key gets zeros and lse = -inf. Slots behind kv_len and
+ * before every row's window are never used, whatever they hold; a key that one
+ * row of a sequence's chunk sees must hold finite values of v (a non-finite one
+ * may reach rows of the chunk that do not see it). A page id outside the pool
+ * reads as zeros, a length beyond the table is cut to it (error bit 0). Results
+ * do not depend on timing: partial sums are joined in a fixed order. */
 jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uint32_t rows, uint32_t heads, float scale,
                                uint32_t window, const jfb_paged_cache * cache, const jfb_paged_batch * batch,
                                void * out, uint64_t out_stride, float * lse, void * workspace,

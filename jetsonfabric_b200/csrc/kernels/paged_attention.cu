@@ -39,7 +39,6 @@ constexpr int kRowsM = 16;
 constexpr int kItemRows = 0;  // units of an item's start and end
 constexpr int kConsumers = 8;
 constexpr int kThreadsRows = (kConsumers + 3) * 32;  // and K's and V's producers, the publisher
-constexpr float kSlack = 8.0f;  // growth of the maximum (log 2) before the sums are rescaled
 
 template <int D>
 struct RowsSmem {
@@ -345,11 +344,11 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
             for (int e = 0; e < 2; ++e) {
                 mx[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
                 mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * scale2;
+                mx[e] = scaled_top(fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)), scale2);
             }
-            // The sums refer to a maximum that all warps share; it moves only
-            // when some row's has grown by more than 2^8.
-            if (bar_consumers_or(mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
+            // The sums refer to a number that all warps share; it moves only
+            // when some row's maximum has outgrown it.
+            if (bar_consumers_or(outgrown<T>(mx[0], m[0]) || outgrown<T>(mx[1], m[1]))) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     if (tig == 0) tops[warp * kRowsM + grp + 8 * e] = mx[e];
@@ -360,9 +359,9 @@ __global__ void __launch_bounds__(kThreadsRows, 1)
                     float top = -INFINITY;
 #pragma unroll
                     for (int x = 0; x < kConsumers; ++x) top = fmaxf(top, tops[x * kRowsM + grp + 8 * e]);
-                    if (top > m[e] + kSlack) {
-                        const float f = exp2_approx(m[e] - top);
-                        m[e] = top;
+                    if (outgrown<T>(top, m[e])) {
+                        const float next = top - kHeadroom<T>, f = exp2_approx(m[e] - next);
+                        m[e] = next;
                         l[e] *= f;
 #pragma unroll
                         for (int j = 0; j < kTilesN; ++j) {

@@ -2,6 +2,8 @@
 // layout and the checks of row arrays.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace jfb {
@@ -13,6 +15,30 @@ namespace paged {
 // (maximum, sum), f32.
 constexpr uint64_t kCounterBytes = 4096;
 constexpr uint64_t kSlotFloats = 256 * (128 + 2);
+
+// A row's exponentials and sums refer to a number m (log 2) that was its
+// maximum less kHeadroom when it was last set; it is set again when the maximum
+// has come to exceed it by more than kSlack + kHeadroom. As operands of the
+// second product the exponentials are rounded to the cache's type. f16 has
+// nothing below 2^-25, where many weak keys beside a strong one would count in
+// the softmax sum and not in the result (2^17 keys of 2^-25.2 each are 0.3 % of
+// it), so its exponentials start at 2^7: they stay below 2^15 and none above
+// 2^-32 of the row's largest is lost. bf16 has the exponents of f32.
+constexpr float kSlack = 8.0f;
+template <typename T>
+constexpr float kHeadroom = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+
+// The scaled maximum, rounded up: no exponential may lie above it, whatever a
+// step of f32 at its size.
+__device__ __forceinline__ float scaled_top(float score, float scale2) { return __fmul_ru(score, scale2); }
+
+// Whether the reference m of a row whose maximum is `top` has to be set again.
+// The difference of close numbers is exact; it is NaN, hence false, where
+// nothing was seen yet.
+template <typename T>
+__device__ __forceinline__ bool outgrown(float top, float m) {
+    return top - m > kSlack + kHeadroom<T>;
+}
 
 struct AttentionParams {
     View view;
@@ -57,9 +83,9 @@ struct RowsOut {
             if (d + 8 < head_dim) *reinterpret_cast<uint4 *>(out + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
         }
     }
-    // top is the maximum in units of log 2
-    __device__ __forceinline__ void store_lse(const AttentionParams & p, float top, float sum) const {
-        if (out != nullptr && p.lse != nullptr) p.lse[at] = sum != 0.0f ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
+    // m is what the sum refers to, in units of log 2
+    __device__ __forceinline__ void store_lse(const AttentionParams & p, float m, float sum) const {
+        if (out != nullptr && p.lse != nullptr) p.lse[at] = sum != 0.0f ? fmaf(m, kLn2, logf(sum)) : -INFINITY;
     }
 };
 

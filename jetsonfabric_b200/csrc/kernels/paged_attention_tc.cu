@@ -24,9 +24,8 @@
 // are formed during its current exponentials.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
-// one its sums refer to (the sums stay far inside f32's range and the
-// probabilities below 2^8 keep their relative precision), so most tiles touch
-// O not at all.
+// one its sums refer to (the sums stay far inside f32's range, the probabilities
+// inside their type's), so most tiles touch O not at all.
 //
 // The exponentials bound the time: 2048 cycles of their unit for the two row
 // tiles of a key tile, 1024 of the tensor pipe. A prompt of 8192 at 28/4 heads takes 411 us
@@ -53,7 +52,6 @@ constexpr uint32_t kPartsTc = 12;
 constexpr int kThreadsTc = 384;
 constexpr int kWarpS = 8, kWarpK = 9, kWarpV = 10;  // warp 11 issues P V
 constexpr uint32_t kColO = 0, kColP = 256, kColS = 384;  // O_1 is 128 and P_1 64 columns further
-constexpr float kSlack = 8.0f;                           // growth of the maximum (log 2) that a rescale waits for
 
 template <int D>
 struct TcSmem {
@@ -307,15 +305,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1) paged_tc_kernel(const __grid_co
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
-                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale2;
+                const float top = scaled_top(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), scale2);
                 // P and O are free again when the previous product is done
                 if (t > t0) {
                     if (!__all_sync(0xffffffffu, mbar_wait(o_full + x, (n - 1) & 1, flags, v.error))) continue;
                     tc_fence_after();
                 }
-                const bool grow = top > m + kSlack;
+                const bool grow = outgrown<T>(top, m);
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float next = grow ? top : m;
+                    const float next = grow ? top - kHeadroom<T> : m;
                     const float f = grow ? exp2_approx(m - next) : 1.0f;
                     m = next;
                     l0 *= f;

@@ -885,3 +885,66 @@ def test_batches_of_short_chunks(P, seqs, new, lo, hi, heads, kvh, window):
     for b, k in enumerate(kv):
         assert torch.equal(again[b, :, :k], got[b, :, :k]) and torch.all(got[b, :, k:] == 9.0)
     assert int(case.error) == 0
+
+
+def test_weak_keys_beside_a_strong_one_count(P):
+    """f16 caches: the first key outweighs each of 100,000 others by 2^25.2 and holds zeros, so that the result is
+    theirs alone. They must not fall out of the second product: the bound has 2^-32 of the row's largest for what
+    f16 cannot hold, where check_attention has 2^-25."""
+    strong, n = 17.46875, 100000  # 25.2 ln 2, exact in f16; the others score 0
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for hd, seqs, new, heads in ((128, sms, 1, 8), (64, sms, 1, 8), (128, 1, 4736, 8), (64, 1, 4736, 8)):
+        # single tokens over one shared prefix, a sequence per SM; a long chunk over it
+        keys = n + new
+        width = -(-keys // 128)
+        k_pool, v_pool = (torch.zeros(width, 128, 1, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+        g = torch.Generator(device="cuda").manual_seed(hd + new)
+        value = (torch.rand(hd, device="cuda", generator=g) + 0.5).half()
+        v_pool[:] = value
+        k_pool[0, 0, 0, 0], v_pool[0, 0] = strong, 0
+        q = torch.zeros(seqs * new, heads, hd, dtype=torch.float16, device="cuda")
+        q[:, :, 0] = 1.0
+        table = torch.arange(width, dtype=torch.int32, device="cuda").expand(seqs, width).contiguous()
+        q_start = torch.arange(0, seqs * new + 1, new, dtype=torch.int32, device="cuda")
+        kv_len = torch.full((seqs,), keys, dtype=torch.int32, device="cuda")
+        cache, batch = P.PagedCache(k_pool, v_pool), P.PagedBatch(q_start, kv_len, table)
+        out, lse = torch.empty_like(q), torch.empty(seqs * new, heads, device="cuda")
+        P.attention(q, cache, batch, out, P.attention_workspace(), scale=1.0, lse=lse)
+        torch.cuda.synchronize()
+        weak = (keys - new + torch.arange(new, device="cuda", dtype=torch.float64)).repeat(seqs)[:, None, None]
+        total = math.exp(strong) + weak
+        spread = weak / total * value.double()
+        e, d = 2.0 ** -11, 2 * U * (hd + 4) * strong + 4 * U * strong
+        tol = e * spread + spread * (e + 2 * d + 2.0 ** -20 + weak * U) * 1.01
+        tol = tol + 2.0 ** -25 + 2.0 ** -32 * math.exp(strong) / total * weak * value.double()
+        err = (out.double() - spread).abs()
+        assert torch.all(err <= tol), (hd, new, (err / tol).max())
+        want = torch.log(total).squeeze(-1)
+        assert torch.all((lse.double() - want).abs() <= d + 2.0 ** -20 * (1 + want) + weak.squeeze(-1) * U)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 700])
+def test_scores_near_the_largest_meant(P, new, dtype):
+    """Scores up to 2^25, where a step of f32 is 4: the largest takes all the weight, and no exponential leaves its
+    type. Neighbouring scores differ by 2^-10 or more of the largest, their error is below 2^-15."""
+    case = Case(P, [new], [3000], kv_heads=1, dtype=dtype, fill=False)
+    steps = 256 if dtype == torch.float16 else 64  # numbers from 1 to 1.5 that both types hold
+    level = 1 + torch.randint(0, steps, (3000,), device="cuda", generator=case.g) / (2 * steps)
+    level[::500] = 1 + torch.arange(6, device="cuda") / (2 * steps) + 0.5  # now and then a new largest
+    case.keys = [(level[:, None, None] * 64).expand(3000, 1, 128).to(dtype).contiguous()]
+    case.put(0, 0, case.keys[0], case.values[0])
+    q = torch.full((new, 6, 128), 64.0, dtype=dtype, device="cuda")
+    scale = 2.0 ** 25 / (64 * 64 * 128 * 2)
+    out, lse = run_attention(P, case, q, scale=scale)
+    first = 3000 - new
+    for r in range(0, new, 37):
+        seen = level[:first + r + 1]
+        best = seen == seen.max()
+        want = case.values[0][:first + r + 1, 0][best].double().mean(0)
+        spread = case.values[0][:first + r + 1, 0][best].double().abs().mean(0)
+        e = torch.finfo(dtype).eps / 2
+        tol = e * want.abs() + spread * (e + 2.0 ** -20) * 1.01 + 2.0 ** -25
+        assert torch.all((out[r].double() - want).abs() <= tol)
+        top = scale * 64 * 64 * 128 * float(seen.max())
+        assert torch.all((lse[r].double() - top).abs() <= top * 2.0 ** -15)
