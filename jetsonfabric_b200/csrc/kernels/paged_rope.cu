@@ -306,8 +306,19 @@ extern "C" jfb_status jfb_rope_frequencies_host(double * freq, double * factor_o
     const auto index_of = [&](double turns) { return d * std::log(trained / (turns * two_pi)) / (2.0 * std::log(base)); };
     double from = 0.0, to = 1.0;
     if (scaling == JFB_ROPE_SCALING_YARN) {
-        from = std::fmax(std::floor(index_of(high)), 0.0);
-        to = std::fmin(std::ceil(index_of(low)), d - 1.0);
+        // Cut to the pairs there are, the ramp from `high` (kept before it) to `low`
+        // (divided behind it) must not turn round: where every pair makes more
+        // turns than `high` or fewer than `low`, it lies behind or before them all.
+        const double first = std::floor(index_of(high)), last = std::ceil(index_of(low));
+        from = std::fmax(first, 0.0);
+        to = std::fmin(last, d - 1.0);
+        if (base > 1.0 && first > d - 1.0) {
+            from = d;
+            to = d + 1.0;
+        } else if (base > 1.0 && last <= 0.0) {
+            from = -2.0;
+            to = -1.0;
+        }
         if (to == from) to += 1e-3;
     }
     for (uint32_t i = 0; i < rope_dims / 2; ++i) {

@@ -51,6 +51,18 @@ def test_yarn_keeps_fast_pairs_and_divides_slow_ones(P):
         assert math.isclose(freq[i], plain[i] * kept + plain[i] / s * (1 - kept), rel_tol=1e-13)
 
 
+@pytest.mark.parametrize("dims,base,trained", [(16, 100.0, 1e7), (64, 1e4, 1e12), (128, 1e6, 1e16), (64, 1e4, 5.0), (128, 1e6, 0.5),
+                                               (64, 1e4, 1e-3), (16, 0.5, 1e7), (16, 0.5, 1.0), (2, 1e4, 1e8), (2, 1e4, 1.0)])
+def test_yarn_beyond_its_ramp(P, dims, base, trained):
+    """A trained context over which every pair makes more turns than `high` keeps all frequencies; one over which
+    none makes as many as `low` divides all."""
+    plain = base ** (-2.0 * np.arange(dims // 2) / dims)
+    turns = trained * plain / (2 * math.pi)
+    assert turns.min() > 32 or turns.max() < 1
+    freq, _ = P.rope_frequencies(dims, base, "yarn", factor=4.0, trained=trained)
+    assert np.allclose(freq, plain if turns.min() > 32 else plain / 4, rtol=1e-14)
+
+
 def test_bands_blend_by_wavelength(P):
     dims, base, trained, s, lo, hi = 128, 5e5, 8192, 8.0, 1.0, 4.0
     freq, factor = P.rope_frequencies(dims, base, "bands", factor=s, trained=trained, low=lo, high=hi)
