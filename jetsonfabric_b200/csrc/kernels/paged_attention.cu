@@ -528,6 +528,22 @@ extern "C" uint64_t jfb_paged_attention_workspace_bytes(void) {
     return kCounterBytes + uint64_t(current_device().sms) * 2 * kSlotFloats * sizeof(float);
 }
 
+// The tcgen05 kernel takes 128 packed rows at once and 10 us more for its start
+// and end, the other 16: from 2 row tiles of 16 a sequence on, if there is work
+// for it, counted in (16 rows, 128 keys) tiles of the keys that the table can
+// hold. Rows kernel / tcgen05 kernel at 28/4 heads, in us: 64 sequences of
+// 1025 to 1280 keys with 2, 4, 6, 8 new tokens 39/58, 64/58, 89/58, 112/59;
+// one of 1000 keys with 8, 16, 48 tokens 13/24, 13/24, 19/26 (672 tiles); 4 of them with
+// 16, 24, 48: 20/21, 25/26, 40/26 (2688); one of 8000 with 8, 16, 48: 21/32, 28/33, 54/42 (5292).
+extern "C" int jfb_paged_attention_uses_tiles(uint32_t rows, uint32_t heads, uint32_t window, const jfb_paged_cache * cache,
+                                              const jfb_paged_batch * batch) {
+    const uint32_t group = heads / cache->kv_heads;
+    uint64_t keys = uint64_t(batch->table_width) * cache->page_size;
+    if (window > 0) keys = std::min(keys, uint64_t(window) + rows / batch->sequences);
+    const double tiles = double((uint64_t(rows) * group + 15) / 16) * cache->kv_heads * double((keys + kTileKeys - 1) / kTileKeys);
+    return group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences && tiles > 2500;
+}
+
 extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uint32_t rows, uint32_t heads, float scale,
                                           uint32_t window, const jfb_paged_cache * cache, const jfb_paged_batch * batch,
                                           void * out, uint64_t out_stride, float * lse, void * workspace,
@@ -569,20 +585,7 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
     }
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
-    const uint32_t group = p.view.group;
-    // The tcgen05 kernel takes 128 packed rows at once and 10 us more for its
-    // start and end, the other 16: from 2 row tiles of 16 a sequence on, if
-    // there is work for it, counted in (16 rows, 128 keys) tiles of the keys that
-    // the table can hold. Rows kernel / tcgen05 kernel at 28/4 heads, in us: 64 sequences of
-    // 1025 to 1280 keys with 2, 4, 6, 8 new tokens 39/58, 64/58, 89/58, 112/59;
-    // one of 1000 keys with 8, 16, 48 tokens 13/24, 13/24, 19/26 (672 tiles); 4 of them with
-    // 16, 24, 48: 20/21, 25/26, 40/26 (2688); one of 8000 with 8, 16, 48: 21/32, 28/33, 54/42 (5292).
-    uint64_t keys = uint64_t(batch->table_width) * cache->page_size;
-    if (window > 0) keys = std::min(keys, uint64_t(window) + rows / batch->sequences);
-    const double tiles = double((uint64_t(rows) * group + 15) / 16) * cache->kv_heads * double((keys + kTileKeys - 1) / kTileKeys);
-    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences && tiles > 2500) {
-        return launch_attention_tc(*cache, mk, mv, p, device, s);
-    }
+    if (jfb_paged_attention_uses_tiles(rows, heads, window, cache, batch)) return launch_attention_tc(*cache, mk, mv, p, device, s);
     if (cache->head_dim <= 64) {
         return half ? launch_rows<__half, 64>(mk, mv, p, device, s) : launch_rows<__nv_bfloat16, 64>(mk, mv, p, device, s);
     }

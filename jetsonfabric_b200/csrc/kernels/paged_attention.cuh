@@ -106,6 +106,13 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Which kernel a (valid) call takes: 1 the tcgen05 one, 0 the few-rows one.
+// Exported, not part of the interface: the tests make sure of what they cover.
+extern "C" int jfb_paged_attention_uses_tiles(uint32_t rows, uint32_t heads, uint32_t window, const jfb_paged_cache * cache,
+                                              const jfb_paged_batch * batch);
+extern "C" int jfb_paged_attention_mass_uses_tiles(uint32_t rows, uint32_t heads, const jfb_paged_cache * cache,
+                                                   const jfb_paged_batch * batch, uint64_t mass_stride);
+
 // The tcgen05 kernel of paged_attention_tc.cu.
 jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap & k, const CUtensorMap & v, AttentionParams p,
                                const Device & device, cudaStream_t s);

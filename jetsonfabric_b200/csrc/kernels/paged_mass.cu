@@ -250,6 +250,20 @@ jfb_status launch_rows(const CUtensorMap & k, const MassParams & p, const Device
 using namespace jfb;
 using namespace jfb::paged;
 
+// The tcgen05 kernel from 2 row tiles of 16 a sequence on, if there is work for
+// it, counted in (16 rows, 128 keys) tiles of the keys that the table and the
+// masses can hold. Rows kernel / tcgen05 kernel at 28/4 heads, in us: 64
+// sequences of 1150 keys with 4, 8, 16 new tokens 58/86, 99/86, 185/87; 4 of
+// them with 8, 16, 40: 11/16, 16/16 (1008 tiles), 31/19; one of 8000 with 4, 8, 16:
+// 11/15 (441), 16/15 (882), 26/15.
+extern "C" int jfb_paged_attention_mass_uses_tiles(uint32_t rows, uint32_t heads, const jfb_paged_cache * cache,
+                                                   const jfb_paged_batch * batch, uint64_t mass_stride) {
+    const uint32_t group = heads / cache->kv_heads;
+    const uint64_t keys = std::min(uint64_t(batch->table_width) * cache->page_size, mass_stride);
+    const double tiles = double((uint64_t(rows) * group + 15) / 16) * cache->kv_heads * double((keys + kTileKeys - 1) / kTileKeys);
+    return group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences && tiles > 700;
+}
+
 extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride, uint32_t rows, uint32_t heads, float scale,
                                                uint32_t window, const float * lse, const jfb_paged_cache * cache,
                                                const jfb_paged_batch * batch, const float * mass_in, float * mass_out,
@@ -284,17 +298,7 @@ extern "C" jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride
     }
     cudaStream_t s = as_stream(stream);
     const bool half = cache->dtype == JFB_DTYPE_F16;
-    const uint32_t group = p.view.group;
-    // The tcgen05 kernel from 2 row tiles of 16 a sequence on, if there is work
-    // for it, counted in (16 rows, 128 keys) tiles of the keys that the table can hold. This kernel /
-    // the tcgen05 kernel at 28/4 heads, in us: 64 sequences of 1150 keys with 4, 8, 16 new tokens 58/86,
-    // 99/86, 185/87; 4 of them with 8, 16, 40: 11/16, 16/16 (1008 tiles), 31/19; one of 8000 with 4, 8, 16:
-    // 11/15 (441), 16/15 (882), 26/15.
-    const uint64_t keys = std::min(uint64_t(batch->table_width) * cache->page_size, mass_stride);
-    const double tiles = double((uint64_t(rows) * group + 15) / 16) * cache->kv_heads * double((keys + kTileKeys - 1) / kTileKeys);
-    if (group <= 128 && uint64_t(rows) * group > 32ull * batch->sequences && tiles > 700) {
-        return launch_mass_tc(*cache, mk, p, device, s);
-    }
+    if (jfb_paged_attention_mass_uses_tiles(rows, heads, cache, batch, mass_stride)) return launch_mass_tc(*cache, mk, p, device, s);
     if (cache->head_dim <= 64) {
         return half ? launch_rows<__half, 64>(mk, p, device, s) : launch_rows<__nv_bfloat16, 64>(mk, p, device, s);
     }

@@ -15,6 +15,7 @@ Evictions are exact.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import pytest
@@ -948,3 +949,161 @@ def test_scores_near_the_largest_meant(P, new, dtype):
         assert torch.all((out[r].double() - want).abs() <= tol)
         top = scale * 64 * 64 * 128 * float(seen.max())
         assert torch.all((lse[r].double() - top).abs() <= top * 2.0 ** -15)
+
+
+# ---- the tcgen05 kernels at the places where they can go wrong --------------------------------
+
+def by_tiles(P, case, heads, window=0, slots=None):
+    """Whether attention, or with `slots` the accumulated weight, takes the tcgen05 kernel."""
+    L = P._bind()
+    if slots is None:
+        return bool(L.jfb_paged_attention_uses_tiles(case.rows, heads, window, case.cache.ref, case.batch.ref))
+    return bool(L.jfb_paged_attention_mass_uses_tiles(case.rows, heads, case.cache.ref, case.batch.ref, C.c_uint64(slots)))
+
+
+def check_masses_by_tiles(P, case, q, lse, scale, window, slots):
+    before = torch.rand(len(case.kv), case.kvh, slots, device="cuda", generator=case.g)
+    got = torch.full_like(before, 9.0)
+    assert by_tiles(P, case, q.shape[1], window, slots)
+    P.attention_mass(q, lse, case.cache, case.batch, got, mass_in=before, scale=scale, window=window, error_flag=case.error)
+    torch.cuda.synchronize()
+    # check_mass's bound, and what it leaves out: f32 has no normal number below 2^-126, so a term there may count as
+    # zero, and a slot is off by up to 2^-126 more for each row and head
+    for b, r, x, d, v in definition(case, q, scale, window):
+        n, kv, G = case.new[b], case.kv[b], q.shape[1] // case.kvh
+        seen = x > -math.inf
+        l = torch.where(seen, lse[r].double().T[..., None], 0.0)
+        p = torch.where(seen, torch.exp(x - l), 0.0)
+        err = p * (2 * d + 2.0 ** -20 * (1 + x.abs().masked_fill(~seen, 0) + l.abs())) + 2.0 ** -126
+        added = p.unflatten(0, (case.kvh, G)).sum((1, 2))
+        old = before[b, :, :kv].double()
+        old[:, max(0, kv - n):] = 0
+        want = old + added
+        tol = err.unflatten(0, (case.kvh, G)).sum((1, 2)) + added * U * (n * G + 8) + 2 * U * want
+        assert torch.all((got[b, :, :kv].double() - want).abs() <= tol), b
+    for b, k in enumerate(case.kv):
+        assert torch.all(got[b, :, k:] == 9.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,kv,heads,kv_heads,hd,ps,window,pad,extra", [
+    ([129, 7, 250], [2000, 900, 300], 5, 1, 64, 64, 0, 5, 20),
+    ([512], [3000], 2, 2, 40, 32, 0, 0, 70),
+    ([700, 1, 64], [2500, 40, 3000], 16, 2, 64, 16, 500, 3, 0),
+    ([300], [1300], 16, 2, 24, 128, 0, 1, 0),
+    ([333, 2], [5000, 700], 8, 1, 8, 8, 2000, 0, 0),
+    ([401], [2600], 9, 3, 104, 16, 0, 2, 0),
+    ([130, 0, 90], [3000, 17, 700], 256, 2, 64, 256, 0, 0, 0),    # 128 query heads share a kv head: one token a row tile
+    ([260], [1500], 65, 1, 128, 64, 0, 0, 0)])                    # 65: the second half of a row tile is nearly empty
+def test_tiles_by_shape(P, dtype, new, kv, heads, kv_heads, hd, ps, window, pad, extra):
+    case = Case(P, new, kv, kv_heads, hd, ps, dtype, seed=hd + len(new), pad=pad, heads_first=len(kv) == 1, extra=extra)
+    q = case.queries(heads)
+    assert by_tiles(P, case, heads, window)
+    workspace = P.attention_workspace()
+    out, lse = run_attention(P, case, q, window, workspace=workspace)
+    check_attention(case, q, out, lse, hd ** -0.5, window)
+    again, lse2 = run_attention(P, case, q, window, workspace=workspace)
+    assert torch.equal(out.nan_to_num(), again.nan_to_num()) and torch.equal(lse, lse2)
+    check_masses_by_tiles(P, case, q, lse, hd ** -0.5, window, max(kv) + 5)
+    assert int(case.error) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rising", [True, False])
+def test_tiles_with_a_moving_maximum(P, dtype, hd, rising):
+    """Every later key scores higher, so that each tile rescales the sums in tensor memory; or lower."""
+    case = Case(P, [150], [2000], kv_heads=1, hd=hd, dtype=dtype, fill=False, extra=240)
+    direction = rand(case.g, hd)
+    direction /= direction.norm()
+    ramp = torch.linspace(-30, 30, 2000, device="cuda")[:, None, None] * (1 if rising else -1)
+    case.keys = [(direction * ramp).to(dtype).reshape(2000, 1, hd)]
+    case.put(0, 0, case.keys[0], case.values[0])
+    q = case.queries(6)
+    q[:] = (direction * 40).to(dtype)
+    assert by_tiles(P, case, 6)
+    out, lse = run_attention(P, case, q, scale=0.1)
+    check_attention(case, q, out, lse, 0.1, 0)
+    check_masses_by_tiles(P, case, q, lse, 0.1, 0, 3000)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tiles_of_large_scores_and_constant_rows(P, dtype):
+    case = Case(P, [200, 200], [600, 601], dtype=dtype, extra=70)
+    q = case.queries(8, std=60.0)
+    q[100] = 0
+    assert by_tiles(P, case, 8)
+    out, lse = run_attention(P, case, q)
+    check_attention(case, q, out, lse, 128 ** -0.5, 0)
+
+
+@pytest.mark.parametrize("hd", [128, 72, 64, 40])
+@pytest.mark.parametrize("odd", [0, 8])
+def test_tiles_at_strides(P, hd, odd):
+    """q a slice of a fused projection, out a slice of a wider buffer, on 32-byte sectors or 16 bytes off them."""
+    heads = 12
+    case = Case(P, [180, 180], [300, 555], hd=hd, pad=1, extra=60)
+    fused = torch.full((case.rows, (heads + 4) * hd + odd), 3.0, dtype=case.dtype, device="cuda")
+    q = fused[:, odd:odd + heads * hd]
+    q.copy_(case.queries(heads).nan_to_num().reshape(case.rows, -1))
+    wide = torch.full((case.rows, (2 + heads) * hd + odd), 7.0, dtype=case.dtype, device="cuda")
+    out = wide[:, odd + hd:odd + (1 + heads) * hd].unflatten(1, (heads, hd))
+    assert by_tiles(P, case, heads)
+    out, lse = run_attention(P, case, q.unflatten(1, (heads, hd)), out=out)
+    check_attention(case, q.unflatten(1, (heads, hd)), out, lse, hd ** -0.5, 0)
+    assert torch.all(wide[:, :odd + hd] == 7.0) and torch.all(wide[:, odd + (1 + heads) * hd:] == 7.0)
+    assert torch.all(fused[:, :odd] == 3.0) and torch.all(fused[:, odd + heads * hd:] == 3.0)
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+def test_tiles_with_bad_pages(P, hd):
+    """Pages outside the pool read as zeros and are flagged, by attention and by the accumulated weight."""
+    case = Case(P, [140, 140], [400, 400], hd=hd, extra=300)
+    case.table[0, 3] = -5
+    case.table[1, 20] = case.k_pool.shape[0]
+    case.table[1, 24] = 2 ** 31 - 1
+    case.table[0, 25] = -1  # behind the keys: not read
+    for b, page in ((0, 3), (1, 20), (1, 24)):
+        case.keys[b][page * 16:page * 16 + 16] = 0
+        case.values[b][page * 16:page * 16 + 16] = 0
+    q = case.queries(8)
+    assert by_tiles(P, case, 8)
+    out, lse = run_attention(P, case, q)
+    check_attention(case, q, out, lse, hd ** -0.5, 0)
+    assert int(case.error) == P.ERROR_RANGE
+    case.error.zero_()
+    check_masses_by_tiles(P, case, q, lse, hd ** -0.5, 0, 2000)
+    assert int(case.error) == P.ERROR_RANGE
+
+
+@pytest.mark.parametrize("new,kv,extra", [([200], [60], 210), ([400, 3], [100, 0], 110)])
+def test_tiles_of_rows_before_the_first_slot(P, new, kv, extra):
+    case = Case(P, new, kv, extra=extra)
+    q = case.queries(8)
+    assert by_tiles(P, case, 8)
+    out, lse = run_attention(P, case, q)
+    check_attention(case, q, out, lse, 128 ** -0.5, 0)
+    check_masses_by_tiles(P, case, q, lse, 128 ** -0.5, 0, 16 * case.width)
+    assert int(case.error) == 0
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+def test_tiles_of_masses_shorter_than_the_keys(P, hd):
+    case = Case(P, [100, 100], [400, 150], hd=hd)
+    heads, new = 32, 100
+    q = case.queries(heads)
+    out, lse = run_attention(P, case, q)
+    before = torch.rand(2, 2, 170, device="cuda", generator=case.g)
+    got = torch.full_like(before, 9.0)
+    assert by_tiles(P, case, heads, slots=170)
+    P.attention_mass(q, lse, case.cache, case.batch, got, mass_in=before, error_flag=case.error)
+    wide = torch.full((2, 2, 400), 9.0, device="cuda")
+    wide[:, :, :170] = before
+    full = torch.full_like(wide, 9.0)
+    P.attention_mass(q, lse, case.cache, case.batch, full, mass_in=wide)
+    torch.cuda.synchronize()
+    assert int(case.error) == P.ERROR_RANGE
+    check_mass(case, q, lse, wide, full, hd ** -0.5, 0)
+    # sums of the same positive terms, 16 a token and `before`, in an order that the cut may change
+    assert torch.allclose(got, full[:, :, :170], rtol=2 * (16 * new + 8) * U, atol=0)
+    assert torch.all(got[1, :, 150:] == 9.0)
