@@ -18,6 +18,8 @@
 //    owns a column slice of one (sequence, head) and walks the rows in order,
 //    reading a whole step before it writes it: a row only moves to lower
 //    slots, so a step overwrites no later step's source.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace jfb {
@@ -247,15 +249,14 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
     // The new length may replace the old one that other CTAs still read: they
     // cut either to the same number of rows.
     if (head == 0 && (blockIdx.x & 1) == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.kv_len_out[b] = int32_t(kept);
-    const uint32_t begin = IN_PLACE ? 0u : blockIdx.y * step, end = IN_PLACE ? kept : min(kept, begin + step);
-    for (uint32_t row0 = begin; row0 < end; row0 += step) {
+    for (uint32_t row0 = blockIdx.y * step; row0 < kept; row0 += gridDim.y * step) {  // in place there is one y
         Piece x[PIECES];
         uint64_t dst[PIECES];
 #pragma unroll
         for (int u = 0; u < PIECES; ++u) {
             const uint32_t i = threadIdx.x + u * THREADS, r = i / width, c = (first + i - r * width) * Piece::kElements;
             dst[u] = ~0ull;
-            if (r < step && row0 + r < end) {
+            if (r < step && row0 + r < kept) {
                 const uint32_t at = row0 + r;
                 const uint32_t j = uint32_t(keep[at]);
                 const int32_t src_page = from[j >> v.page_shift], dst_page = to[at >> v.page_shift];
@@ -343,8 +344,9 @@ extern "C" jfb_status jfb_paged_evict(const float * mass, uint64_t mass_stride, 
     const bool sectors = !in_place && cache->head_dim % 16 == 0 && (cache->page_stride | cache->token_stride | cache->head_stride) % 16 == 0 &&
                          ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) & 31u) == 0;
     const uint32_t step = kFarThreads * kFarPieces / (sectors ? pieces / 2 : pieces);
-    const uint32_t steps = in_place ? 1u : (budget + step - 1) / step;
-    if (steps > 65535u) return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_evict: a budget of %u is too large", budget);
+    // a CTA for every step of the rows that a sequence can keep, as far as the grid goes
+    const uint64_t most = std::min({uint64_t(budget), uint64_t(batch->table_width) * cache->page_size, mass_stride});
+    const uint32_t steps = in_place ? 1u : uint32_t(std::min<uint64_t>((most + step - 1) / step, 65535u));
     cudaStream_t s = as_stream(stream);
     // Short lines: a small CTA, whose barriers are cheaper (one sequence of 700
     // keys, 2 kv heads: 9.3 us with both steps, 12 with 1024 threads).

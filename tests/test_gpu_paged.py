@@ -700,6 +700,45 @@ def test_evict_flags_bad_pages(P):
     assert torch.equal(case.k_pool[spare[1]].view(torch.int16), before[spare[1]].view(torch.int16))  # not moved
 
 
+@pytest.mark.parametrize("kv,budget", [(500, 1100000), (1100000, 1060000)])
+def test_evict_with_a_budget_beyond_the_grid(P, kv, budget):
+    """Out of place, a budget of more steps than a grid has rows: of a short sequence, and of one that fills it."""
+    g = torch.Generator(device="cuda").manual_seed(budget)
+    ps, hd, room = 1024, 128, 136  # rows of 16-byte pieces that are not whole 32-byte sectors
+    old, new = -(-kv // ps), -(-min(kv, budget) // ps)
+    store = torch.empty(2, old + new, ps, 1, room, dtype=torch.float16, device="cuda")
+    for pool in store:
+        for page in pool:
+            page.copy_(torch.randn(page.shape, device="cuda", generator=g))
+    k_pool, v_pool = store[0, ..., :hd], store[1, ..., :hd]
+    table = torch.randperm(old + new, generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    width = -(-budget // ps)
+    new_table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")  # pages that nothing is kept in are not read
+    new_table[0, :new] = table[old:]
+    kv_len = torch.tensor([kv], dtype=torch.int32, device="cuda")
+    cache = P.PagedCache(k_pool, v_pool)
+    batch = P.PagedBatch(torch.zeros(2, dtype=torch.int32, device="cuda"), kv_len, table[None, :old].contiguous())
+    mass = torch.randint(0, 1000, (1, 1, kv), device="cuda", generator=g).float()
+    keep = torch.empty(1, 1, budget, dtype=torch.int32, device="cuda")
+    length, mass_out = torch.empty_like(kv_len), torch.zeros(1, 1, budget, device="cuda")
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    P.evict(mass, cache, batch, keep, length, recent=100, mass_out=mass_out, page_table_out=new_table, error_flag=error)
+    torch.cuda.synchronize()
+    kept = min(kv, budget)
+    assert int(length) == kept and int(error) == 0
+    if kv > budget:
+        early = torch.sort(mass[0, 0, :kv - 100], descending=True, stable=True).indices[:budget - 100]
+        want = torch.cat((torch.sort(early).values, torch.arange(kv - 100, kv, device="cuda")))
+    else:
+        want = torch.arange(kv, device="cuda")
+    assert torch.equal(keep[0, 0, :kept].long(), want) and torch.all(keep[0, 0, kept:] == -1)
+    assert torch.equal(mass_out[0, 0, :kept], mass[0, 0, want])
+    at = torch.arange(kept, device="cuda")
+    for pool in (k_pool, v_pool):
+        source = pool[table[want // ps].long(), want % ps, 0]
+        assert torch.equal(pool[new_table[0, at // ps].long(), at % ps, 0], source)
+
+
 # ---- as they are used together ----------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
