@@ -187,9 +187,11 @@ jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride, uint32_t 
  * mass_out [sequences][kv_heads][mass_out_stride] (>= budget). keep
  * [sequences][kv_heads][budget] receives the kept slots in order, -1 behind
  * them, and kv_len_out [sequences] the new lengths, min(kv_len, budget).
- * page_table_out is either the batch's own page_table (the compaction is in
- * place; mass_out may be mass, kv_len_out kv_len) or shares no page with it;
- * either way no page stands in it twice.
+ * page_table_out is either the batch's own page_table, the same address (the
+ * compaction is in place; mass_out may be mass, kv_len_out kv_len), or shares
+ * no page with it; either way no page stands in it twice. A copy of the batch's
+ * table is neither: nothing is moved for a sequence whose first page is its own
+ * (error bit 0).
  * A length beyond the table or mass_stride is cut to it; a kept row with a
  * page id outside the pool on either side is not moved (error bit 0). The
  * batch's q_start is not read. */

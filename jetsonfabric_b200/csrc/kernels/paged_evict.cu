@@ -246,6 +246,10 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
     const uint32_t width = v.head_dim / Piece::kElements / p.slices, first = blockIdx.z * width;  // pieces of a row
     const uint32_t step = THREADS * PIECES / width;                                  // rows read before they are written
     const uint32_t kept = min(evict_length(p, b), p.budget);
+    // Out of place the CTAs move in no order: through a copy of the batch's own
+    // table they would read what others wrote. Its first page tells (every row's
+    // page would cost 3 us of 65).
+    const bool copied = !IN_PLACE && to[0] == from[0];
     // The new length may replace the old one that other CTAs still read: they
     // cut either to the same number of rows.
     if (head == 0 && (blockIdx.x & 1) == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.kv_len_out[b] = int32_t(kept);
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) move_kernel(const EvictParams p) {
                 const uint32_t at = row0 + r;
                 const uint32_t j = uint32_t(keep[at]);
                 const int32_t src_page = from[j >> v.page_shift], dst_page = to[at >> v.page_shift];
-                if (src_page >= 0 && uint32_t(src_page) < v.pages && dst_page >= 0 && uint32_t(dst_page) < v.pages) {
+                if (!copied && src_page >= 0 && uint32_t(src_page) < v.pages && dst_page >= 0 && uint32_t(dst_page) < v.pages) {
                     const uint64_t in = uint64_t(head) * v.head_stride + c;
                     dst[u] = uint64_t(dst_page) * v.page_stride + (at & (v.page_size - 1)) * v.token_stride + in;
                     const uint64_t src = uint64_t(src_page) * v.page_stride + (j & (v.page_size - 1)) * v.token_stride + in;

@@ -325,8 +325,10 @@ def evict(mass, cache: PagedCache, batch: PagedBatch, keep, kv_len_out, recent: 
     and the heaviest others, ties to the lowest slot (jfb_paged_evict). keep int32
     [sequences, kv_heads, budget] receives the kept slots, kv_len_out [sequences]
     the new lengths. Without mass_out the masses move in place, without
-    page_table_out (which must share no page with the batch's) the cache does; no
-    page may then belong to two sequences."""
+    page_table_out the cache does; no page may then belong to two sequences.
+    page_table_out is the batch's own tensor (in place) or shares no page with
+    it: a copy of the batch's table would have rows overwrite others that are
+    still to be moved, so nothing is moved then and the error flag is set."""
     _on(batch, cache)
     slots = _masses(mass, batch, cache, "mass")
     mass_out = mass if mass_out is None else mass_out

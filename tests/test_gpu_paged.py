@@ -700,6 +700,21 @@ def test_evict_flags_bad_pages(P):
     assert torch.equal(case.k_pool[spare[1]].view(torch.int16), before[spare[1]].view(torch.int16))  # not moved
 
 
+@pytest.mark.parametrize("hd", [128, 24])
+def test_evict_refuses_a_copy_of_the_table(P, hd):
+    """Out of place within a sequence's own pages: nothing is moved, and the call says so."""
+    case = Case(P, [0, 0], [3000, 40], hd=hd)
+    mass = torch.rand(2, 2, 3000, device="cuda", generator=case.g)
+    before_k, before_v = case.k_pool.clone(), case.v_pool.clone()
+    keep = torch.empty(2, 2, 1000, dtype=torch.int32, device="cuda")
+    P.evict(mass, case.cache, case.batch, keep, torch.empty_like(case.kv_len), recent=10, mass_out=torch.empty(2, 2, 1000, device="cuda"),
+            page_table_out=case.table.clone(), error_flag=case.error)
+    torch.cuda.synchronize()
+    assert int(case.error) == P.ERROR_RANGE
+    assert torch.equal(case.k_pool.view(torch.int16), before_k.view(torch.int16))
+    assert torch.equal(case.v_pool.view(torch.int16), before_v.view(torch.int16))
+
+
 @pytest.mark.parametrize("kv,budget", [(500, 1100000), (1100000, 1060000)])
 def test_evict_with_a_budget_beyond_the_grid(P, kv, budget):
     """Out of place, a budget of more steps than a grid has rows: of a short sequence, and of one that fills it."""
