@@ -557,6 +557,10 @@ extern "C" jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uin
         return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention needs a positive scale up to 1e38 and a window below 2^31");
     }
     if (rows == 0 || batch->sequences == 0) return status_ok();
+    // one item's results would replace queries that another has still to read
+    if (rows_overlap(q, q_stride, out, out_stride, rows, uint64_t(heads) * cache->head_dim)) {
+        return status_error(JFB_STATUS_INVALID_ARGUMENT, "jfb_paged_attention: q and out overlap");
+    }
     const Device device = current_device();
     const uint32_t sms = device.sms;
     if (sms == 0 || sms * 2 * sizeof(uint32_t) > kCounterBytes) {

@@ -117,6 +117,17 @@ extern "C" int jfb_paged_attention_mass_uses_tiles(uint32_t rows, uint32_t heads
 jfb_status launch_attention_tc(const jfb_paged_cache & cache, const CUtensorMap & k, const CUtensorMap & v, AttentionParams p,
                                const Device & device, cudaStream_t s);
 
+// Whether rows of `width` 16-bit elements at two strides share bytes: in an
+// address range that both lie in, slices of wider rows of one stride need not.
+inline bool rows_overlap(const void * a, uint64_t a_stride, const void * b, uint64_t b_stride, uint32_t rows, uint64_t width) {
+    if (rows == 0) return false;
+    const uint64_t x = reinterpret_cast<uintptr_t>(a) / 2, y = reinterpret_cast<uintptr_t>(b) / 2;
+    if (x + (rows - 1) * a_stride + width <= y || y + (rows - 1) * b_stride + width <= x) return false;
+    if (a_stride != b_stride) return true;
+    const uint64_t apart = (x > y ? x - y : y - x) % a_stride;
+    return apart < width || a_stride - apart < width;
+}
+
 // Query-shaped rows [rows][heads x head_dim] of 16-bit numbers.
 inline jfb_status check_rows(const char * what, const void * x, uint64_t stride, uint32_t rows, uint32_t heads,
                              const jfb_paged_cache & c) {

@@ -180,6 +180,17 @@ def test_attention_refusals(P, call, bad):
     refused(call(P, cache(P), batch(P), **bad))
 
 
+@pytest.mark.parametrize("q,qs,out,os,rows,overlap", [
+    (A, 512, A, 512, 3, True), (A, 512, A + 16, 512, 1, True), (A, 512, A + 1024, 512, 3, True), (A, 512, A + 3072, 512, 3, False),
+    (A + 3072, 512, A, 512, 3, False), (A + 3056, 512, A, 512, 3, True), (A, 512, A + 1024, 512, 1, False),
+    (A, 1024, A + 1024, 1024, 3, False), (A + 1024, 1024, A, 1024, 3, False), (A, 1024, A + 1008, 1024, 3, True),  # slices of one buffer
+    (A, 1024, A + 1040, 1024, 3, True), (A, 1024, A + 1040, 1024, 1, False), (A, 1032, A + 1024, 1024, 3, True)])
+def test_attention_refuses_out_over_q(P, q, qs, out, os, rows, overlap):
+    st = attention_call(P, cache(P), batch(P), q=q, qs=qs, out=out, os=os, rows=rows)
+    # what passes is refused for its missing workspace, or for the missing device
+    assert st.code != 0 and (b"overlap" in st.message if isinstance(st.message, bytes) else "overlap" in st.message) == overlap
+
+
 @pytest.mark.parametrize("bad", [dict(lse=None), dict(slots=0)])
 def test_mass_refusals(P, bad):
     refused(mass_call(P, cache(P), batch(P), **bad))
