@@ -227,7 +227,9 @@ __global__ void __launch_bounds__(kThreadsMass, 1)
     }
     __syncthreads();
     KeyTileWalk & w = walks[warp];
-    const bool work = w.unit < w.end && (smem_u32(smem) & 1023u) == 0;
+    const bool aligned = (smem_u32(smem) & 1023u) == 0;  // the swizzled tiles need it
+    const bool work = w.unit < w.end && aligned;
+    if (!aligned && threadIdx.x == 0) flag_error(v.error, JFB_PAGED_ERROR_TIMEOUT);
     // rows that no query fills stay zero (and this may have held the walk's scratch)
     for (uint32_t i = threadIdx.x; i < L::kRows / 16; i += kThreadsMass) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
