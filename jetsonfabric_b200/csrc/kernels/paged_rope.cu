@@ -11,7 +11,7 @@
 // (one when few rows would leave SMs idle), its threads 16-byte vectors: both
 // partners of 8 pairs (half layout) or a run of 8 elements. Sixteen small CTAs
 // an SM keep more loads in flight than several items per thread did (2, 4 and 8
-// of them: 63, 73 and 89 us against 55 for 16192 rows of 36 heads, bf16, 5.5
+// of them: 63, 73 and 89 us against 55 for 16192 rows of 36 heads, bf16, 5.4
 // TB/s). Rows or rotations that are not made of 8-element runs take an
 // element-wise form.
 #include <cmath>
@@ -392,8 +392,11 @@ extern "C" jfb_status jfb_rope_paged_append(const void * q, const void * k, cons
     p.heads = heads;
     p.rope_dims = dims;
     p.factor = rope->factor;
-    // few rows: one per CTA, to fill the SMs; many: four share the work of finding their sequences and angles (110 us with one)
-    p.rows_per_cta = rows >= 8u * 148u * kMaxRows ? kMaxRows : 1;
+    // Few rows: one per CTA, to fill the SMs; many: four share the work of finding their sequences and angles, and leave
+    // fewer threads idle where a row has few heads. One / four, in us, for 12/2 heads (f32 in), 28/4 (bf16), 40/8 (f32):
+    // 1000 rows 6.8/8.8, 10.0/13.9, 13.1/19.5; 2000 10.2/12.3, 11.4/16.1, 19.9/24.5; 4000 14.7/14.6, 18.6/21.3, 33.0/37.1;
+    // 6000 19.2/15.8, 25.7/28.0, 45.1/46.7; 8000 23.9/23.2, 32.2/31.3, 57.5/65.2; 16192 42.0/37.4, 56.1/56.4, 108/113.
+    p.rows_per_cta = rows >= 8u * current_device().sms * kMaxRows ? kMaxRows : 1;
     const bool inter = rope->interleaved != 0;
     // 16-byte vectors: runs of 8 elements on both sides of every pair, aligned rows
     const bool vec = (inter ? dims % 8 == 0 : dims % 16 == 0) && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) &&
