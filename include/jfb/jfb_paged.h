@@ -190,8 +190,8 @@ jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride, uint32_t 
  * page_table_out is either the batch's own page_table, the same address (the
  * compaction is in place; mass_out may be mass, kv_len_out kv_len), or shares
  * no page with it; either way no page stands in it twice. A copy of the batch's
- * table is neither: nothing is moved for a sequence whose first page is its own
- * (error bit 0).
+ * table is neither: a sequence whose first page stays its own keeps its rows
+ * where they are (error bit 0 if it is cut).
  * A length beyond the table or mass_stride is cut to it; a kept row with a
  * page id outside the pool on either side is not moved (error bit 0). The
  * batch's q_start is not read. */

@@ -715,6 +715,25 @@ def test_evict_refuses_a_copy_of_the_table(P, hd):
     assert torch.equal(case.v_pool.view(torch.int16), before_v.view(torch.int16))
 
 
+def test_evict_leaves_uncut_sequences_on_their_pages(P):
+    """A sequence within the budget may keep its pages while another moves to new ones."""
+    case = Case(P, [0, 0], [300, 40], extra=7)
+    mass = torch.rand(2, 2, 300, device="cuda", generator=case.g)
+    weights = mass.cpu().tolist()
+    table = case.table[:, :7].clone()
+    table[0] = case.table[0, 19:26]
+    keep, length = torch.empty(2, 2, 100, dtype=torch.int32, device="cuda"), torch.empty_like(case.kv_len)
+    P.evict(mass, case.cache, case.batch, keep, length, recent=10, mass_out=torch.empty(2, 2, 100, device="cuda"),
+            page_table_out=table, error_flag=case.error)
+    torch.cuda.synchronize()
+    assert int(case.error) == 0 and length.tolist() == [100, 40]
+    for b, h in ((0, 0), (0, 1), (1, 0), (1, 1)):
+        want = torch.tensor(kept_slots(weights[b][h], case.kv[b], 100, 10)).cuda()
+        slot = torch.arange(len(want), device="cuda")
+        assert torch.equal(case.k_pool[table[b, slot // 16].long(), slot % 16, h], case.keys[b][want, h])
+        assert torch.equal(case.v_pool[table[b, slot // 16].long(), slot % 16, h], case.values[b][want, h])
+
+
 @pytest.mark.parametrize("kv,budget", [(500, 1100000), (1100000, 1060000)])
 def test_evict_with_a_budget_beyond_the_grid(P, kv, budget):
     """Out of place, a budget of more steps than a grid has rows: of a short sequence, and of one that fills it."""
