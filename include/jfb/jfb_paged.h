@@ -138,7 +138,8 @@ jfb_status jfb_rope_paged_append(const void * q, const void * k, const void * v,
 
 /* Workspace of jfb_paged_attention on the current device: one size for every
  * shape. Zero-filled before its first use; every call that completes leaves
- * it ready for the next. Calls that overlap on the GPU need one each. */
+ * it ready for the next, after error bit 1 it is zero-filled again. Calls that
+ * overlap on the GPU need one each. */
 uint64_t jfb_paged_attention_workspace_bytes(void);
 
 /* Attention of the batch's rows over their sequences' keys. Row r of sequence
@@ -146,7 +147,7 @@ uint64_t jfb_paged_attention_workspace_bytes(void);
  *     x_j = scale * q . k_j,   out = sum_j exp(x_j - lse) v_j,
  *     lse = log sum_j exp(x_j).
  * scale is positive, up to 1e38. Query head h reads kv head
- * h / (heads / kv_heads). q and out do not overlap; they have the
+ * h / (heads / kv_heads). q and out do not overlap (refused); they have the
  * cache's dtype, rows of heads x head_dim at their strides (elements,
  * multiples of 8, 16-byte aligned pointers); lse (may be NULL) is f32
  * [rows][heads]. Scores, the softmax's maximum and sum and the output sums are
@@ -158,7 +159,10 @@ uint64_t jfb_paged_attention_workspace_bytes(void);
  * row of a sequence's chunk sees must hold finite values of v (a non-finite one
  * may reach rows of the chunk that do not see it). A page id outside the pool
  * reads as zeros, a length beyond the table is cut to it (error bit 0). Results
- * do not depend on timing: partial sums are joined in a fixed order. */
+ * do not depend on timing: partial sums are joined in a fixed order. One kernel
+ * is chosen for all sequences of the call, by the mean of their rows and the
+ * width of the table: single tokens and long chunks are faster in calls of
+ * their own. */
 jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uint32_t rows, uint32_t heads, float scale,
                                uint32_t window, const jfb_paged_cache * cache, const jfb_paged_batch * batch,
                                void * out, uint64_t out_stride, float * lse, void * workspace,
@@ -171,9 +175,10 @@ jfb_status jfb_paged_attention(const void * q, uint64_t q_stride, uint32_t rows,
  * mass_in[b][h][j] for the slots the sequence held before this call, and 0
  * for its new tokens' slots or when mass_in is NULL. Both are f32
  * [sequences][kv_heads][mass_stride]; mass_in may be mass_out. Slots at and
- * behind kv_len are left as they were. Sums are f32, in a fixed order. A length
- * beyond mass_stride or the table is cut to it, a page id outside the pool
- * reads as zeros (error bit 0). */
+ * behind kv_len are left as they were. Sums are f32, in a fixed order; a weight
+ * below 2^-126 counts as zero. A length beyond mass_stride or the table is cut
+ * to it, a page id outside the pool reads as zeros (error bit 0). The kernel is
+ * chosen as for the attention. */
 jfb_status jfb_paged_attention_mass(const void * q, uint64_t q_stride, uint32_t rows, uint32_t heads, float scale,
                                     uint32_t window, const float * lse, const jfb_paged_cache * cache,
                                     const jfb_paged_batch * batch, const float * mass_in, float * mass_out,

@@ -31,7 +31,7 @@ namespace {
 // A part of an item that began in another CTA is published by a warp of its
 // own, so that the consumers go on to their next item at once.
 //
-// 6 sequences of 9001 to 65001 keys, 28/4 heads: 79 us (88 % of the measured
+// 6 sequences of 9001 to 65001 keys, 28/4 heads: 82 us (84 % of the measured
 // copy bandwidth); 64 of 1025 to 1280: 37 us (63 %), of which the way to the
 // first tile and the ends are a third.
 
@@ -532,9 +532,18 @@ extern "C" uint64_t jfb_paged_attention_workspace_bytes(void) {
 // and end, the other 16: from 2 row tiles of 16 a sequence on, if there is work
 // for it, counted in (16 rows, 128 keys) tiles of the keys that the table can
 // hold. Rows kernel / tcgen05 kernel at 28/4 heads, in us: 64 sequences of
-// 1025 to 1280 keys with 2, 4, 6, 8 new tokens 39/58, 64/58, 89/58, 112/59;
-// one of 1000 keys with 8, 16, 48 tokens 13/24, 13/24, 19/26 (672 tiles); 4 of them with
-// 16, 24, 48: 20/21, 25/26, 40/26 (2688); one of 8000 with 8, 16, 48: 21/32, 28/33, 54/42 (5292).
+// 1025 to 1280 keys with 2, 4, 6, 8 new tokens 39/50, 64/50, 88/51, 113/52;
+// one of 1000 keys with 8, 16, 48 tokens 13/20, 13/20, 19/24 (672 tiles); 4 of them with
+// 16, 24, 40, 48: 20/20, 24/22, 33/24 (2240), 40/24 (2688); one of 8000 with 8, 16, 48: 21/32,
+// 28/32, 54/41 (5292). The few-rows kernel is kept where that is not much.
+//
+// The host knows neither the lengths nor how the rows divide among the
+// sequences (a captured call serves others). So the keys are the table's width,
+// which costs a short context in a wide table up to the difference above (one
+// of 1000 keys with 8 tokens: 13 us, 20 in a table 128 times as wide), and one
+// kernel serves all sequences by their mean: 63 single tokens (37 us by
+// themselves) with a chunk of 220 over 8000 keys (50) take 258 us on the
+// few-rows kernel, with one of 512 (70) 108 on the other.
 extern "C" int jfb_paged_attention_uses_tiles(uint32_t rows, uint32_t heads, uint32_t window, const jfb_paged_cache * cache,
                                               const jfb_paged_batch * batch) {
     const uint32_t group = heads / cache->kv_heads;

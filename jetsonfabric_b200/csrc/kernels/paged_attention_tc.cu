@@ -27,9 +27,13 @@
 // one its sums refer to (the sums stay far inside f32's range, the probabilities
 // inside their type's), so most tiles touch O not at all.
 //
-// The exponentials bound the time: 2048 cycles of their unit for the two row
-// tiles of a key tile, 1024 of the tensor pipe. A prompt of 8192 at 28/4 heads takes 411 us
-// (1170 TFLOP/s of the measured 1665), at the power cap's 1.6 GHz or so.
+// Two row tiles of a key tile need the tensor pipe (four products of 128 x 128
+// x 128 at 8192 operations a cycle) and the exponentials' unit (16 a cycle) for
+// 2048 cycles each: neither alone bounds the time, but a row tile's products and
+// exponentials follow one another, and with one S between the two row tiles they
+// overlap only in part. A prompt of 8192 at 28/4 heads, 397,000 cycles of both
+// (209 us at 1.9 GHz), takes 426 us after a pause and 471 to 478 (1010 TFLOP/s
+// of the measured 1665) in long runs, where the power cap leaves 1.62 GHz.
 #include "paged_attention.cuh"
 #include "paged_tc.cuh"
 

@@ -253,9 +253,15 @@ using namespace jfb::paged;
 // The tcgen05 kernel from 2 row tiles of 16 a sequence on, if there is work for
 // it, counted in (16 rows, 128 keys) tiles of the keys that the table and the
 // masses can hold. Rows kernel / tcgen05 kernel at 28/4 heads, in us: 64
-// sequences of 1150 keys with 4, 8, 16 new tokens 58/86, 99/86, 185/87; 4 of
-// them with 8, 16, 40: 11/16, 16/16 (1008 tiles), 31/19; one of 8000 with 4, 8, 16:
-// 11/15 (441), 16/15 (882), 26/15.
+// sequences of 1150 keys with 4, 8, 16 new tokens 58/84, 99/84, 185/85; 4 of 1000
+// with 8, 16, 40: 11/14, 16/14 (896 tiles), 31/18; one of 1000 with 16, 48: 15/14, 35/14
+// (672); one of 8000 with 4, 8, 16: 11/14 (504), 16/14 (1008), 26/14.
+//
+// As for the attention, the keys are those the arrays can hold and the rows
+// those of the mean sequence: 63 single tokens (23 us by themselves) with a
+// chunk of 220 over 8000 keys (35) take 2490 us here, where the chunk's rows go
+// through each key tile 16 at a time on the one CTA that holds it; with one of
+// 512 (58) 267 on the tcgen05 kernel.
 extern "C" int jfb_paged_attention_mass_uses_tiles(uint32_t rows, uint32_t heads, const jfb_paged_cache * cache,
                                                    const jfb_paged_batch * batch, uint64_t mass_stride) {
     const uint32_t group = heads / cache->kv_heads;
