@@ -181,8 +181,8 @@ def test_attention_refusals(P, call, bad):
 
 
 @pytest.mark.parametrize("q,qs,out,os,rows,overlap", [
-    (A, 512, A, 512, 3, True), (A, 512, A + 16, 512, 1, True), (A, 512, A + 1024, 512, 3, True), (A, 512, A + 3072, 512, 3, False),
-    (A + 3072, 512, A, 512, 3, False), (A + 3056, 512, A, 512, 3, True), (A, 512, A + 1024, 512, 1, False),
+    (A, 512, A, 512, 3, True), (A, 512, A + 16, 512, 1, True), (A, 512, A + 1024, 512, 3, True), (A, 512, A + 5120, 512, 5, False),
+    (A + 5120, 512, A, 512, 5, False), (A + 5104, 512, A, 512, 5, True), (A, 512, A + 1024, 512, 1, False),
     (A, 1024, A + 1024, 1024, 3, False), (A + 1024, 1024, A, 1024, 3, False), (A, 1024, A + 1008, 1024, 3, True),  # slices of one buffer
     (A, 1024, A + 1040, 1024, 3, True), (A, 1024, A + 1040, 1024, 1, False), (A, 1032, A + 1024, 1024, 3, True)])
 def test_attention_refuses_out_over_q(P, q, qs, out, os, rows, overlap):
